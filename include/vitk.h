@@ -201,6 +201,66 @@ int vitk_window_attn_bwd(const void* qkv, const float* bias_table, const void* o
                          int B, int H, int W, int heads, int dh, int window, int shift, float scale,
                          int dtype, void* stream);
 
+/* ---- Attention with a sliding window and first tokens that stay visible (no counterpart in the reference) ----
+ * Of a sequence of n tokens, query i sees key j when
+ *   causal != 0:  j <= i and (i - j < window or j < sinks)
+ *   causal == 0:  |i - j| < window or j < sinks or i < sinks   (the first tokens see all and are seen by all)
+ * o = softmax(scale q.k^T over the visible keys) v; a query that sees nothing gives 0.  q:[B, N, Hq, dh], k, v:[B, N, Hkv, dh]
+ * with element strides *_b, *_n, *_h and consecutive elements inside a head; query head h reads key head h / (Hq / Hkv).
+ * lengths:[B] int32 on the device (NULL: N tokens each): tokens behind a sequence's length are neither read as keys nor
+ * computed as queries, whatever memory holds there; their outputs and gradients are written as 0.
+ * o:[B, N, Hq, dh] contiguous.  For a backward pass: lse:[B, Hq, N] (base-2 logarithm of each row's sum, +inf for a row
+ * that sees nothing) and, in bf16, o_f32 (o unrounded, contiguous), both NULL without one.
+ * vitk_slide_attn_bwd reads q, k, v, d_o, lse, o_f32 (fp32: o) and writes dq, dk, dv (strided; dq, or dk and dv together,
+ * may be NULL: not wanted); delta:[B, Hq, N] is workspace.  Sums have a fixed order: equal inputs give equal bits.
+ * dh 32, 64 or 128; every pointer 16-byte aligned, every stride a multiple of 16 bytes; Hq % Hkv == 0; window, sinks >= 0;
+ * scale > 0. */
+typedef struct vitk_slide_attn {
+    const void* q; const void* k; const void* v;
+    void* o; float* o_f32; float* lse;
+    const int* lengths;
+    const void* d_o; float* delta;
+    void* dq; void* dk; void* dv;
+    long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
+    long do_b, do_n, do_h, dq_b, dq_n, dq_h, dk_b, dk_n, dk_h, dv_b, dv_n, dv_h;
+    int B, N, Hq, Hkv, dh;
+    int window, sinks, causal;
+    float scale;
+} vitk_slide_attn;
+int vitk_slide_attn_fwd(const vitk_slide_attn* a, int dtype, void* stream);
+int vitk_slide_attn_bwd(const vitk_slide_attn* a, int dtype, void* stream);
+/* One query per sequence, the last of its lengths[b] cached tokens: it sees j < sinks and j >= lengths[b] - window.
+ * q:[B, Hq, dh], o:[B, Hq, dh] contiguous, k, v:[B, cap, Hkv, dh] strided; a sequence of length 0 gives 0.
+ * The visible keys are shared out over `splits` workgroups per (sequence, key head), 1 <= splits <= 1024; with more than
+ * one, workspace holds B * Hq * splits * (dh + 2) floats. */
+typedef struct vitk_slide_cache {
+    const void* q; const void* k; const void* v; void* o;
+    const int* lengths;
+    float* workspace;
+    long q_b, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
+    int B, cap, Hq, Hkv, dh;
+    int window, sinks, splits;
+    float scale;
+} vitk_slide_cache;
+int vitk_slide_decode(const vitk_slide_cache* a, int dtype, void* stream);
+
+/* ---- Rotary positions with several axes (no counterpart in the reference) ----
+ * Each head of dh elements holds P = pairs[0] + ... + pairs[axes-1] <= dh / 2 pairs, (i, i + P) or, interleaved,
+ * (2 i, 2 i + 1); the rest of the head is copied.  Pair i of axis a turns by pos[token][a] * base^(-i / pairs[a]),
+ * backwards when `inverse` (the gradient).  Angles are reduced to one turn in 64 bits.
+ * x, y:[B, N, H, dh] in `dtype` with element strides and consecutive elements inside a head (y may be x);
+ * pos: pos_kind 0 int64, 1 int32, 2 fp32, 3 fp64, [N, axes] with rows of `axes` elements, pos_b elements from one sequence to the
+ * next (0: shared).  dh even, <= 256; 1 <= axes <= 8. */
+typedef struct vitk_rope {
+    const void* x; void* y; const void* pos;
+    long x_b, x_n, x_h, y_b, y_n, y_h, pos_b;
+    int B, N, H, dh;
+    int axes, pos_kind, interleaved, inverse;
+    int pairs[8];
+    double base;
+} vitk_rope;
+int vitk_axial_rope(const vitk_rope* a, int dtype, void* stream);
+
 /* RKR weight fold (models/ViT/modeling_RKR.py:56-78 RG_FC.forward + SFG_FC.forward moved to the weight side):
  * Wt[o][i] = (W[o][i] + sum_k RM[k][o] LM[i][k]) * F[o], bt[o] = b[o] * F[o]; W:[O,I], LM:[I,K], RM:[K,O],
  * F:[O] or NULL (no scale); all fp32; K <= 8, I % 4 == 0.  vitk_rkr_fold_bwd turns dWt, dbt into the
@@ -350,6 +410,33 @@ int vitk_sgd_norm_sq(const void* table, int n_entries, int n_blocks, float* slot
  * mom = first ? g' : momentum*mom + (1 - dampening)*g';  param -= lr*mom.  Gradients are left as they are. */
 int vitk_sgd_step(const void* table, int n_entries, int n_blocks, const float* slots, float max_norm,
                   float lr, float momentum, float dampening, float weight_decay, void* stream);
+
+/* ---- AdamW over many tensors (no counterpart in the reference, whose loop uses SGD) ----
+ * A device-resident table as above (block0 counts blocks of 8192 elements; a call on a later part of a table counts from
+ * its first entry's block0); all tensors fp32 except 8-bit states.
+ * flags: bit 0 = the states hold nothing yet and are taken as zero; bit 1 = every pointer of the entry allows 16-byte
+ * (8-bit states: 4-byte) accesses.
+ * state_bits 32: m, v fp32 [n].  state_bits 8: m, v e4m3 codes [n], m_scale, v_scale fp32 [ceil(n / 256)]: an element of
+ * the first moment is code * scale, of the second (code * scale)^2. */
+typedef struct vitk_adamw_entry {
+    void* param; void* grad; void* m; void* v;
+    float* m_scale; float* v_scale;
+    long n;
+    int block0;
+    int flags;
+} vitk_adamw_entry;
+/* slots (device, VITK_ADAMW_SLOTS doubles owned by the caller): slots[0] := sum of squares of every gradient in the
+ * table, in 64 bits and in a fixed order; norm (device, may be NULL) := its root. */
+#define VITK_ADAMW_SLOTS (1 + 1024)
+int vitk_adamw_norm(const void* table, int n_entries, int n_blocks, double* slots, float* norm, void* stream);
+/* g = coef * grad, coef = slots ? min(1, max_norm / (sqrt(slots[0]) + 1e-6)) : 1
+ * m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ * param = param (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * `step` counts from 1.  Eight-bit states are rounded at random from the word of (seed, step, element): the expectation
+ * of what is held is the moment itself. */
+int vitk_adamw_step(const void* table, int n_entries, int n_blocks, const double* slots, double max_norm, double lr,
+                    double beta1, double beta2, double eps, double weight_decay, long step, int state_bits, uint32_t seed,
+                    void* stream);
 
 /* ---- Gradient exchange (DistributedDataParallel at train.py:274-278: broadcast at wrap time, mean
  * all-reduce of every gradient inside loss.backward() at train.py:528) ----

@@ -1,0 +1,294 @@
+// AdamW over a table of tensors: one pass for the gradients' norm, one for the update.
+//
+//   coef = min(1, max_norm / (|g| + 1e-6));  g' = coef g
+//   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// HBM-bound: 4 bytes of every parameter for the norm, then 28 (states in 32 bits) or 16 + 4/256 (in 8).
+//
+// States in 8 bits are e4m3 codes in units of a scale that 256 consecutive elements share (largest value / 448); the
+// second moment is held as its root, which halves the range that the code has to span.  A code's neighbours are 1/16 to
+// 1/8 of it apart and the second moment moves by a thousandth per step: rounded to nearest it would never move.  So
+// codes are rounded at random, m in proportion to its distance from the two neighbours and v in proportion to the
+// distance of their SQUARES (in proportion to the roots, E[v] would grow by the variance of the root at each step, more
+// than the 1 - b2 that pulls it back).  A root that is not zero is never held as zero: the next step would divide by eps.
+// The update itself uses the moments before they are rounded.  Nothing below is contracted, and
+// sums have a fixed order, so codes, scales and parameters are the same bits wherever the same inputs are.
+#include "common.h"
+
+namespace {
+
+#pragma clang fp contract(off)
+
+constexpr int CHUNK = 8192;              // elements of a workgroup
+constexpr int BLOCK = 256;               // elements that share a scale: one wave, four each
+constexpr int PARTIALS = 1024;
+static_assert(1 + PARTIALS == VITK_ADAMW_SLOTS, "slots layout");
+constexpr float TOP = 448.f;             // largest e4m3 value
+
+struct Entry {                           // mirrors vitk_adamw_entry
+    float* p; const float* g; void* m; void* v; float* ms; float* vs;
+    long n;
+    int block0;
+    int flags;
+};
+static_assert(sizeof(Entry) == sizeof(vitk_adamw_entry), "table layout");
+
+struct Consts { float b1, c1, b2, c2, decay, step, root, eps; double max_norm; uint32_t key; };
+
+__device__ __forceinline__ int find(const Entry* tab, int n, int block) {
+    int lo = 0, hi = n - 1;              // last entry with block0 <= block
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab[mid].block0 <= block) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ double block_sum(double s) {
+    __shared__ double part[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__global__ __launch_bounds__(256) void adamw_norm_kernel(const Entry* tab, int n, int n_blocks, double* partial) {
+    double s = 0.0;
+    for (int blk = blockIdx.x; blk < n_blocks; blk += gridDim.x) {     // always in this order
+        const Entry en = tab[find(tab, n, blk)];
+        const long base = (long)(blk - en.block0) * CHUNK;
+        const int cnt = en.n - base < CHUNK ? (int)(en.n - base) : CHUNK;
+        const float* g = en.g + base;
+        const int whole = en.flags & 2 ? cnt & ~3 : 0;
+        for (int i = threadIdx.x * 4; i < whole; i += 1024) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(g + i);
+            s += ((double)x[0] * x[0] + (double)x[1] * x[1]) + ((double)x[2] * x[2] + (double)x[3] * x[3]);
+        }
+        for (int i = whole + threadIdx.x; i < cnt; i += 256) s += (double)g[i] * g[i];
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) partial[blockIdx.x] = s;
+}
+__global__ __launch_bounds__(256) void adamw_norm_final_kernel(const double* partial, int nb, double* slots, float* norm) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < nb; i += 256) s += partial[i];
+    s = block_sum(s);
+    if (threadIdx.x == 0) {
+        slots[0] = s;
+        if (norm) *norm = (float)sqrt(s);
+    }
+}
+
+__device__ __forceinline__ float clip(const double* slots, const Consts& c) {
+    if (!slots) return 1.f;
+    const double r = c.max_norm / (sqrt(slots[0]) + 1e-6);
+    return r < 1.0 ? (float)r : (r >= 1.0 ? 1.f : (float)r);           // a NaN stays one
+}
+__device__ __forceinline__ void update(float& p, float g, float& m, float& v, float& root, float coef, const Consts& c) {
+    g = g * coef;
+    m = m * c.b1 + g * c.c1;
+    v = v * c.b2 + (g * g) * c.c2;
+    root = sqrtf(v);
+    p = p * c.decay - (m / (root * c.root + c.eps)) * c.step;
+}
+
+__global__ __launch_bounds__(256) void adamw32_kernel(const Entry* tab, int n, const double* slots, Consts c) {
+    const float coef = clip(slots, c);
+    const int block = blockIdx.x + tab[0].block0;
+    const Entry en = tab[find(tab, n, block)];
+    const long base = (long)(block - en.block0) * CHUNK;
+    const int cnt = en.n - base < CHUNK ? (int)(en.n - base) : CHUNK;
+    float* p = en.p + base;
+    const float* g = en.g + base;
+    float* m = (float*)en.m + base;
+    float* v = (float*)en.v + base;
+    const bool fresh = en.flags & 1;
+    const int whole = en.flags & 2 ? cnt & ~3 : 0;
+    float root;
+    for (int i = threadIdx.x * 4; i < whole; i += 1024) {
+        f32x4 pv = *reinterpret_cast<const f32x4*>(p + i);
+        const f32x4 gv = *reinterpret_cast<const f32x4*>(g + i);
+        f32x4 mv = {0.f, 0.f, 0.f, 0.f}, vv = mv;
+        if (!fresh) {
+            mv = *reinterpret_cast<const f32x4*>(m + i);
+            vv = *reinterpret_cast<const f32x4*>(v + i);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float a = pv[k], b = mv[k], d = vv[k];
+            update(a, gv[k], b, d, root, coef, c);
+            pv[k] = a; mv[k] = b; vv[k] = d;
+        }
+        *reinterpret_cast<f32x4*>(m + i) = mv;
+        *reinterpret_cast<f32x4*>(v + i) = vv;
+        *reinterpret_cast<f32x4*>(p + i) = pv;
+    }
+    for (int i = whole + threadIdx.x; i < cnt; i += 256) {
+        float a = p[i], b = fresh ? 0.f : m[i], d = fresh ? 0.f : v[i];
+        update(a, g[i], b, d, root, coef, c);
+        p[i] = a; m[i] = b; v[i] = d;
+    }
+}
+
+// ----------------------------------------------------------------------------- 8-bit states
+// The word of an element: 16 bits for the first moment, 16 for the second.
+__device__ __forceinline__ uint32_t word_of(long e, uint32_t key) {
+    return mix32((uint32_t)e ^ key ^ ((uint32_t)(e >> 32) * 0x9E3779B1U));
+}
+// Codes of magnitude a <= 448 between 2^-6 and 448 have three bits behind the leading one; below 2^-6 they are
+// multiples of 2^-9, which is what three bits are once 2^-6 is added.
+__device__ __forceinline__ float code_m(float y, uint32_t r16) {
+    float a = fabsf(y);
+    const float less = a < 0.015625f ? 0.015625f : 0.f;
+    const uint32_t b = (__float_as_uint(a + less) + (r16 << 4) + 8u) & ~0xFFFFFu;
+    a = fminf(__uint_as_float(b) - less, TOP);
+    return y < 0.f ? -a : a;
+}
+__device__ __forceinline__ float code_v(float y, uint32_t r16) {
+    const float less = y < 0.015625f ? 0.015625f : 0.f;
+    const uint32_t b = __float_as_uint(fminf(y, TOP) + less) & ~0xFFFFFu;
+    const float lo = __uint_as_float(b) - less, hi = fminf(__uint_as_float(b + 0x100000u) - less, TOP);
+    const float u = ((float)r16 + 0.5f) * 1.52587890625e-5f;
+    const float l2 = lo * lo;
+    const float a = u * (hi * hi - l2) < y * y - l2 ? hi : lo;
+    return y > 0.f ? fmaxf(a, 0.001953125f) : a;
+}
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
+    return x;
+}
+template <bool VEC>
+__device__ __forceinline__ void step8(const Entry& en, long base, int cnt, float coef, const Consts& c) {
+    const int lane = threadIdx.x & 63;
+    const bool fresh = en.flags & 1;
+    for (int blk = threadIdx.x >> 6; blk * BLOCK < cnt; blk += 4) {
+        const int i0 = blk * BLOCK + lane * 4;
+        const long at = base + i0;
+        const int left = cnt - i0;                       // this lane's elements: min(4, left)
+        const bool whole = VEC && left >= 4;
+        float p[4] = {}, g[4] = {}, m[4] = {}, v[4] = {}, root[4] = {};
+        uint32_t mc = 0, vc = 0;
+        if (whole) {
+            Vec4<float>::load(en.p + at, p);
+            Vec4<float>::load(en.g + at, g);
+            if (!fresh) {
+                mc = *reinterpret_cast<const uint32_t*>((const uint8_t*)en.m + at);
+                vc = *reinterpret_cast<const uint32_t*>((const uint8_t*)en.v + at);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < left) {
+                    p[k] = en.p[at + k];
+                    g[k] = en.g[at + k];
+                    if (!fresh) {
+                        mc |= (uint32_t)((const uint8_t*)en.m)[at + k] << (8 * k);
+                        vc |= (uint32_t)((const uint8_t*)en.v)[at + k] << (8 * k);
+                    }
+                }
+        }
+        const long sb = (base + blk * BLOCK) / BLOCK;
+        const float ms = fresh ? 0.f : en.ms[sb], vs = fresh ? 0.f : en.vs[sb];
+        m[0] = __builtin_amdgcn_cvt_f32_fp8(mc, 0); m[1] = __builtin_amdgcn_cvt_f32_fp8(mc, 1);
+        m[2] = __builtin_amdgcn_cvt_f32_fp8(mc, 2); m[3] = __builtin_amdgcn_cvt_f32_fp8(mc, 3);
+        v[0] = __builtin_amdgcn_cvt_f32_fp8(vc, 0); v[1] = __builtin_amdgcn_cvt_f32_fp8(vc, 1);
+        v[2] = __builtin_amdgcn_cvt_f32_fp8(vc, 2); v[3] = __builtin_amdgcn_cvt_f32_fp8(vc, 3);
+        float tm = 0.f, tv = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            m[k] = m[k] * ms;
+            v[k] = v[k] * vs;
+            v[k] = v[k] * v[k];
+            update(p[k], g[k], m[k], v[k], root[k], coef, c);
+            tm = fmaxf(tm, fabsf(m[k]));
+            tv = fmaxf(tv, root[k]);
+        }
+        tm = wave_max(tm);
+        tv = wave_max(tv);
+        const float im = tm >= 1.925929944387236e-34f ? TOP / tm : 0.f;          // 2^-112: nothing to hold
+        const float iv = tv >= 1.925929944387236e-34f ? TOP / tv : 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t w = word_of(at + k, c.key);
+            m[k] = code_m(m[k] * im, w & 0xFFFFu);
+            v[k] = code_v(root[k] * iv, w >> 16);
+        }
+        mc = __builtin_amdgcn_cvt_pk_fp8_f32(m[0], m[1], 0, false);
+        mc = __builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], mc, true);
+        vc = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+        vc = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], vc, true);
+        if (whole) {
+            Vec4<float>::store(en.p + at, p);
+            *reinterpret_cast<uint32_t*>((uint8_t*)en.m + at) = mc;
+            *reinterpret_cast<uint32_t*>((uint8_t*)en.v + at) = vc;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (k < left) {
+                    en.p[at + k] = p[k];
+                    ((uint8_t*)en.m)[at + k] = (uint8_t)(mc >> (8 * k));
+                    ((uint8_t*)en.v)[at + k] = (uint8_t)(vc >> (8 * k));
+                }
+        }
+        if (lane == 0) {
+            en.ms[sb] = im > 0.f ? tm * (1.f / TOP) : 0.f;
+            en.vs[sb] = iv > 0.f ? tv * (1.f / TOP) : 0.f;
+        }
+    }
+}
+__global__ __launch_bounds__(256) void adamw8_kernel(const Entry* tab, int n, const double* slots, Consts c) {
+    const float coef = clip(slots, c);
+    const int block = blockIdx.x + tab[0].block0;
+    const Entry en = tab[find(tab, n, block)];
+    const long base = (long)(block - en.block0) * CHUNK;
+    const int cnt = en.n - base < CHUNK ? (int)(en.n - base) : CHUNK;
+    if (en.flags & 2) step8<true>(en, base, cnt, coef, c);
+    else step8<false>(en, base, cnt, coef, c);
+}
+
+uint32_t host_mix32(uint32_t x) {
+    x ^= x >> 16; x *= 0x7feb352dU;
+    x ^= x >> 15; x *= 0x846ca68bU;
+    return x ^ (x >> 16);
+}
+
+}  // namespace
+
+extern "C" int vitk_adamw_norm(const void* table, int n_entries, int n_blocks, double* slots, float* norm, void* stream) {
+    if (!table || !slots) return VITK_ERR_NULL;
+    if (n_entries <= 0 || n_blocks <= 0) return VITK_ERR_SHAPE;
+    hipStream_t st = (hipStream_t)stream;
+    const int nb = n_blocks < PARTIALS ? n_blocks : PARTIALS;
+    hipLaunchKernelGGL(adamw_norm_kernel, dim3(nb), dim3(256), 0, st, (const Entry*)table, n_entries, n_blocks, slots + 1);
+    VITK_CHECK_LAUNCH();
+    hipLaunchKernelGGL(adamw_norm_final_kernel, dim3(1), dim3(256), 0, st, slots + 1, nb, slots, norm);
+    VITK_CHECK_LAUNCH();
+    return 0;
+}
+
+extern "C" int vitk_adamw_step(const void* table, int n_entries, int n_blocks, const double* slots, double max_norm, double lr,
+                               double beta1, double beta2, double eps, double weight_decay, long step, int state_bits,
+                               uint32_t seed, void* stream) {
+    if (!table) return VITK_ERR_NULL;
+    if (n_entries <= 0 || n_blocks <= 0 || step < 1) return VITK_ERR_SHAPE;
+    if (state_bits != 32 && state_bits != 8) return VITK_ERR_UNSUPPORTED;
+    if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0)) return VITK_ERR_SHAPE;
+    Consts c{};
+    c.b1 = (float)beta1; c.c1 = (float)(1.0 - beta1);
+    c.b2 = (float)beta2; c.c2 = (float)(1.0 - beta2);
+    c.decay = (float)(1.0 - lr * weight_decay);
+    c.step = (float)(lr / (1.0 - pow(beta1, (double)step)));
+    c.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+    c.eps = (float)eps;
+    c.max_norm = max_norm;
+    c.key = host_mix32(seed + (uint32_t)step * 0x9E3779B1U);
+    hipStream_t st = (hipStream_t)stream;
+    if (state_bits == 32)
+        hipLaunchKernelGGL(adamw32_kernel, dim3(n_blocks), dim3(256), 0, st, (const Entry*)table, n_entries, slots, c);
+    else
+        hipLaunchKernelGGL(adamw8_kernel, dim3(n_blocks), dim3(256), 0, st, (const Entry*)table, n_entries, slots, c);
+    VITK_CHECK_LAUNCH();
+    return 0;
+}

@@ -128,3 +128,142 @@ class FusedSGD(torch.optim.Optimizer):
         if max_grad_norm is not None:
             return self._slots[0].sqrt()
         return None
+
+
+_ADAMW_ENTRY = np.dtype([("param", "<u8"), ("grad", "<u8"), ("m", "<u8"), ("v", "<u8"), ("m_scale", "<u8"),
+                         ("v_scale", "<u8"), ("n", "<i8"), ("block0", "<i4"), ("flags", "<i4")])
+_ADAMW_SLOTS = 1 + 1024      # VITK_ADAMW_SLOTS (include/vitk.h)
+_SCALE_BLOCK = 256           # elements of an 8-bit state that share a scale
+assert _ADAMW_ENTRY.itemsize == 64
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) over all tensors in one launch, with gradient clipping by the joint norm.
+
+    ``state_bits`` 32: moments in fp32, the arithmetic and the state names of torch.optim.AdamW (`exp_avg`, `exp_avg_sq`),
+    whose state dicts it loads.  8: e4m3 codes of the parameter's shape with one fp32 scale for each 256 consecutive
+    elements (`exp_avg_scale`, `exp_avg_sq_scale`); an element of `exp_avg` is code * scale, of `exp_avg_sq`
+    (code * scale)^2.  Codes are rounded at random from (``seed``, step, element), so that their expectation is the
+    moment; replicas with equal gradients stay bit-identical.  Parameters and gradients are contiguous fp32 tensors on
+    one GPU.  A step counts on the host, so it is not captured into a graph."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
+            raise ValueError("lr, eps and weight_decay must be non-negative")
+        if not all(0.0 <= b < 1.0 for b in betas):
+            raise ValueError("betas lie in [0, 1)")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits is 8 or 32")
+        self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFF
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self._slots = None
+        self._dev = None          # the table on the device
+        self._last = None         # its contents (numpy), to skip uploads of an unchanged table
+        self._ring, self._turn = [], 0
+
+    def load_state_dict(self, state_dict):
+        held = [s for s in state_dict["state"].values() if s]
+        if any(("exp_avg_scale" in s) != (self.state_bits == 8) for s in held):
+            raise ValueError(f"the state dict's moments are not in {self.state_bits} bits")
+        super().load_state_dict(state_dict)
+        for p, st in self.state.items():
+            if st:
+                st["step"] = int(st["step"])
+                kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32      # exact: codes came back as fp32
+                for name, value in st.items():
+                    if name != "step":      # copies: the state dict's tensors may be another optimizer's
+                        st[name] = torch.empty(value.shape, dtype=torch.float32 if name.endswith("_scale") else kind,
+                                               device=p.device).copy_(value)
+
+    def _row(self, p, block0):
+        g, st = p.grad, self.state[p]
+        if not (p.is_cuda and p.dtype == torch.float32 and g.dtype == torch.float32 and not g.is_sparse
+                and p.is_contiguous() and g.is_contiguous()):
+            raise ValueError("FusedAdamW needs contiguous fp32 parameters and gradients on the GPU")
+        n = p.numel()
+        if not st:
+            kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
+            st["step"] = 0
+            st["exp_avg"] = torch.empty(p.shape, dtype=kind, device=p.device)
+            st["exp_avg_sq"] = torch.empty(p.shape, dtype=kind, device=p.device)
+            if self.state_bits == 8:
+                for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+                    st[name] = torch.empty(-(-n // _SCALE_BLOCK), dtype=torch.float32, device=p.device)
+        m, v = st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
+        ms, vs = (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr()) if self.state_bits == 8 else (0, 0)
+        vec = (p.data_ptr() | g.data_ptr()) % 16 == 0 and (m | v) % (4 if self.state_bits == 8 else 16) == 0
+        return (p.data_ptr(), g.data_ptr(), m, v, ms, vs, n, block0, (1 if st["step"] == 0 else 0) | (2 if vec else 0))
+
+    def _upload(self, host, dev):
+        """The table on the device; uploads go through a ring of pinned buffers, each guarded by an event, so the host
+        never waits for the step it has just enqueued."""
+        if self._last is not None and self._last.shape == host.shape and np.array_equal(self._last, host):
+            return
+        nbytes = host.nbytes
+        if self._dev is None or self._dev.numel() < nbytes:
+            self._dev = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        if not self._ring or self._ring[0][0].numel() < nbytes:
+            self._ring = [(torch.empty(max(2 * nbytes, 1 << 14), dtype=torch.uint8, pin_memory=True), torch.cuda.Event())
+                          for _ in range(4)]
+            self._turn = 0
+        else:
+            self._ring[self._turn][1].synchronize()
+        buf, ev = self._ring[self._turn]
+        buf.numpy()[:nbytes] = host.view(np.uint8)
+        self._dev[:nbytes].copy_(buf[:nbytes], non_blocking=True)
+        ev.record()
+        self._turn = (self._turn + 1) % 4
+        self._last = host
+
+    @torch.no_grad()
+    def step(self, closure=None, max_grad_norm=None):
+        """One update.  With `max_grad_norm`, gradients of ALL groups are clipped by their joint 2-norm first and that
+        norm is returned as a 0-d tensor."""
+        if closure is not None:
+            raise ValueError("FusedAdamW does not re-evaluate the model")
+        if max_grad_norm is not None and not max_grad_norm >= 0.0:
+            raise ValueError("max_grad_norm must be non-negative")
+        # one launch for the tensors of a group that have taken the same number of steps
+        runs = []
+        for group in self.param_groups:
+            by_step = {}
+            for p in group["params"]:
+                if p.grad is not None and p.numel():
+                    by_step.setdefault(self.state[p].get("step", 0), []).append(p)
+            runs += [(group, t, ps) for t, ps in by_step.items()]
+        if not runs:
+            return None
+        dev = runs[0][2][0].device
+        if any(p.device != dev for _, _, ps in runs for p in ps):
+            raise ValueError("FusedAdamW updates tensors of one device")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW.step counts steps on the host and is not captured into a graph")
+        rows, spans, blocks = [], [], 0
+        for group, t, ps in runs:
+            first, at = len(rows), blocks
+            for p in ps:
+                rows.append(self._row(p, blocks))
+                blocks += (p.numel() + _CHUNK - 1) // _CHUNK
+            spans.append((first, len(rows) - first, blocks - at))
+        with torch.cuda.device(dev):
+            self._upload(np.array(rows, dtype=_ADAMW_ENTRY), dev)
+            if self._slots is None:
+                self._slots = torch.empty(_ADAMW_SLOTS, dtype=torch.float64, device=dev)
+            stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+            base = self._dev.data_ptr()
+            slots = norm = None
+            if max_grad_norm is not None:
+                norm = torch.empty((), dtype=torch.float32, device=dev)
+                slots = self._slots.data_ptr()
+                vitk.check(vitk.lib.vitk_adamw_norm(base, len(rows), blocks, slots, norm.data_ptr(), stream), "adamw_norm")
+            for (group, t, ps), (first, cnt, nblk) in zip(runs, spans):
+                b1, b2 = group["betas"]
+                vitk.check(vitk.lib.vitk_adamw_step(base + first * _ADAMW_ENTRY.itemsize, cnt, nblk, slots,
+                                                    float(max_grad_norm or 0.0), float(group["lr"]), float(b1), float(b2),
+                                                    float(group["eps"]), float(group["weight_decay"]), t + 1,
+                                                    self.state_bits, self.seed, stream), "adamw_step")
+                for p in ps:
+                    self.state[p]["step"] = t + 1
+            # the parameters were written through raw pointers: renew the GEMM operands kept with them (one launch)
+            vitk.ops.refresh_operands([p for _, _, ps in runs for p in ps])
+        return norm

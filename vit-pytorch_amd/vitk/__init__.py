@@ -28,6 +28,27 @@ class EpilogueArgs(ctypes.Structure):
                 ("npatch", ctypes.c_int), ("dropout_p", ctypes.c_float), ("seed", ctypes.c_uint64)]
 
 
+def _fields(text):
+    """'vp: q k v; l: q_b q_n' -> ctypes fields, in that order."""
+    kinds = {"vp": ctypes.c_void_p, "l": ctypes.c_long, "i": ctypes.c_int, "f": ctypes.c_float, "d": ctypes.c_double}
+    return [(n, kinds[k.strip()]) for k, names in (part.split(":") for part in text.split(";")) for n in names.split()]
+
+
+class SlideAttn(ctypes.Structure):
+    _fields_ = _fields("vp: q k v o o_f32 lse lengths d_o delta dq dk dv; l: q_b q_n q_h k_b k_n k_h v_b v_n v_h "
+                       "do_b do_n do_h dq_b dq_n dq_h dk_b dk_n dk_h dv_b dv_n dv_h; i: B N Hq Hkv dh window sinks causal; f: scale")
+
+
+class SlideCache(ctypes.Structure):
+    _fields_ = _fields("vp: q k v o lengths workspace; l: q_b q_h k_b k_n k_h v_b v_n v_h; "
+                       "i: B cap Hq Hkv dh window sinks splits; f: scale")
+
+
+class Rope(ctypes.Structure):
+    _fields_ = _fields("vp: x y pos; l: x_b x_n x_h y_b y_n y_h pos_b; i: B N H dh axes pos_kind interleaved inverse") + \
+        [("pairs", ctypes.c_int * 8), ("base", ctypes.c_double)]
+
+
 _vp, _i, _l, _f, _u64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float, ctypes.c_uint64
 
 # name -> argtypes; every function returns int (0 = ok)
@@ -75,6 +96,12 @@ PROTOTYPES = {
     "vitk_gemm_set_persistent": [_i],
     "vitk_sgd_norm_sq": [_vp, _i, _i, _vp, _vp],
     "vitk_sgd_step": [_vp, _i, _i, _vp, _f, _f, _f, _f, _f, _vp],
+    "vitk_slide_attn_fwd": [ctypes.POINTER(SlideAttn), _i, _vp],
+    "vitk_slide_attn_bwd": [ctypes.POINTER(SlideAttn), _i, _vp],
+    "vitk_slide_decode": [ctypes.POINTER(SlideCache), _i, _vp],
+    "vitk_axial_rope": [ctypes.POINTER(Rope), _i, _vp],
+    "vitk_adamw_norm": [_vp, _i, _i, _vp, _vp, _vp],
+    "vitk_adamw_step": [_vp, _i, _i, _vp] + [ctypes.c_double] * 6 + [_l, _i, ctypes.c_uint32, _vp],
     "vitk_comm_unique_id": [_vp, ctypes.c_size_t],
     "vitk_comm_init": [_i, _i, _vp, ctypes.POINTER(ctypes.c_void_p)],
     "vitk_allreduce": [_vp, _vp, ctypes.c_size_t, _i, _i, _vp],

@@ -1051,3 +1051,8 @@ class PatchEmbedFn(torch.autograd.Function):
 
 def patch_embed(img, conv_w, conv_b, cls, pos, dropout_p, dtype):
     return PatchEmbedFn.apply(img, conv_w, conv_b, cls, pos, float(dropout_p), dtype)
+
+
+# ----------------------------------------------------------------------------- long token sequences
+from .seq_ops import (axial_rope, grid_positions, sliding_attention, sliding_attention_decode,  # noqa: E402,F401
+                      sliding_attention_qkv)
