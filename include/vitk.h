@@ -221,12 +221,15 @@ typedef struct vitk_slide_attn {
     const int* lengths;
     const void* d_o; float* delta;
     void* dq; void* dk; void* dv;
+    float* workspace;
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h;
     long do_b, do_n, do_h, dq_b, dq_n, dq_h, dk_b, dk_n, dk_h, dv_b, dv_n, dv_h;
     int B, N, Hq, Hkv, dh;
     int window, sinks, causal;
     float scale;
 } vitk_slide_attn;
+/* Bytes of `workspace` (16-byte aligned, contents undefined) that the forward or the backward call needs; 0: it may be NULL. */
+size_t vitk_slide_attn_workspace(const vitk_slide_attn* a, int backward);
 int vitk_slide_attn_fwd(const vitk_slide_attn* a, int dtype, void* stream);
 int vitk_slide_attn_bwd(const vitk_slide_attn* a, int dtype, void* stream);
 /* One query per sequence, the last of its lengths[b] cached tokens: it sees j < sinks and j >= lengths[b] - window.

@@ -143,6 +143,22 @@ def test_what_lies_behind_a_sequence_is_not_looked_at(dt, causal):
             assert (a[1, 71:] == 0).all()
 
 
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("level", [-900.0, 900.0])
+def test_scores_far_from_zero(dt, causal, level):
+    """Every score near -900 or 900: the sums' logarithms lie far outside the range of an exponential."""
+    from vitk import ops
+    B, N, H, dh = 1, 333, 2, 64
+    q, k, v, d_o = (_rand(B, N, H, dh, dtype=dt, seed=s) for s in range(4))
+    q, k = q * 0.25, k * 0.25
+    q[..., 0], k[..., 0] = 85.0, level * 8 / 85.0
+    kw = dict(window=20, sinks=3, causal=causal)
+    want = SO.sliding_attention(q, k, v, 20, 3, causal, None, dh ** -0.5, R[dt], d_o)
+    for name, got in zip(("o", "dq", "dk", "dv"), _grads(*(t.to(DEV) for t in (q, k, v, d_o)), **kw)):
+        _hold(name, got, *want[name])
+
+
 def test_strides_orders_and_repeats_give_the_same_bits():
     q, k, v, d_o = _case(BF)
     kw = dict(window=33, sinks=2, causal=True)

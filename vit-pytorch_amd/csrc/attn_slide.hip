@@ -12,6 +12,13 @@
 // r = 4 b + e of lane half h holds tile row 8 b + 4 h + e, and the second product's left operand is read from the LDS
 // tile in that same order of rows.  Rows behind a sequence's length are staged as zeros, whatever memory holds there:
 // a probability of zero times a NaN would be a NaN.
+//
+// Rows that see a window cost the same everywhere; the first tokens do not: every query looks at their keys, and without a
+// causal mask they look at every key.  The workgroup of a tile therefore handles the tile's BAND only (its window and, for
+// ordinary rows, the few first tokens on the other side), and what the first tokens see beyond their band is cut into
+// chunks of FAR items: 32 first tokens against a share of the far rows, dealt out to four waves that meet in LDS.
+// Bands and chunks of a first token leave 32-bit records in a workspace, which a last small launch adds in a fixed order.
+// (Without the split one workgroup per head walked the whole sequence: 6.9 ms instead of the time below at 16384 tokens.)
 #include <initializer_list>
 
 #include "common.h"
@@ -30,6 +37,11 @@ struct Slide {
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, do_b, do_n, do_h, dq_b, dq_n, dq_h, dk_b, dk_n, dk_h, dv_b, dv_n, dv_h;
     int window, sinks;
     float scale;
+    int rows;                  // first tokens with records, a multiple of 32 (0: none)
+    int chunks;                // far items of each 32 of them; a row has chunks + 1 records, the band's last
+    float* ws;                 // forward: records of dh + 2; backward: dk | dv, then dq, records of dh
+    float* ws_q;
+    int far_items, items;      // of this launch: far ones come first, then bands
 };
 
 // ----------------------------------------------------------------------------- which pairs are visible
@@ -64,22 +76,19 @@ __device__ __forceinline__ Tiles tiles_of(int lo, int hi, int first, int n, int 
     t.hi = hi >= lo ? hi / T + 1 : 0;
     return t;
 }
+// The band of query rows [qa, qb], of key rows [ka, kb].  A window of 0 is listed like one of 1, so that far rows always lie
+// behind the diagonal.
 template <bool CAUSAL> __device__ __forceinline__ Tiles key_tiles(int qa, int qb, int n, int w, int f, int T) {
     if (qa >= n) return Tiles{0, 0, 0};
     qb = qb < n ? qb : n - 1;
-    if constexpr (CAUSAL) {
-        const int first = f < qb + 1 ? f : qb + 1;
-        return tiles_of(qa - w + 1, w > 0 ? qb : -1, first, n, T);
-    }
-    if (qa < f) return tiles_of(0, n - 1, 0, n, T);
-    return tiles_of(qa - w + 1, w > 0 ? qb + w - 1 : -1, f, n, T);
+    const int r = (w > 1 ? w : 1) - 1;
+    return tiles_of(qa - r, CAUSAL ? qb : qb + r, CAUSAL && f > qb + 1 ? qb + 1 : f, n, T);
 }
 template <bool CAUSAL> __device__ __forceinline__ Tiles query_tiles(int ka, int kb, int n, int w, int f, int T) {
     if (ka >= n) return Tiles{0, 0, 0};
     kb = kb < n ? kb : n - 1;
-    if constexpr (CAUSAL) return tiles_of(ka, ka < f ? n - 1 : (w > 0 ? kb + w - 1 : -1), 0, n, T);
-    if (ka < f) return tiles_of(0, n - 1, 0, n, T);
-    return tiles_of(ka - w + 1, w > 0 ? kb + w - 1 : -1, f, n, T);
+    const int r = (w > 1 ? w : 1) - 1;
+    return tiles_of(CAUSAL ? ka : ka - r, kb + r, CAUSAL ? 0 : f, n, T);
 }
 
 // ----------------------------------------------------------------------------- operands
@@ -175,6 +184,17 @@ template <typename T, int DH, int NT> __device__ __forceinline__ void stage(char
         *reinterpret_cast<u32x4*>(tile + row * ROW + ch * 16) = z;
     }
 }
+// The same for 32 rows by one wave.
+template <typename T, int DH> __device__ __forceinline__ void stage_wave(char* tile, const T* base, long ld, int r0, int end, int lane) {
+    constexpr int C = Shape<T, DH>::CHUNKS, ROW = Shape<T, DH>::ROW;
+#pragma unroll
+    for (int i = 0; i < 32 * C / 64; ++i) {
+        const int idx = lane + i * 64, row = idx / C, ch = idx % C;
+        u32x4 z = {0, 0, 0, 0};
+        if (r0 + row < end) z = *reinterpret_cast<const u32x4*>(base + (long)(r0 + row) * ld + ch * (16 / (int)sizeof(T)));
+        *reinterpret_cast<u32x4*>(tile + row * ROW + ch * 16) = z;
+    }
+}
 // acc[d][column] of this lane's column, times `mul`, to a row of DH elements.
 template <typename T, int DH> __device__ __forceinline__ void put(T* row, const f32x16* acc, float mul, int lane) {
 #pragma unroll
@@ -224,18 +244,81 @@ struct Softmax {
     __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
 };
 
+// ----------------------------------------------------------------------------- work items
+// Far items first (the longest), then bands, a head's tiles in a row.  Workgroups go round the 8 XCDs in turn: each XCD
+// gets a run of neighbouring items, whose tiles of the other axis it finds in its own L2.
+struct Item { bool far, none; int x, h, b; };
+__device__ __forceinline__ Item item_of(const Slide& p, int heads, int tiles) {
+    Item it{};
+    const int id = blockIdx.x;
+    it.far = id < p.far_items;
+    int k;
+    if (it.far) {
+        k = id;
+        tiles = p.chunks * (p.rows / 32);
+    } else {
+        const int m = p.items - p.far_items, each = (m + 7) / 8, r = id - p.far_items;
+        k = (r & 7) * each + (r >> 3);
+        it.none = (r >> 3) >= each || k >= m;
+    }
+    it.x = k % tiles;
+    it.h = k / tiles % heads;
+    it.b = k / tiles / heads;
+    return it;
+}
+// Sums of the four waves, [32 columns][DH] each, in LDS; `extra` behind them.
+template <int DH> constexpr int join_bytes() { return 4 * 32 * (DH + 4) * (int)sizeof(float); }
+
+// One record of the softmax of a row from the four waves': called by all threads, f(column, d, sum, maximum, total).
+template <int DH, typename F> __device__ __forceinline__ void join_waves(char* lds, const f32x16* acc, float m, float l, int tid, F f) {
+    constexpr int W = DH + 4;
+    const int lane = tid & 63, wave = tid >> 6;
+    float* out = reinterpret_cast<float*>(lds);
+    float* mine = out + (wave * 32 + (lane & 31)) * W;
+    __syncthreads();
+    put<float, DH>(mine, acc, 1.f, lane);
+    if (lane < 32) { mine[DH] = m; mine[DH + 1] = l; }
+    __syncthreads();
+    for (int idx = tid; idx < 32 * DH; idx += 256) {
+        const int c = idx / DH, d = idx % DH;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, out[(w * 32 + c) * W + DH]);
+        float x = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float* rec = out + (w * 32 + c) * W;
+            const float e = rec[DH] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(rec[DH] - top);
+            x += rec[d] * e;
+            sum += rec[DH + 1] * e;
+        }
+        f(c, d, x, top, sum);
+    }
+}
+// The plain sum of the four waves', to records `stride` floats apart.
+template <int DH> __device__ __forceinline__ void add_waves(char* lds, const f32x16* acc, float* rec, long stride, int tid) {
+    constexpr int W = DH + 4;
+    const int lane = tid & 63, wave = tid >> 6;
+    float* out = reinterpret_cast<float*>(lds);
+    __syncthreads();
+    put<float, DH>(out + (wave * 32 + (lane & 31)) * W, acc, 1.f, lane);
+    __syncthreads();
+    for (int idx = tid; idx < 32 * DH; idx += 256) {
+        const int c = idx / DH, d = idx % DH;
+        const float* o = out + c * W + d;
+        rec[c * stride + d] = (o[0] + o[32 * W]) + (o[64 * W] + o[96 * W]);
+    }
+}
+
 // ----------------------------------------------------------------------------- forward
-// One workgroup: 128 queries of one (sequence, head), each wave 32 of them; key tiles stream through LDS.
+// Band: 128 queries of one (sequence, head), each wave 32 of them; key tiles stream through LDS.
 template <typename T, int DH, bool CAUSAL>
-__global__ __launch_bounds__(256, 1) void slide_fwd_kernel(Slide p) {
+__device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
-    extern __shared__ __align__(16) char lds[];
     char* Ks = lds;
     char* Vs = lds + S::KT * S::ROW;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = blockIdx.y, b = blockIdx.z, hk = h / p.G;
-    const int n = length_of(p, b);
-    const int q0 = blockIdx.x * TQ, qa = q0 + wave * 32, qi = qa + (lane & 31);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int qa = q0 + wave * 32, qi = qa + (lane & 31);
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
     Kept<T, DH> q;
@@ -267,15 +350,92 @@ __global__ __launch_bounds__(256, 1) void slide_fwd_kernel(Slide p) {
             gather<DH>(acc, Vs, sub, s, lane, T{});
         }
     }
-    const float l = sm.total();
+    const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
     if (qi < p.N) {
+        if (!CAUSAL && qi < p.rows) {
+            float* rec = p.ws + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * (DH + 4);
+            put<float, DH>(rec, acc, 1.f, lane);
+            if (lane < 32) { rec[DH] = m; rec[DH + 1] = l; }
+            return;
+        }
         const float inv = l > 0.f ? 1.f / l : 0.f;
         const long row = ((long)b * p.N + qi) * p.Hq + h;
         put<T, DH>((T*)p.o + row * DH, acc, inv, lane);
         if (p.o32) put<float, DH>(p.o32 + row * DH, acc, inv, lane);
         // base-2 logarithm of the row's sum; +inf for a row that sees nothing, so that backward's probabilities are 0
-        if (p.lse && lane < 32) p.lse[((long)b * p.Hq + h) * p.N + qi] = l > 0.f ? sm.m * sc + __log2f(l) : INFINITY;
+        if (p.lse && lane < 32) p.lse[((long)b * p.Hq + h) * p.N + qi] = l > 0.f ? m + __log2f(l) : INFINITY;
     }
+}
+// Far: 32 first queries against every (4 chunks)-th 32 keys behind their band.
+template <typename T, int DH>
+__device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h, int b, int n) {
+    using S = Shape<T, DH>;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int chunk = x % p.chunks, qa = x / p.chunks * 32, qi = qa + (lane & 31);
+    char* Ks = lds + wave * 2 * 32 * S::ROW;
+    char* Vs = Ks + 32 * S::ROW;
+    const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
+    const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
+    const bool mine = qi < n && qi < p.sinks;
+    Kept<T, DH> q;
+    q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, mine);
+    const float sc = p.scale * LOG2E;
+    f32x16 acc[DH / 32] = {};
+    Softmax sm;
+    const int q0 = qa / TQ * TQ;
+    const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
+    const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
+        stage_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
+        stage_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
+        wave_lds_fence();
+        f32x16 s = product<DH>(Ks, 0, q, lane);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (!mine || k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= n) s[r] = -INFINITY;
+        const float alpha = sm.step(s, sc);
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
+        gather<DH>(acc, Vs, 0, s, lane, T{});
+        wave_lds_fence();
+    }
+    const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
+    float* base = p.ws + ((((long)b * p.Hq + h) * p.rows + qa) * (p.chunks + 1) + chunk) * (DH + 4);
+    join_waves<DH>(lds, acc, m, l, tid, [&](int c, int d, float sum, float top, float total) {
+        float* rec = base + (long)c * (p.chunks + 1) * (DH + 4);
+        rec[d] = sum;
+        if (d == 0) { rec[DH] = top; rec[DH + 1] = total; }
+    });
+}
+template <typename T, int DH, bool CAUSAL>
+__global__ __launch_bounds__(256, 1) void slide_fwd_kernel(Slide p) {
+    extern __shared__ __align__(16) char lds[];
+    const Item it = item_of(p, p.Hq, (p.N + TQ - 1) / TQ);
+    if (it.none) return;
+    const int n = length_of(p, it.b);
+    if constexpr (!CAUSAL)
+        if (it.far) return fwd_far<T, DH>(p, lds, it.x, it.h, it.b, n);
+    fwd_band<T, DH, CAUSAL>(p, lds, it.x * TQ, it.h, it.b, n);
+}
+// The records of the first rows become outputs.
+template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_fwd_join_kernel(Slide p) {
+    const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, d = threadIdx.x;
+    if (d >= DH) return;
+    const float* rec = p.ws + (((long)b * p.Hq + h) * p.rows + i) * (p.chunks + 1) * (DH + 4);
+    float top = -INFINITY;
+    for (int s = 0; s <= p.chunks; ++s) top = fmaxf(top, rec[s * (DH + 4) + DH]);
+    float x = 0.f, sum = 0.f;
+    for (int s = 0; s <= p.chunks; ++s) {
+        const float* r = rec + s * (DH + 4);
+        const float e = r[DH] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[DH] - top);
+        x += r[d] * e;
+        sum += r[DH + 1] * e;
+    }
+    x = sum > 0.f ? x / sum : 0.f;
+    const long row = ((long)b * p.N + i) * p.Hq + h;
+    ((T*)p.o)[row * DH + d] = (T)x;
+    if (p.o32) p.o32[row * DH + d] = x;
+    if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.N + i] = sum > 0.f ? top + __log2f(sum) : INFINITY;
 }
 
 // ----------------------------------------------------------------------------- backward
@@ -305,15 +465,12 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta
 }
 
 template <typename T, int DH, bool CAUSAL>
-__global__ __launch_bounds__(256, 1) void slide_dq_kernel(Slide p) {
+__device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
-    extern __shared__ __align__(16) char lds[];
     char* Ks = lds;
     char* Vs = lds + S::KT * S::ROW;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int h = blockIdx.y, b = blockIdx.z, hk = h / p.G;
-    const int n = length_of(p, b);
-    const int q0 = blockIdx.x * TQ, qa = q0 + wave * 32, qi = qa + (lane & 31);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int qa = q0 + wave * 32, qi = qa + (lane & 31);
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
     Kept<T, DH> q, d_o;
@@ -346,21 +503,94 @@ __global__ __launch_bounds__(256, 1) void slide_dq_kernel(Slide p) {
             gather<DH>(acc, Ks, sub, s, lane, T{});
         }
     }
-    if (qi < p.N) put<T, DH>((T*)p.dq + b * p.dq_b + (long)qi * p.dq_n + h * p.dq_h, acc, qi < n ? p.scale : 0.f, lane);
+    if (qi >= p.N) return;
+    if (!CAUSAL && qi < p.rows)
+        put<float, DH>(p.ws_q + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * DH, acc, 1.f, lane);
+    else
+        put<T, DH>((T*)p.dq + b * p.dq_b + (long)qi * p.dq_n + h * p.dq_h, acc, qi < n ? p.scale : 0.f, lane);
+}
+template <typename T, int DH>
+__device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, int b, int n) {
+    using S = Shape<T, DH>;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int chunk = x % p.chunks, qa = x / p.chunks * 32, qi = qa + (lane & 31);
+    char* Ks = lds + wave * 2 * 32 * S::ROW;
+    char* Vs = Ks + 32 * S::ROW;
+    const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
+    const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
+    const bool mine = qi < n && qi < p.sinks;
+    Kept<T, DH> q, d_o;
+    q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, mine);
+    d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, mine);
+    const long st = ((long)b * p.Hq + h) * p.N + qi;
+    const float lse = mine ? p.lse[st] : INFINITY, delta = mine ? p.delta[st] : 0.f;      // not mine: probabilities of 0
+    const float sc = p.scale * LOG2E;
+    f32x16 acc[DH / 32] = {};
+    const int q0 = qa / TQ * TQ;
+    const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
+    const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
+        stage_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
+        stage_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
+        wave_lds_fence();
+        f32x16 s = product<DH>(Ks, 0, q, lane);
+        const f32x16 dp = product<DH>(Vs, 0, d_o, lane);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] - delta);
+            s[r] = k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) < n ? x : 0.f;      // of no key it may be infinite
+        }
+        gather<DH>(acc, Ks, 0, s, lane, T{});
+        wave_lds_fence();
+    }
+    const long stride = (long)(p.chunks + 1) * DH;
+    add_waves<DH>(lds, acc, p.ws_q + (((long)b * p.Hq + h) * p.rows + qa) * stride + chunk * DH, stride, tid);
+}
+template <typename T, int DH, bool CAUSAL>
+__global__ __launch_bounds__(256, 1) void slide_dq_kernel(Slide p) {
+    extern __shared__ __align__(16) char lds[];
+    const Item it = item_of(p, p.Hq, (p.N + TQ - 1) / TQ);
+    if (it.none) return;
+    const int n = length_of(p, it.b);
+    if constexpr (!CAUSAL)
+        if (it.far) return dq_far<T, DH>(p, lds, it.x, it.h, it.b, n);
+    dq_band<T, DH, CAUSAL>(p, lds, it.x * TQ, it.h, it.b, n);
 }
 
-// One workgroup: 128 keys of one (sequence, key head); the queries of every head that shares it stream through LDS.
+// 32 x 32 scores, their probabilities and score gradients, and what they add to dV and dK: rows of the tile are queries,
+// columns keys.  `ok(row, s)`: whether the pair is visible, asked only when `masked`.
+template <typename T, int DH, typename F>
+__device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const float* lse, const float* delta, int sub,
+                                         const Kept<T, DH>& k, const Kept<T, DH>& v, f32x16* dk, f32x16* dv, float sc, int lane,
+                                         bool masked, F ok) {
+    f32x16 s = product<DH>(Qs, sub, k, lane);
+    f32x16 dp = product<DH>(Os, sub, v, lane);
+#pragma unroll
+    for (int bb = 0; bb < 4; ++bb) {
+        const int r0 = sub + 8 * bb + 4 * (lane >> 5);
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(lse + r0);
+        const f32x4 de = *reinterpret_cast<const f32x4*>(delta + r0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = 4 * bb + e;
+            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -ls[e]));
+            if (masked && !ok(r0 + e)) x = 0.f;
+            s[r] = x;
+            dp[r] = x * (dp[r] - de[e]);
+        }
+    }
+    gather<DH>(dv, Os, sub, s, lane, T{});
+    gather<DH>(dk, Qs, sub, dp, lane, T{});
+}
+// Band: 128 keys of one (sequence, key head); the queries of every head that shares it stream through LDS.
 template <typename T, int DH, bool CAUSAL>
-__global__ __launch_bounds__(256, 1) void slide_dkv_kernel(Slide p) {
+__device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int hk, int b, int n) {
     using S = Shape<T, DH>;
-    extern __shared__ __align__(16) char lds[];
     char* Qs = lds;
     char* Os = lds + S::KT * S::ROW;
     float* Ls = reinterpret_cast<float*>(lds + 2 * S::KT * S::ROW);     // [KT] lse, [KT] delta
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int hk = blockIdx.y, b = blockIdx.z;
-    const int n = length_of(p, b);
-    const int k0 = blockIdx.x * TQ, ka = k0 + wave * 32, kj = ka + (lane & 31);
+    const int ka = k0 + wave * 32, kj = ka + (lane & 31);
     Kept<T, DH> k, v;
     k.load((const T*)p.k + b * p.k_b + hk * p.k_h + (long)kj * p.k_n, lane >> 5, kj < n);
     v.load((const T*)p.v + b * p.v_b + hk * p.v_h + (long)kj * p.v_n, lane >> 5, kj < n);
@@ -388,30 +618,83 @@ __global__ __launch_bounds__(256, 1) void slide_dkv_kernel(Slide p) {
                 const int qa = q0 + sub;
                 const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
                 if (cov == 0) continue;
-                f32x16 s = product<DH>(Qs, sub, k, lane);
-                f32x16 dp = product<DH>(Os, sub, v, lane);
-#pragma unroll
-                for (int bb = 0; bb < 4; ++bb) {
-                    const int r0 = sub + 8 * bb + 4 * (lane >> 5);
-                    const f32x4 ls = *reinterpret_cast<const f32x4*>(Ls + r0);
-                    const f32x4 de = *reinterpret_cast<const f32x4*>(Ls + S::KT + r0);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * bb + e;
-                        float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -ls[e]));
-                        if (cov == 1 && !visible<CAUSAL>(q0 + r0 + e, kj, n, p.window, p.sinks)) x = 0.f;
-                        s[r] = x;
-                        dp[r] = x * (dp[r] - de[e]);
-                    }
-                }
-                gather<DH>(dv, Os, sub, s, lane, T{});
-                gather<DH>(dk, Qs, sub, dp, lane, T{});
+                dkv_tile<T, DH>(Qs, Os, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1,
+                                [&](int r) { return visible<CAUSAL>(q0 + r, kj, n, p.window, p.sinks); });
             }
         }
     }
-    if (kj < p.N) {
+    if (kj >= p.N) return;
+    if (kj < p.rows) {
+        float* rec = p.ws + ((((long)b * p.Hkv + hk) * p.rows + kj) * (p.chunks + 1) + p.chunks) * (2 * DH);
+        put<float, DH>(rec, dk, 1.f, lane);
+        put<float, DH>(rec + DH, dv, 1.f, lane);
+    } else {
         put<T, DH>((T*)p.dk + b * p.dk_b + (long)kj * p.dk_n + hk * p.dk_h, dk, kj < n ? p.scale : 0.f, lane);
         put<T, DH>((T*)p.dv + b * p.dv_b + (long)kj * p.dv_n + hk * p.dv_h, dv, kj < n ? 1.f : 0.f, lane);
+    }
+}
+// Far: 32 first keys against every (4 chunks)-th 32 queries behind their band, of every head that shares them.
+template <typename T, int DH, bool CAUSAL>
+__device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk, int b, int n) {
+    using S = Shape<T, DH>;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int chunk = x % p.chunks, ka = x / p.chunks * 32, kj = ka + (lane & 31);
+    char* Qs = lds + wave * (2 * 32 * S::ROW + 256);
+    char* Os = Qs + 32 * S::ROW;
+    float* Ls = reinterpret_cast<float*>(Os + 32 * S::ROW);             // [32] lse, [32] delta
+    const bool mine = kj < n && kj < p.sinks;
+    Kept<T, DH> k, v;
+    k.load((const T*)p.k + b * p.k_b + hk * p.k_h + (long)kj * p.k_n, lane >> 5, mine);
+    v.load((const T*)p.v + b * p.v_b + hk * p.v_h + (long)kj * p.v_n, lane >> 5, mine);
+    const float sc = p.scale * LOG2E;
+    f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
+    const int k0 = ka / TQ * TQ;
+    const Tiles tl = query_tiles<CAUSAL>(k0, k0 + TQ - 1, n, p.window, p.sinks, S::KT);
+    const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    const int per = ka < n && from < n ? (n - from + 31) / 32 : 0;
+    for (int t = chunk * 4 + wave; t < per * p.G; t += p.chunks * 4) {
+        const int h = hk * p.G + t / per, q0 = from + t % per * 32;
+        const long st = ((long)b * p.Hq + h) * p.N + q0;
+        stage_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, lane);
+        stage_wave<T, DH>(Os, (const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n, q0, n, lane);
+        const int r = lane & 31;
+        Ls[lane] = q0 + r < n ? (lane < 32 ? p.lse[st + r] : p.delta[st + r]) : (lane < 32 ? INFINITY : 0.f);
+        wave_lds_fence();
+        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, !mine, [](int) { return false; });
+        wave_lds_fence();
+    }
+    const long stride = (long)(p.chunks + 1) * 2 * DH;
+    float* rec = p.ws + (((long)b * p.Hkv + hk) * p.rows + ka) * stride + chunk * 2 * DH;
+    add_waves<DH>(lds, dk, rec, stride, tid);
+    add_waves<DH>(lds, dv, rec + DH, stride, tid);
+}
+template <typename T, int DH, bool CAUSAL>
+__global__ __launch_bounds__(256, 1) void slide_dkv_kernel(Slide p) {
+    extern __shared__ __align__(16) char lds[];
+    const Item it = item_of(p, p.Hkv, (p.N + TQ - 1) / TQ);
+    if (it.none) return;
+    const int n = length_of(p, it.b);
+    if (it.far) dkv_far<T, DH, CAUSAL>(p, lds, it.x, it.h, it.b, n);
+    else dkv_band<T, DH, CAUSAL>(p, lds, it.x * TQ, it.h, it.b, n);
+}
+// The records of the first rows become gradients: blockIdx.y < Hkv dk and dv, behind them dq (if it has records).
+template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_bwd_join_kernel(Slide p, int kv_heads) {
+    const int i = blockIdx.x, b = blockIdx.z, d = threadIdx.x;
+    if (d >= DH) return;
+    const bool there = i < length_of(p, b);
+    const int h = (int)blockIdx.y - kv_heads;
+    if (h < 0) {
+        const int hk = blockIdx.y;
+        const float* rec = p.ws + (((long)b * p.Hkv + hk) * p.rows + i) * (p.chunks + 1) * (2 * DH) + d;
+        float k = 0.f, v = 0.f;
+        for (int s = 0; s <= p.chunks; ++s) { k += rec[s * 2 * DH]; v += rec[s * 2 * DH + DH]; }
+        ((T*)p.dk)[b * p.dk_b + i * p.dk_n + hk * p.dk_h + d] = (T)(there ? k * p.scale : 0.f);
+        ((T*)p.dv)[b * p.dv_b + i * p.dv_n + hk * p.dv_h + d] = (T)(there ? v : 0.f);
+    } else {
+        const float* rec = p.ws_q + (((long)b * p.Hq + h) * p.rows + i) * (p.chunks + 1) * DH + d;
+        float q = 0.f;
+        for (int s = 0; s <= p.chunks; ++s) q += rec[s * DH];
+        ((T*)p.dq)[b * p.dq_b + i * p.dq_n + h * p.dq_h + d] = (T)(there ? q * p.scale : 0.f);
     }
 }
 
@@ -451,17 +734,8 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
     for (int t = split * 4 + wave; t < tf + tw; t += p.splits * 4) {
         const int k0 = t < tf ? t * 32 : back + (t - tf) * 32;
         const int end = t < tf ? f : n;
-#pragma unroll
-        for (int i = 0; i < 32 * S::CHUNKS / 64; ++i) {
-            const int idx = lane + i * 64, row = idx / S::CHUNKS, ch = idx % S::CHUNKS;
-            u32x4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
-            if (k0 + row < end) {
-                x = *reinterpret_cast<const u32x4*>(K + (long)(k0 + row) * p.k_n + ch * (16 / (int)sizeof(T)));
-                y = *reinterpret_cast<const u32x4*>(V + (long)(k0 + row) * p.v_n + ch * (16 / (int)sizeof(T)));
-            }
-            *reinterpret_cast<u32x4*>(Ks + row * S::ROW + ch * 16) = x;
-            *reinterpret_cast<u32x4*>(Vs + row * S::ROW + ch * 16) = y;
-        }
+stage_wave<T, DH>(Ks, K, p.k_n, k0, end, lane);
+        stage_wave<T, DH>(Vs, V, p.v_n, k0, end, lane);
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
         if (k0 + 32 > end) {
@@ -475,30 +749,9 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
         gather<DH>(acc, Vs, 0, s, lane, T{});
         wave_lds_fence();
     }
-    // the four waves' sums side by side: [wave][32 heads][DH + 2]
-    float l = sm.total();
-    const float m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
-    __syncthreads();
-    constexpr int W = DH + 4;
-    float* out = reinterpret_cast<float*>(lds);
-    float* mine = out + (wave * 32 + (lane & 31)) * W;
-    put<float, DH>(mine, acc, 1.f, lane);
-    if (lane < 32) { mine[DH] = m; mine[DH + 1] = l; }
-    __syncthreads();
-    for (int idx = tid; idx < 32 * DH; idx += 256) {
-        const int c = idx / DH, d = idx % DH;
-        if (g0 + c >= p.G) continue;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, out[(w * 32 + c) * W + DH]);
-        float x = 0.f, sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float* rec = out + (w * 32 + c) * W;
-            const float e = rec[DH] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(rec[DH] - top);
-            x += rec[d] * e;
-            sum += rec[DH + 1] * e;
-        }
+    const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
+    join_waves<DH>(lds, acc, m, l, tid, [&](int c, int d, float x, float top, float sum) {
+        if (g0 + c >= p.G) return;
         const long row = (long)b * p.Hq + hk * p.G + g0 + c;
         if (p.splits == 1) {
             ((T*)p.o)[row * DH + d] = (T)(sum > 0.f ? x / sum : 0.f);
@@ -507,7 +760,7 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
             rec[d] = x;
             if (d == 0) { rec[DH] = top; rec[DH + 1] = sum; }
         }
-    }
+    });
 }
 template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_join_kernel(Decode p) {
     const long row = blockIdx.x;
@@ -531,33 +784,95 @@ template <typename K> int allow_lds(K kernel, int bytes) {
     if (bytes <= 64 * 1024) return 0;
     return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
-template <typename T, int DH, bool CAUSAL> int run_fwd(const Slide& p, hipStream_t st) {
-    const int bytes = 2 * Shape<T, DH>::KT * Shape<T, DH>::ROW;
+// Records of the first tokens: rows (a multiple of 32; 0: none needed), chunks of far items for each 32 of them, and floats
+// of workspace.  A chunk gives each wave about 8 far tiles, fewer chunks where there are items enough without them.
+struct Records { int rows, chunks; long floats; };
+Records records_of(int B, int N, int heads, int G, int width, int window, int sinks) {
+    Records r{0, 0, 0};
+    if (sinks <= 0 || window >= N) return r;
+    r.rows = (sinks + 31) / 32 * 32;
+    const long far = (long)G * ((N + 31) / 32), items = (long)B * heads * (r.rows / 32);
+    const long most = (2048 + items - 1) / items;
+    r.chunks = (int)((far + 31) / 32);
+    if (r.chunks > most) r.chunks = (int)most;
+    if (r.chunks > 512) r.chunks = 512;
+    r.floats = (long)B * heads * r.rows * (r.chunks + 1) * width;
+    return r;
+}
+// Window and sinks of N tokens without what they cannot tell apart: all visible is a window of N.
+void reach(const vitk_slide_attn* a, int& window, int& sinks) {
+    window = a->window < a->N ? a->window : a->N;
+    sinks = a->sinks;
+    if (sinks >= a->N) window = a->N;
+    if (window >= a->N) sinks = 0;
+}
+unsigned grid_of(Slide& p, int heads, bool far) {
+    p.far_items = far ? p.chunks * (p.rows / 32) * heads * p.B : 0;
+    const long bands = (long)vitk_ceil_div(p.N, TQ) * heads * p.B;
+    p.items = (int)(p.far_items + bands);
+    return (unsigned)(p.far_items + (bands + 7) / 8 * 8);
+}
+template <typename T, int DH> constexpr int lds_bytes(bool far, bool backward) {
+    const int band = 2 * Shape<T, DH>::KT * Shape<T, DH>::ROW + (backward ? 2 * Shape<T, DH>::KT * 4 : 0);
+    const int staged = 4 * (2 * 32 * Shape<T, DH>::ROW + (backward ? 256 : 0));
+    const int joined = join_bytes<DH>(), wide = staged > joined ? staged : joined;
+    return far && wide > band ? wide : band;
+}
+template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipStream_t st) {
+    if (!CAUSAL) {
+        const Records r = records_of(p.B, p.N, p.Hq, 1, DH + 4, p.window, p.sinks);
+        p.rows = r.rows; p.chunks = r.chunks; p.ws = ws;
+        if (r.rows && !ws) return VITK_ERR_NULL;
+    }
+    const int bytes = lds_bytes<T, DH>(p.rows > 0, false);
     if (int e = allow_lds(slide_fwd_kernel<T, DH, CAUSAL>, bytes)) return e;
-    hipLaunchKernelGGL((slide_fwd_kernel<T, DH, CAUSAL>), dim3(vitk_ceil_div(p.N, TQ), p.Hq, p.B), dim3(256), bytes, st, p);
+    const unsigned grid = grid_of(p, p.Hq, p.rows > 0);
+    hipLaunchKernelGGL((slide_fwd_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
     VITK_CHECK_LAUNCH();
+    if (p.rows) {
+        hipLaunchKernelGGL((slide_fwd_join_kernel<T, DH>), dim3(p.rows < p.N ? p.rows : p.N, p.Hq, p.B), dim3(DH < 64 ? 64 : DH), 0, st, p);
+        VITK_CHECK_LAUNCH();
+    }
     return 0;
 }
-template <typename T, int DH, bool CAUSAL> int run_bwd(const Slide& p, const float* o32, hipStream_t st) {
-    const int bytes = 2 * Shape<T, DH>::KT * Shape<T, DH>::ROW + 2 * Shape<T, DH>::KT * (int)sizeof(float);
+template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, const float* o32, float* ws, hipStream_t st) {
+    const Records rk = records_of(p.B, p.N, p.Hkv, p.G, 2 * DH, p.window, p.sinks);
+    const Records rq = CAUSAL ? Records{0, 0, 0} : records_of(p.B, p.N, p.Hq, 1, DH, p.window, p.sinks);
+    if (rk.rows && !ws) return VITK_ERR_NULL;
+    const int bytes = lds_bytes<T, DH>(rk.rows > 0, true);
     if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL>, bytes)) return e;
     if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL>, bytes)) return e;
     const long rows = (long)p.B * p.N * p.Hq;
     hipLaunchKernelGGL((slide_delta_kernel<T, DH>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, o32);
     VITK_CHECK_LAUNCH();
-    const int tiles = vitk_ceil_div(p.N, TQ);
+    p.ws = ws;
+    p.ws_q = ws + rk.floats;
+    const dim3 join(DH < 64 ? 64 : DH);
+    const unsigned first = (unsigned)(rk.rows < p.N ? rk.rows : p.N);
     if (p.dk) {
-        hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL>), dim3(tiles, p.Hkv, p.B), dim3(256), bytes, st, p);
+        p.rows = rk.rows; p.chunks = rk.chunks;
+        const unsigned grid = grid_of(p, p.Hkv, rk.rows > 0);
+        hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
         VITK_CHECK_LAUNCH();
+        if (p.rows) {
+            hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(first, p.Hkv, p.B), join, 0, st, p, p.Hkv);
+            VITK_CHECK_LAUNCH();
+        }
     }
     if (p.dq) {
-        hipLaunchKernelGGL((slide_dq_kernel<T, DH, CAUSAL>), dim3(tiles, p.Hq, p.B), dim3(256), bytes, st, p);
+        p.rows = rq.rows; p.chunks = rq.chunks;
+        const unsigned grid = grid_of(p, p.Hq, rq.rows > 0);
+        hipLaunchKernelGGL((slide_dq_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
         VITK_CHECK_LAUNCH();
+        if (p.rows) {
+            hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(first, p.Hq, p.B), join, 0, st, p, 0);
+            VITK_CHECK_LAUNCH();
+        }
     }
     return 0;
 }
 template <typename T, int DH> int run_decode(const Decode& p, hipStream_t st) {
-    const int tiles = 4 * 2 * 32 * Shape<T, DH>::ROW, join = 4 * 32 * (DH + 4) * (int)sizeof(float);
+    const int tiles = 4 * 2 * 32 * Shape<T, DH>::ROW, join = join_bytes<DH>();
     const int bytes = tiles > join ? tiles : join;
     if (int e = allow_lds(slide_decode_kernel<T, DH>, bytes)) return e;
     hipLaunchKernelGGL((slide_decode_kernel<T, DH>), dim3(p.splits, p.Hkv * ((p.G + 31) / 32), p.B), dim3(256), bytes, st, p);
@@ -592,8 +907,10 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     p.q_b = a->q_b; p.q_n = a->q_n; p.q_h = a->q_h;
     p.k_b = a->k_b; p.k_n = a->k_n; p.k_h = a->k_h;
     p.v_b = a->v_b; p.v_n = a->v_n; p.v_h = a->v_h;
-    p.window = a->window < a->N ? a->window : a->N;
-    p.sinks = a->sinks < a->N ? a->sinks : a->N;
+    reach(a, p.window, p.sinks);
+    if ((uintptr_t)a->workspace % 16) return VITK_ERR_SHAPE;
+    // items of a launch are counted in 31 bits
+    if (((long)a->N / TQ + 2) * a->Hq * a->B > (1L << 30)) return VITK_ERR_SHAPE;
     p.scale = a->scale;
     if (!backward) {
         if (!a->o) return VITK_ERR_NULL;
@@ -623,11 +940,25 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     if (a->dh == 64) return a->causal ? CALL(float, 64, true) : CALL(float, 64, false);                               \
     return a->causal ? CALL(float, 128, true) : CALL(float, 128, false)
 
+extern "C" size_t vitk_slide_attn_workspace(const vitk_slide_attn* a, int backward) {
+    if (!a || a->B <= 0 || a->N <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->dh <= 0) return 0;
+    int window, sinks;
+    reach(a, window, sinks);
+    long n = 0;
+    if (!backward) {
+        if (!a->causal) n = records_of(a->B, a->N, a->Hq, 1, a->dh + 4, window, sinks).floats;
+    } else {
+        n = records_of(a->B, a->N, a->Hkv, a->Hq / a->Hkv, 2 * a->dh, window, sinks).floats;
+        if (!a->causal) n += records_of(a->B, a->N, a->Hq, 1, a->dh, window, sinks).floats;
+    }
+    return (size_t)n * sizeof(float);
+}
+
 extern "C" int vitk_slide_attn_fwd(const vitk_slide_attn* a, int dtype, void* stream) {
     Slide p;
     if (int e = fill(a, dtype, false, p)) return e;
     hipStream_t st = (hipStream_t)stream;
-#define FWD(T, DH, C) run_fwd<T, DH, C>(p, st)
+#define FWD(T, DH, C) run_fwd<T, DH, C>(p, a->workspace, st)
     SLIDE_FORMS(FWD);
 }
 
@@ -636,7 +967,7 @@ extern "C" int vitk_slide_attn_bwd(const vitk_slide_attn* a, int dtype, void* st
     if (int e = fill(a, dtype, true, p)) return e;
     hipStream_t st = (hipStream_t)stream;
     const float* o32 = dtype == VITK_BF16 ? a->o_f32 : (const float*)a->o;
-#define BWD(T, DH, C) run_bwd<T, DH, C>(p, o32, st)
+#define BWD(T, DH, C) run_bwd<T, DH, C>(p, o32, a->workspace, st)
     SLIDE_FORMS(BWD);
 }
 
