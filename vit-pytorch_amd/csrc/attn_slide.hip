@@ -41,6 +41,7 @@ struct Slide {
     int chunks;                // far items of each 32 of them; a row has chunks + 1 records, the band's last
     float* ws;                 // forward: records of dh + 2; backward: dk | dv, then dq, records of dh
     float* ws_q;
+    int tk;                    // keys of a band of the dK / dV kernel
     int far_items, items;      // of this launch: far ones come first, then bands
 };
 
@@ -122,17 +123,15 @@ template <int DH> struct Kept<float, DH> {
         }
     }
 };
-// 32 tile rows from r0 times the kept rows, over the head: C[row][column].
-template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<bf16_t, DH>& kept, int lane) {
-    f32x16 acc = {};
+// 32 tile rows from r0 times the kept rows, over the head, on top of acc: C[row][column].
+template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<bf16_t, DH>& kept, int lane, f32x16 acc = {}) {
     const char* a = tile + (r0 + (lane & 31)) * Shape<bf16_t, DH>::ROW + (lane >> 5) * 16;
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c)
         acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(a + 32 * c), kept.f[c], acc, 0, 0, 0);
     return acc;
 }
-template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<float, DH>& kept, int lane) {
-    f32x16 acc = {};
+template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<float, DH>& kept, int lane, f32x16 acc = {}) {
     const char* a = tile + (r0 + (lane & 31)) * Shape<float, DH>::ROW + (lane >> 5) * (DH * 2);
 #pragma unroll
     for (int t = 0; t < DH / 8; ++t) {
@@ -173,28 +172,26 @@ template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char
             acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
                 *reinterpret_cast<const float*>(a + (8 * (r >> 2) + (r & 3)) * Shape<float, DH>::ROW + 128 * d), w[r], acc[d], 0, 0, 0);
 }
-// Rows [r0, r0 + KT) of a matrix into an LDS tile; rows from `end` on are zeros.
-template <typename T, int DH, int NT> __device__ __forceinline__ void stage(char* tile, const T* base, long ld, int r0, int end, int tid) {
-    constexpr int C = Shape<T, DH>::CHUNKS, ROW = Shape<T, DH>::ROW;
+// Rows of a matrix on their way into an LDS tile.  Rows behind the last one of the sequence are that one again: finite, and
+// without weight.
+template <typename T, int DH, int ROWS, int NT> struct Fetch {
+    static constexpr int C = Shape<T, DH>::CHUNKS, ROW = Shape<T, DH>::ROW;
+    u32x4 x[ROWS * C / NT];
+    __device__ __forceinline__ void load(const T* base, long ld, int r0, int n, int tid) {
 #pragma unroll
-    for (int i = 0; i < Shape<T, DH>::KT * C / NT; ++i) {
-        const int idx = tid + i * NT, row = idx / C, ch = idx % C;
-        u32x4 z = {0, 0, 0, 0};
-        if (r0 + row < end) z = *reinterpret_cast<const u32x4*>(base + (long)(r0 + row) * ld + ch * (16 / (int)sizeof(T)));
-        *reinterpret_cast<u32x4*>(tile + row * ROW + ch * 16) = z;
+        for (int i = 0; i < ROWS * C / NT; ++i) {
+            const int idx = tid + i * NT, r = r0 + idx / C;
+            x[i] = *reinterpret_cast<const u32x4*>(base + (long)(r < n ? r : n - 1) * ld + idx % C * (16 / (int)sizeof(T)));
+        }
     }
-}
-// The same for 32 rows by one wave.
-template <typename T, int DH> __device__ __forceinline__ void stage_wave(char* tile, const T* base, long ld, int r0, int end, int lane) {
-    constexpr int C = Shape<T, DH>::CHUNKS, ROW = Shape<T, DH>::ROW;
+    __device__ __forceinline__ void store(char* tile, int tid) const {
 #pragma unroll
-    for (int i = 0; i < 32 * C / 64; ++i) {
-        const int idx = lane + i * 64, row = idx / C, ch = idx % C;
-        u32x4 z = {0, 0, 0, 0};
-        if (r0 + row < end) z = *reinterpret_cast<const u32x4*>(base + (long)(r0 + row) * ld + ch * (16 / (int)sizeof(T)));
-        *reinterpret_cast<u32x4*>(tile + row * ROW + ch * 16) = z;
+        for (int i = 0; i < ROWS * C / NT; ++i) {
+            const int idx = tid + i * NT;
+            *reinterpret_cast<u32x4*>(tile + idx / C * ROW + idx % C * 16) = x[i];
+        }
     }
-}
+};
 // acc[d][column] of this lane's column, times `mul`, to a row of DH elements.
 template <typename T, int DH> __device__ __forceinline__ void put(T* row, const f32x16* acc, float mul, int lane) {
 #pragma unroll
@@ -219,27 +216,42 @@ __device__ __forceinline__ int length_of(const Slide& p, int b) {
 }
 
 // ----------------------------------------------------------------------------- softmax of a column, tile after tile
-// m: running maximum of the raw scores, l: running sum of exp2((s - m) sc), this lane half's rows only until finish().
+// m: a maximum of the raw scores, l: running sum of exp2((s - m) sc), of this lane half's rows only until total().
+__device__ __forceinline__ float max3_raw(float a, float b, float c) {      // fmaxf() would quiet every input first
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 struct Softmax {
     float m = -INFINITY, l = 0.f;
-    // s -> probabilities relative to the new maximum; returns the factor of everything before.
-    __device__ __forceinline__ float step(f32x16& s, float sc) {
-        float t = s[0];
+    // NS score tiles -> probabilities relative to m.  m follows the maximum only once that is 8 binary orders above it (in
+    // some column of the wave): until then probabilities stay below 2^8, and the accumulators need no factor, which for a
+    // head of 128 costs more than the exponentials.  `rescale(alpha)` applies it to everything before.
+    template <int NS, typename F> __device__ __forceinline__ void step(f32x16* s, float sc, F rescale) {
+        float t = -INFINITY;
 #pragma unroll
-        for (int r = 1; r < 16; ++r) t = fmaxf(t, s[r]);
-        t = fmaxf(t, __shfl_xor(t, 32, 64));
-        const float mn = fmaxf(m, t);
-        const float nb = mn == -INFINITY ? 0.f : -mn * sc;         // nothing visible yet: every term is exp2(-inf) = 0
-        const float alpha = __builtin_amdgcn_exp2f(__builtin_fmaf(m, sc, nb));
-        float sum = 0.f;
+        for (int k = 0; k < NS; ++k)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, nb));
-            sum += s[r];
+            for (int r = 0; r < 16; r += 2) t = max3_raw(t, s[k][r], s[k][r + 1]);
+        if (__any(t * sc > m * sc + 8.f)) {           // a row that has seen nothing: 0 > -inf, or -inf > -inf, which waits
+            t = fmaxf(t, __shfl_xor(t, 32, 64));
+            const float mn = fmaxf(m, t);
+            const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * sc);
+            l *= alpha;
+            m = mn;
+            rescale(alpha);
         }
-        l = l * alpha + sum;
-        m = mn;
-        return alpha;
+        const float nb = m == -INFINITY ? 0.f : -m * sc;          // nothing visible yet: every term is exp2(-inf) = 0
+#pragma unroll
+        for (int k = 0; k < NS; ++k) {
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[k][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][r], sc, nb));
+                sum += s[k][r];
+            }
+            l += sum;
+        }
     }
     __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
 };
@@ -310,13 +322,50 @@ template <int DH> __device__ __forceinline__ void add_waves(char* lds, const f32
     }
 }
 
+// Tiles of two matrices through LDS, two buffers deep: while one tile is used, the next one's loads are in flight, and one
+// barrier a tile orders the two.  use(first tile, second tile, first row).
+template <typename T, int DH, typename F>
+__device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T* B, long ldb, const Tiles& tl, int n, int tid, F use) {
+    using S = Shape<T, DH>;
+    constexpr int BYTES = S::KT * S::ROW;
+    Fetch<T, DH, S::KT, 256> fa, fb;
+    const int cnt = tl.count();
+    if (cnt > 0) {
+        fa.load(A, lda, tl.at(0) * S::KT, n, tid);
+        fb.load(B, ldb, tl.at(0) * S::KT, n, tid);
+        fa.store(lds, tid);
+        fb.store(lds + BYTES, tid);
+    }
+    for (int t = 0; t < cnt; ++t) {
+        char* now = lds + (t & 1) * 2 * BYTES;
+        char* next = lds + (~t & 1) * 2 * BYTES;
+        __syncthreads();
+        if (t + 1 < cnt) {
+            fa.load(A, lda, tl.at(t + 1) * S::KT, n, tid);
+            fb.load(B, ldb, tl.at(t + 1) * S::KT, n, tid);
+        }
+        use(now, now + BYTES, tl.at(t) * S::KT);
+        if (t + 1 < cnt) {
+            fa.store(next, tid);
+            fb.store(next + BYTES, tid);
+        }
+    }
+}
+// 32 rows of two matrices into LDS tiles of this wave alone.
+template <typename T, int DH>
+__device__ __forceinline__ void stage_wave(char* a, const T* A, long lda, char* b, const T* B, long ldb, int r0, int n, int lane) {
+    Fetch<T, DH, 32, 64> fa, fb;
+    fa.load(A, lda, r0, n, lane);
+    fb.load(B, ldb, r0, n, lane);
+    fa.store(a, lane);
+    fb.store(b, lane);
+}
+
 // ----------------------------------------------------------------------------- forward
 // Band: 128 queries of one (sequence, head), each wave 32 of them; key tiles stream through LDS.
 template <typename T, int DH, bool CAUSAL>
 __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
-    char* Ks = lds;
-    char* Vs = lds + S::KT * S::ROW;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
     const int qa = q0 + wave * 32, qi = qa + (lane & 31);
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
@@ -326,30 +375,41 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
     const float sc = p.scale * LOG2E;
     f32x16 acc[DH / 32] = {};
     Softmax sm;
-    const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    for (int t = 0; t < tl.count(); ++t) {
-        const int k0 = tl.at(t) * S::KT;
-        __syncthreads();
-        stage<T, DH, 256>(Ks, K, p.k_n, k0, n, tid);
-        stage<T, DH, 256>(Vs, V, p.v_n, k0, n, tid);
-        __syncthreads();
+    const auto rescale = [&](float alpha) {
 #pragma unroll
-        for (int sub = 0; sub < S::KT; sub += 32) {
-            const int ka = k0 + sub;
-            const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
-            if (cov == 0) continue;
-            f32x16 s = product<DH>(Ks, sub, q, lane);
-            if (cov == 1) {
+        for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
+    };
+    const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
+    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&](const char* Ks, const char* Vs, int k0) {
+        constexpr int SUBS = S::KT / 32;
+        int cov[SUBS];
+#pragma unroll
+        for (int u = 0; u < SUBS; ++u) {
+            const int ka = k0 + 32 * u;
+            cov[u] = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
+        }
+        const auto scores = [&](int u, int how) {
+            f32x16 x = product<DH>(Ks, 32 * u, q, lane);
+            if (how == 1) {
+                const int j = k0 + 32 * u + 4 * (lane >> 5);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (!visible<CAUSAL>(qi, ka + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), n, p.window, p.sinks)) s[r] = -INFINITY;
+                    if (!visible<CAUSAL>(qi, j + 8 * (r >> 2) + (r & 3), n, p.window, p.sinks)) x[r] = -INFINITY;
             }
-            const float alpha = sm.step(s, sc);
-#pragma unroll
-            for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
-            gather<DH>(acc, Vs, sub, s, lane, T{});
+            return x;
+        };
+        if (SUBS == 2 && cov[0] && cov[SUBS - 1]) {
+            f32x16 s[2] = {scores(0, cov[0]), scores(1, cov[SUBS - 1])};
+            sm.step<2>(s, sc, rescale);
+            gather<DH>(acc, Vs, 0, s[0], lane, T{});
+            gather<DH>(acc, Vs, 32, s[1], lane, T{});
+        } else if (cov[0] || cov[SUBS - 1]) {
+            const int u = cov[0] ? 0 : SUBS - 1;
+            f32x16 s = scores(u, cov[0] ? cov[0] : cov[SUBS - 1]);
+            sm.step<1>(&s, sc, rescale);
+            gather<DH>(acc, Vs, 32 * u, s, lane, T{});
         }
-    }
+    });
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
     if (qi < p.N) {
         if (!CAUSAL && qi < p.rows) {
@@ -386,16 +446,16 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
-        stage_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
-        stage_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
+        stage_wave<T, DH>(Ks, K, p.k_n, Vs, V, p.v_n, k0, n, lane);
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
             if (!mine || k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= n) s[r] = -INFINITY;
-        const float alpha = sm.step(s, sc);
+        sm.step<1>(&s, sc, [&](float alpha) {
 #pragma unroll
-        for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
+            for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
+        });
         gather<DH>(acc, Vs, 0, s, lane, T{});
         wave_lds_fence();
     }
@@ -408,7 +468,7 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
     });
 }
 template <typename T, int DH, bool CAUSAL>
-__global__ __launch_bounds__(256, 1) void slide_fwd_kernel(Slide p) {
+__global__ __launch_bounds__(256, 2) void slide_fwd_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
     const Item it = item_of(p, p.Hq, (p.N + TQ - 1) / TQ);
     if (it.none) return;
@@ -467,8 +527,6 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta
 template <typename T, int DH, bool CAUSAL>
 __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
-    char* Ks = lds;
-    char* Vs = lds + S::KT * S::ROW;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
     const int qa = q0 + wave * 32, qi = qa + (lane & 31);
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
@@ -481,12 +539,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     const float sc = p.scale * LOG2E;
     f32x16 acc[DH / 32] = {};
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    for (int t = 0; t < tl.count(); ++t) {
-        const int k0 = tl.at(t) * S::KT;
-        __syncthreads();
-        stage<T, DH, 256>(Ks, K, p.k_n, k0, n, tid);
-        stage<T, DH, 256>(Vs, V, p.v_n, k0, n, tid);
-        __syncthreads();
+    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&](const char* Ks, const char* Vs, int k0) {
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
@@ -495,14 +548,15 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
             f32x16 s = product<DH>(Ks, sub, q, lane);
             const f32x16 dp = product<DH>(Vs, sub, d_o, lane);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] - delta);
-                if (cov == 1 && !visible<CAUSAL>(qi, ka + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), n, p.window, p.sinks)) x = 0.f;
-                s[r] = x;
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] - delta);
+            if (cov == 1) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!visible<CAUSAL>(qi, ka + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), n, p.window, p.sinks)) s[r] = 0.f;
             }
             gather<DH>(acc, Ks, sub, s, lane, T{});
         }
-    }
+    });
     if (qi >= p.N) return;
     if (!CAUSAL && qi < p.rows)
         put<float, DH>(p.ws_q + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * DH, acc, 1.f, lane);
@@ -530,8 +584,7 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
-        stage_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
-        stage_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
+        stage_wave<T, DH>(Ks, K, p.k_n, Vs, V, p.v_n, k0, n, lane);
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
         const f32x16 dp = product<DH>(Vs, 0, d_o, lane);
@@ -547,7 +600,7 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     add_waves<DH>(lds, acc, p.ws_q + (((long)b * p.Hq + h) * p.rows + qa) * stride + chunk * DH, stride, tid);
 }
 template <typename T, int DH, bool CAUSAL>
-__global__ __launch_bounds__(256, 1) void slide_dq_kernel(Slide p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void slide_dq_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
     const Item it = item_of(p, p.Hq, (p.N + TQ - 1) / TQ);
     if (it.none) return;
@@ -558,70 +611,108 @@ __global__ __launch_bounds__(256, 1) void slide_dq_kernel(Slide p) {
 }
 
 // 32 x 32 scores, their probabilities and score gradients, and what they add to dV and dK: rows of the tile are queries,
-// columns keys.  `ok(row, s)`: whether the pair is visible, asked only when `masked`.
+// columns keys; nls, nde: the rows' negative lse and delta (the second product starts from the latter).  `ok(row)`:
+// whether the pair is visible, asked only when `masked`.
 template <typename T, int DH, typename F>
-__device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const float* lse, const float* delta, int sub,
+__device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const float* nls, const float* nde, int sub,
                                          const Kept<T, DH>& k, const Kept<T, DH>& v, f32x16* dk, f32x16* dv, float sc, int lane,
                                          bool masked, F ok) {
-    f32x16 s = product<DH>(Qs, sub, k, lane);
-    f32x16 dp = product<DH>(Os, sub, v, lane);
+    const int r0 = sub + 4 * (lane >> 5);
+    f32x16 s = product<DH>(Qs, sub, k, lane), dp;
 #pragma unroll
-    for (int bb = 0; bb < 4; ++bb) {
-        const int r0 = sub + 8 * bb + 4 * (lane >> 5);
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(lse + r0);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(delta + r0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int r = 4 * bb + e;
-            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -ls[e]));
-            if (masked && !ok(r0 + e)) x = 0.f;
-            s[r] = x;
-            dp[r] = x * (dp[r] - de[e]);
-        }
+    for (int r = 0; r < 16; r += 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(nde + r0 + 2 * r);
+        dp[r] = x[0]; dp[r + 1] = x[1]; dp[r + 2] = x[2]; dp[r + 3] = x[3];
     }
+    dp = product<DH>(Os, sub, v, lane, dp);
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(nls + r0 + 2 * r);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], sc, x[e]));
+    }
+    if (masked) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (!ok(r0 + 8 * (r >> 2) + (r & 3))) s[r] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] *= s[r];
     gather<DH>(dv, Os, sub, s, lane, T{});
     gather<DH>(dk, Qs, sub, dp, lane, T{});
 }
-// Band: 128 keys of one (sequence, key head); the queries of every head that shares it stream through LDS.
-template <typename T, int DH, bool CAUSAL>
+// Band: 32 KG keys of one (sequence, key head); the queries of every head that shares it stream through LDS.  Wave w keeps
+// keys 32 (w % KG); with KG = 2 the other two waves take every second 32 queries and the halves are added at the end.
+template <typename T, int DH, bool CAUSAL, int KG>
 __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int hk, int b, int n) {
     using S = Shape<T, DH>;
-    char* Qs = lds;
-    char* Os = lds + S::KT * S::ROW;
-    float* Ls = reinterpret_cast<float*>(lds + 2 * S::KT * S::ROW);     // [KT] lse, [KT] delta
+    constexpr int BYTES = S::KT * S::ROW, BUF = 2 * BYTES + 2 * S::KT * 4;      // Q, dO, -lse, -delta
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int ka = k0 + wave * 32, kj = ka + (lane & 31);
+    const int ka = k0 + wave % KG * 32, kj = ka + (lane & 31), part = wave / KG;
     Kept<T, DH> k, v;
     k.load((const T*)p.k + b * p.k_b + hk * p.k_h + (long)kj * p.k_n, lane >> 5, kj < n);
     v.load((const T*)p.v + b * p.v_b + hk * p.v_h + (long)kj * p.v_n, lane >> 5, kj < n);
     const float sc = p.scale * LOG2E;
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
-    const Tiles tl = query_tiles<CAUSAL>(k0, k0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    for (int g = 0; g < p.G; ++g) {
-        const int h = hk * p.G + g;
-        const T* Q = (const T*)p.q + b * p.q_b + h * p.q_h;
-        const T* DO = (const T*)p.d_o + b * p.do_b + h * p.do_h;
-        const long st = ((long)b * p.Hq + h) * p.N;
-        for (int t = 0; t < tl.count(); ++t) {
-            const int q0 = tl.at(t) * S::KT;
-            __syncthreads();
-            stage<T, DH, 256>(Qs, Q, p.q_n, q0, n, tid);
-            stage<T, DH, 256>(Os, DO, p.do_n, q0, n, tid);
-            if (tid < S::KT) {
-                const int i = q0 + tid;
-                Ls[tid] = i < n ? p.lse[st + i] : INFINITY;
-                Ls[S::KT + tid] = i < n ? p.delta[st + i] : 0.f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int sub = 0; sub < S::KT; sub += 32) {
-                const int qa = q0 + sub;
-                const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
-                if (cov == 0) continue;
-                dkv_tile<T, DH>(Qs, Os, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1,
-                                [&](int r) { return visible<CAUSAL>(q0 + r, kj, n, p.window, p.sinks); });
-            }
+    const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
+    const int per = tl.count(), cnt = per * p.G;
+    Fetch<T, DH, S::KT, 256> fq, fo;
+    float fl = 0.f;
+    const auto load = [&](int t) {
+        const int h = hk * p.G + t / per, q0 = tl.at(t % per) * S::KT;
+        fq.load((const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, tid);
+        fo.load((const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n, q0, n, tid);
+        if (tid < 2 * S::KT) {
+            const int i = q0 + (tid < S::KT ? tid : tid - S::KT);
+            fl = -(tid < S::KT ? p.lse : p.delta)[((long)b * p.Hq + h) * p.N + (i < n ? i : n - 1)];
+            if (i >= n) fl = tid < S::KT ? -INFINITY : 0.f;
         }
+    };
+    const auto store = [&](char* buf) {
+        fq.store(buf, tid);
+        fo.store(buf + BYTES, tid);
+        if (tid < 2 * S::KT) reinterpret_cast<float*>(buf + 2 * BYTES)[tid] = fl;
+    };
+    if (cnt > 0) {
+        load(0);
+        store(lds);
+    }
+    for (int t = 0; t < cnt; ++t) {
+        const char* now = lds + (t & 1) * BUF;
+        __syncthreads();
+        if (t + 1 < cnt) load(t + 1);
+        const int q0 = tl.at(t % per) * S::KT;
+        const float* Ls = reinterpret_cast<const float*>(now + 2 * BYTES);
+#pragma unroll
+        for (int sub = 0; sub < S::KT; sub += 32) {
+            if (KG == 2 && (((S::KT > 32 ? sub / 32 : t) + part) & 1)) continue;
+            const int qa = q0 + sub;
+            const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
+            if (cov == 0) continue;
+            dkv_tile<T, DH>(now, now + BYTES, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1,
+                            [&](int r) { return visible<CAUSAL>(q0 + r, kj, n, p.window, p.sinks); });
+        }
+        if (t + 1 < cnt) store(lds + (~t & 1) * BUF);
+    }
+    if constexpr (KG == 2) {
+        constexpr int W = DH + 4;
+        static_assert(64 * 2 * W * 4 <= 2 * BUF, "the halves meet in the tiles' buffers");
+        float* at = reinterpret_cast<float*>(lds) + (wave % 2 * 32 + (lane & 31)) * 2 * W;
+        __syncthreads();
+        if (part) {
+            put<float, DH>(at, dk, 1.f, lane);
+            put<float, DH>(at + W, dv, 1.f, lane);
+        }
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int c = 32 * d + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                dk[d][r] += at[c];
+                dv[d][r] += at[W + c];
+            }
     }
     if (kj >= p.N) return;
     if (kj < p.rows) {
@@ -648,17 +739,17 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     v.load((const T*)p.v + b * p.v_b + hk * p.v_h + (long)kj * p.v_n, lane >> 5, mine);
     const float sc = p.scale * LOG2E;
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
-    const int k0 = ka / TQ * TQ;
-    const Tiles tl = query_tiles<CAUSAL>(k0, k0 + TQ - 1, n, p.window, p.sinks, S::KT);
+    const int k0 = ka / p.tk * p.tk;
+    const Tiles tl = query_tiles<CAUSAL>(k0, k0 + p.tk - 1, n, p.window, p.sinks, S::KT);
     const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     const int per = ka < n && from < n ? (n - from + 31) / 32 : 0;
     for (int t = chunk * 4 + wave; t < per * p.G; t += p.chunks * 4) {
         const int h = hk * p.G + t / per, q0 = from + t % per * 32;
         const long st = ((long)b * p.Hq + h) * p.N + q0;
-        stage_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, lane);
-        stage_wave<T, DH>(Os, (const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n, q0, n, lane);
+        stage_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, Os, (const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n,
+                          q0, n, lane);
         const int r = lane & 31;
-        Ls[lane] = q0 + r < n ? (lane < 32 ? p.lse[st + r] : p.delta[st + r]) : (lane < 32 ? INFINITY : 0.f);
+        Ls[lane] = q0 + r < n ? -(lane < 32 ? p.lse : p.delta)[st + r] : (lane < 32 ? -INFINITY : 0.f);
         wave_lds_fence();
         dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, !mine, [](int) { return false; });
         wave_lds_fence();
@@ -668,14 +759,14 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     add_waves<DH>(lds, dk, rec, stride, tid);
     add_waves<DH>(lds, dv, rec + DH, stride, tid);
 }
-template <typename T, int DH, bool CAUSAL>
+template <typename T, int DH, bool CAUSAL, int KG>
 __global__ __launch_bounds__(256, 1) void slide_dkv_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
-    const Item it = item_of(p, p.Hkv, (p.N + TQ - 1) / TQ);
+    const Item it = item_of(p, p.Hkv, (p.N + 32 * KG - 1) / (32 * KG));
     if (it.none) return;
     const int n = length_of(p, it.b);
     if (it.far) dkv_far<T, DH, CAUSAL>(p, lds, it.x, it.h, it.b, n);
-    else dkv_band<T, DH, CAUSAL>(p, lds, it.x * TQ, it.h, it.b, n);
+    else dkv_band<T, DH, CAUSAL, KG>(p, lds, it.x * (32 * KG), it.h, it.b, n);
 }
 // The records of the first rows become gradients: blockIdx.y < Hkv dk and dv, behind them dq (if it has records).
 template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_bwd_join_kernel(Slide p, int kv_heads) {
@@ -734,8 +825,7 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
     for (int t = split * 4 + wave; t < tf + tw; t += p.splits * 4) {
         const int k0 = t < tf ? t * 32 : back + (t - tf) * 32;
         const int end = t < tf ? f : n;
-stage_wave<T, DH>(Ks, K, p.k_n, k0, end, lane);
-        stage_wave<T, DH>(Vs, V, p.v_n, k0, end, lane);
+        stage_wave<T, DH>(Ks, K, p.k_n, Vs, V, p.v_n, k0, end, lane);
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
         if (k0 + 32 > end) {
@@ -743,9 +833,10 @@ stage_wave<T, DH>(Ks, K, p.k_n, k0, end, lane);
             for (int r = 0; r < 16; ++r)
                 if (k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= end) s[r] = -INFINITY;
         }
-        const float alpha = sm.step(s, sc);
+        sm.step<1>(&s, sc, [&](float alpha) {
 #pragma unroll
-        for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
+            for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
+        });
         gather<DH>(acc, Vs, 0, s, lane, T{});
         wave_lds_fence();
     }
@@ -806,14 +897,14 @@ void reach(const vitk_slide_attn* a, int& window, int& sinks) {
     if (sinks >= a->N) window = a->N;
     if (window >= a->N) sinks = 0;
 }
-unsigned grid_of(Slide& p, int heads, bool far) {
+unsigned grid_of(Slide& p, int heads, bool far, int rows = TQ) {
     p.far_items = far ? p.chunks * (p.rows / 32) * heads * p.B : 0;
-    const long bands = (long)vitk_ceil_div(p.N, TQ) * heads * p.B;
+    const long bands = (long)vitk_ceil_div(p.N, rows) * heads * p.B;
     p.items = (int)(p.far_items + bands);
     return (unsigned)(p.far_items + (bands + 7) / 8 * 8);
 }
 template <typename T, int DH> constexpr int lds_bytes(bool far, bool backward) {
-    const int band = 2 * Shape<T, DH>::KT * Shape<T, DH>::ROW + (backward ? 2 * Shape<T, DH>::KT * 4 : 0);
+    const int band = 2 * (2 * Shape<T, DH>::KT * Shape<T, DH>::ROW + (backward ? 2 * Shape<T, DH>::KT * 4 : 0));
     const int staged = 4 * (2 * 32 * Shape<T, DH>::ROW + (backward ? 256 : 0));
     const int joined = join_bytes<DH>(), wide = staged > joined ? staged : joined;
     return far && wide > band ? wide : band;
@@ -841,7 +932,8 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, const float* o32
     if (rk.rows && !ws) return VITK_ERR_NULL;
     const int bytes = lds_bytes<T, DH>(rk.rows > 0, true);
     if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL>, bytes)) return e;
-    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL>, bytes)) return e;
+    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, 4>, bytes)) return e;
+    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, 2>, bytes)) return e;
     const long rows = (long)p.B * p.N * p.Hq;
     hipLaunchKernelGGL((slide_delta_kernel<T, DH>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, o32);
     VITK_CHECK_LAUNCH();
@@ -851,8 +943,12 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, const float* o32
     const unsigned first = (unsigned)(rk.rows < p.N ? rk.rows : p.N);
     if (p.dk) {
         p.rows = rk.rows; p.chunks = rk.chunks;
-        const unsigned grid = grid_of(p, p.Hkv, rk.rows > 0);
-        hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
+        // few key heads leave CUs without a band of 128 keys: bands of 64 below two of them for each CU
+        const bool narrow = (long)vitk_ceil_div(p.N, TQ) * p.Hkv * p.B < 512;
+        p.tk = narrow ? 64 : 128;
+        const unsigned grid = grid_of(p, p.Hkv, rk.rows > 0, p.tk);
+        if (narrow) hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, 2>), dim3(grid), dim3(256), bytes, st, p);
+        else hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, 4>), dim3(grid), dim3(256), bytes, st, p);
         VITK_CHECK_LAUNCH();
         if (p.rows) {
             hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(first, p.Hkv, p.B), join, 0, st, p, p.Hkv);
