@@ -46,11 +46,38 @@ struct Slide {
 };
 
 // ----------------------------------------------------------------------------- which pairs are visible
-template <bool CAUSAL> __device__ __forceinline__ bool visible(int i, int j, int n, int w, int f) {
-    if (i >= n || j >= n) return false;
-    if constexpr (CAUSAL) return j <= i && (i - j < w || j < f);
-    const int d = i - j;
-    return (d < w && -d < w) || j < f || i < f;
+// What one row sees of the other axis: len rows from lo on, and the rows before f.
+struct Span {
+    int lo, len, f;
+    __device__ __forceinline__ bool sees(int x) const { return (unsigned)(x - lo) < (unsigned)len || x < f; }
+};
+__device__ __forceinline__ Span span(int lo, int hi, int f) { return Span{lo, hi >= lo ? hi - lo + 1 : 0, f}; }
+__device__ __forceinline__ int least(int a, int b) { return a < b ? a : b; }
+template <bool CAUSAL> __device__ __forceinline__ Span keys_of(int i, int n, int w, int f) {
+    if (i >= n) return Span{0, 0, 0};
+    if (CAUSAL) return span(w > 0 ? i - w + 1 : i + 1, i, least(f, i + 1));
+    if (i < f) return Span{0, n, 0};
+    return span(w > 0 ? i - w + 1 : n, least(i + w, n) - 1, least(f, n));
+}
+template <bool CAUSAL> __device__ __forceinline__ Span queries_of(int j, int n, int w, int f) {
+    if (j >= n) return Span{0, 0, 0};
+    if (CAUSAL) return span(j, j < f ? n - 1 : least(j + w, n) - 1, 0);
+    if (j < f) return Span{0, n, 0};
+    return span(w > 0 ? j - w + 1 : n, least(j + w, n) - 1, least(f, n));
+}
+// s[r] of the rows that are not seen; register r holds row x0 + 8 (r / 4) + r % 4.  `first`: whether rows before f may be
+// among them.
+__device__ __forceinline__ void hide(f32x16& s, const Span& v, int x0, bool first, float with) {
+    const int d = x0 - v.lo;
+    if (first) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (!v.sees(x0 + 8 * (r >> 2) + (r & 3))) s[r] = with;
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if ((unsigned)(d + 8 * (r >> 2) + (r & 3)) >= (unsigned)v.len) s[r] = with;
+    }
 }
 // Of the rectangle [ia, ib] x [ja, jb]: 0 nothing is visible, 2 everything is, 1 look at each pair.
 template <bool CAUSAL> __device__ __forceinline__ int coverage(int ia, int ib, int ja, int jb, int n, int w, int f) {
@@ -93,10 +120,21 @@ template <bool CAUSAL> __device__ __forceinline__ Tiles query_tiles(int ka, int 
 }
 
 // ----------------------------------------------------------------------------- operands
+// An LDS tile: rows one behind the other, the 16-byte chunks of a row in an order of its own, so that what 16 lanes read
+// side by side lies in all 64 banks: chunk c of row r at place c ^ mix(r).  Read are one chunk of 16 rows in a row (all
+// mixes of 16 rows differ, as far as a row has chunks), and, transposed, 64 bytes of four rows (bf16: the mixes of rows
+// 0 ... 3 differ in the bits above those 64 bytes) or 128 bytes of rows r and r + 4 (fp32).
 template <typename T, int DH> struct Shape {
-    static constexpr int ROW = DH * (int)sizeof(T) + 16;          // bytes of an LDS tile row: 16 of padding
-    static constexpr int CHUNKS = DH * (int)sizeof(T) / 16;
+    static constexpr int ROW = DH * (int)sizeof(T);
+    static constexpr int CHUNKS = ROW / 16;
     static constexpr int KT = sizeof(T) == 2 ? 64 : 32;           // rows of a staged tile
+    static constexpr int PER = ROW >= 256 ? 1 : 256 / ROW;        // rows in 64 banks
+    static __device__ __forceinline__ int mix(int r) {
+        if constexpr (sizeof(T) == 2) return ((r & 3) / PER << 2) | ((r >> 2) & 3);
+        else if constexpr (PER == 2) return (r >> 1) & 7;
+        else return ((r >> 2) & 1) << 3 | ((r >> 3) & 1) << 2 | (r & 3);
+    }
+    static __device__ __forceinline__ int at(int r, int chunk) { return r * ROW + ((chunk ^ mix(r)) << 4); }
 };
 // What a wave keeps of its 32 rows: column lane & 31, half h of the reduction.
 template <typename T, int DH> struct Kept;
@@ -125,17 +163,19 @@ template <int DH> struct Kept<float, DH> {
 };
 // 32 tile rows from r0 times the kept rows, over the head, on top of acc: C[row][column].
 template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<bf16_t, DH>& kept, int lane, f32x16 acc = {}) {
-    const char* a = tile + (r0 + (lane & 31)) * Shape<bf16_t, DH>::ROW + (lane >> 5) * 16;
+    const int a = Shape<bf16_t, DH>::at(lane & 31, lane >> 5);
+    tile += r0 * Shape<bf16_t, DH>::ROW;
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c)
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(a + 32 * c), kept.f[c], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(tile + (a ^ (c << 5))), kept.f[c], acc, 0, 0, 0);
     return acc;
 }
 template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<float, DH>& kept, int lane, f32x16 acc = {}) {
-    const char* a = tile + (r0 + (lane & 31)) * Shape<float, DH>::ROW + (lane >> 5) * (DH * 2);
+    const int a = Shape<float, DH>::at(lane & 31, (lane >> 5) * (DH / 8));
+    tile += r0 * Shape<float, DH>::ROW;
 #pragma unroll
     for (int t = 0; t < DH / 8; ++t) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a + 16 * t);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(tile + (a ^ (t << 4)));
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], kept.f[4 * t + i], acc, 0, 0, 0);
     }
@@ -144,51 +184,95 @@ template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, in
 // acc[d][column] += sum over 32 tile rows from r0 of tile[row][d] * w[row][column]; w as a product left it.  In bf16
 // the weights are rounded to the operand type here: 2^-9 of each, independent, and the sums stay in 32 bits.
 template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, bf16_t) {
+    using S = Shape<bf16_t, DH>;
     const int l15 = lane & 15, g = lane >> 4;
     bf16x8 b[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) b[c][e] = (bf16_t)w[8 * c + e];
-    const char* a = tile + (r0 + 4 * (g >> 1) + (l15 >> 2)) * Shape<bf16_t, DH>::ROW + (16 * (g & 1) + 4 * (l15 & 3)) * 2;
+    // the transposing read takes 8 bytes of rows r ... r + 3 from each 16 lanes
+    const int r = 4 * (g >> 1) + (l15 >> 2), ch = 2 * (g & 1) + ((l15 & 3) >> 1), half = (l15 & 1) * 8;
+    const int a0 = S::at(r, ch) + half, a1 = S::at(r + 8, ch) + half;
+    tile += r0 * S::ROW;
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const char* p = a + 16 * c * Shape<bf16_t, DH>::ROW + 64 * d;
-            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((VITK_LDS bf16x4*)(p));
-            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((VITK_LDS bf16x4*)(p + 8 * Shape<bf16_t, DH>::ROW));
+            const char* t = tile + 16 * c * S::ROW;
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((VITK_LDS bf16x4*)(t + (a0 ^ (d << 6))));
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((VITK_LDS bf16x4*)(t + (a1 ^ (d << 6))));
             acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]},
                                                              b[c], acc[d], 0, 0, 0);
         }
     }
 }
 template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, float) {
-    const char* a = tile + (r0 + 4 * (lane >> 5)) * Shape<float, DH>::ROW + (lane & 31) * 4;
+    using S = Shape<float, DH>;
+    const int ch = (lane & 31) >> 2, low = (lane & 3) * 4;
+    tile += r0 * S::ROW;
 #pragma unroll
-    for (int d = 0; d < DH / 32; ++d)
+    for (int r = 0; r < 16; ++r) {
+        const int a = S::at(8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), ch) + low;
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-                *reinterpret_cast<const float*>(a + (8 * (r >> 2) + (r & 3)) * Shape<float, DH>::ROW + 128 * d), w[r], acc[d], 0, 0, 0);
+        for (int d = 0; d < DH / 32; ++d)
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*reinterpret_cast<const float*>(tile + (a ^ (d << 7))), w[r], acc[d], 0, 0, 0);
+    }
 }
-// Rows of a matrix on their way into an LDS tile.  Rows behind the last one of the sequence are that one again: finite, and
-// without weight.
-template <typename T, int DH, int ROWS, int NT> struct Fetch {
-    static constexpr int C = Shape<T, DH>::CHUNKS, ROW = Shape<T, DH>::ROW;
-    u32x4 x[ROWS * C / NT];
-    __device__ __forceinline__ void load(const T* base, long ld, int r0, int n, int tid) {
+// Rows behind the last one of the sequence are staged as that one again: finite, and without weight.
+//
+// Straight into LDS, 16 bytes a lane in the order of the lanes: each lane fetches the chunk that belongs at its place.  By all
+// four waves (`voff`: where this thread's chunks lie from the tile's first row on.
+__device__ __forceinline__ void dma16(const void* base, int off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* from, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(VITK_LDS const char*)p; }
+template <typename T, int DH> struct Stage {
+    using S = Shape<T, DH>;
+    static constexpr int PARTS = S::KT * S::CHUNKS / 256;
+    int voff[PARTS];
+    int ld;
+    __device__ __forceinline__ static int place(int i, int tid) { return i * 256 + tid; }
+    __device__ __forceinline__ int offset(int i, int tid, int last) const {
+        const int pl = place(i, tid), r = pl / S::CHUNKS, ch = (pl % S::CHUNKS) ^ S::mix(r);
+        return (r < last ? r : last) * ld * (int)sizeof(T) + ch * 16;
+    }
+    __device__ __forceinline__ Stage(long stride, int tid) : ld((int)stride) {
 #pragma unroll
-        for (int i = 0; i < ROWS * C / NT; ++i) {
-            const int idx = tid + i * NT, r = r0 + idx / C;
-            x[i] = *reinterpret_cast<const u32x4*>(base + (long)(r < n ? r : n - 1) * ld + idx % C * (16 / (int)sizeof(T)));
+        for (int i = 0; i < PARTS; ++i) voff[i] = offset(i, tid, S::KT);
+    }
+    __device__ __forceinline__ void start(char* tile, const T* base, int r0, int n, int tid) const {
+        const T* from = base + (long)r0 * ld;
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds_addr(tile) + (tid & ~63) * 16);
+        if (r0 + S::KT <= n) {
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) dma16(from, voff[i], to + i * 4096);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) dma16(from, offset(i, tid, n - 1 - r0), to + i * 4096);
         }
     }
-    __device__ __forceinline__ void store(char* tile, int tid) const {
+};
+// By one wave, through its registers.
+template <typename T, int DH> struct Fetch {
+    using S = Shape<T, DH>;
+    u32x4 x[32 * S::CHUNKS / 64];
+    __device__ __forceinline__ void load(const T* base, long ld, int r0, int n, int lane) {
 #pragma unroll
-        for (int i = 0; i < ROWS * C / NT; ++i) {
-            const int idx = tid + i * NT;
-            *reinterpret_cast<u32x4*>(tile + idx / C * ROW + idx % C * 16) = x[i];
+        for (int i = 0; i < 32 * S::CHUNKS / 64; ++i) {
+            const int idx = lane + i * 64, r = r0 + idx / S::CHUNKS;
+            x[i] = *reinterpret_cast<const u32x4*>(base + (long)(r < n ? r : n - 1) * ld + idx % S::CHUNKS * (16 / (int)sizeof(T)));
+        }
+    }
+    __device__ __forceinline__ void store(char* tile, int lane) const {
+#pragma unroll
+        for (int i = 0; i < 32 * S::CHUNKS / 64; ++i) {
+            const int idx = lane + i * 64;
+            *reinterpret_cast<u32x4*>(tile + S::at(idx / S::CHUNKS, idx % S::CHUNKS)) = x[i];
         }
     }
 };
@@ -284,7 +368,7 @@ template <int DH> constexpr int join_bytes() { return 4 * 32 * (DH + 4) * (int)s
 // One record of the softmax of a row from the four waves': called by all threads, f(column, d, sum, maximum, total).
 template <int DH, typename F> __device__ __forceinline__ void join_waves(char* lds, const f32x16* acc, float m, float l, int tid, F f) {
     constexpr int W = DH + 4;
-    const int lane = tid & 63, wave = tid >> 6;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* out = reinterpret_cast<float*>(lds);
     float* mine = out + (wave * 32 + (lane & 31)) * W;
     __syncthreads();
@@ -310,7 +394,7 @@ template <int DH, typename F> __device__ __forceinline__ void join_waves(char* l
 // The plain sum of the four waves', to records `stride` floats apart.
 template <int DH> __device__ __forceinline__ void add_waves(char* lds, const f32x16* acc, float* rec, long stride, int tid) {
     constexpr int W = DH + 4;
-    const int lane = tid & 63, wave = tid >> 6;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* out = reinterpret_cast<float*>(lds);
     __syncthreads();
     put<float, DH>(out + (wave * 32 + (lane & 31)) * W, acc, 1.f, lane);
@@ -322,43 +406,40 @@ template <int DH> __device__ __forceinline__ void add_waves(char* lds, const f32
     }
 }
 
-// Tiles of two matrices through LDS, two buffers deep: while one tile is used, the next one's loads are in flight, and one
+// Tiles of two matrices through LDS, two buffers deep: while one tile is used, the next one is on its way, and one
 // barrier a tile orders the two.  use(first tile, second tile, first row).
 template <typename T, int DH, typename F>
 __device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T* B, long ldb, const Tiles& tl, int n, int tid, F use) {
     using S = Shape<T, DH>;
     constexpr int BYTES = S::KT * S::ROW;
-    Fetch<T, DH, S::KT, 256> fa, fb;
+    const Stage<T, DH> fa(lda, tid), fb(ldb, tid);
     const int cnt = tl.count();
     if (cnt > 0) {
-        fa.load(A, lda, tl.at(0) * S::KT, n, tid);
-        fb.load(B, ldb, tl.at(0) * S::KT, n, tid);
-        fa.store(lds, tid);
-        fb.store(lds + BYTES, tid);
+        fa.start(lds, A, tl.at(0) * S::KT, n, tid);
+        fb.start(lds + BYTES, B, tl.at(0) * S::KT, n, tid);
     }
     for (int t = 0; t < cnt; ++t) {
         char* now = lds + (t & 1) * 2 * BYTES;
         char* next = lds + (~t & 1) * 2 * BYTES;
+        dma_wait();
         __syncthreads();
         if (t + 1 < cnt) {
-            fa.load(A, lda, tl.at(t + 1) * S::KT, n, tid);
-            fb.load(B, ldb, tl.at(t + 1) * S::KT, n, tid);
+            fa.start(next, A, tl.at(t + 1) * S::KT, n, tid);
+            fb.start(next + BYTES, B, tl.at(t + 1) * S::KT, n, tid);
         }
         use(now, now + BYTES, tl.at(t) * S::KT);
-        if (t + 1 < cnt) {
-            fa.store(next, tid);
-            fb.store(next + BYTES, tid);
-        }
     }
 }
-// 32 rows of two matrices into LDS tiles of this wave alone.
-template <typename T, int DH>
-__device__ __forceinline__ void stage_wave(char* a, const T* A, long lda, char* b, const T* B, long ldb, int r0, int n, int lane) {
-    Fetch<T, DH, 32, 64> fa, fb;
-    fa.load(A, lda, r0, n, lane);
-    fb.load(B, ldb, r0, n, lane);
-    fa.store(a, lane);
-    fb.store(b, lane);
+// 32 rows from r0 of a matrix into an LDS tile of this wave alone.
+template <typename T, int DH> __device__ __forceinline__ void start_wave(char* tile, const T* base, long ld, int r0, int n, int lane) {
+    using S = Shape<T, DH>;
+    const unsigned to = __builtin_amdgcn_readfirstlane(lds_addr(tile));
+    const T* from = base + r0 * ld;
+#pragma unroll
+    for (int i = 0; i < 32 * S::CHUNKS / 64; ++i) {
+        const int pl = i * 64 + lane, r = pl / S::CHUNKS, ch = (pl % S::CHUNKS) ^ S::mix(r);
+        dma16(from, (r0 + r < n ? r : n - 1 - r0) * (int)ld * (int)sizeof(T) + ch * 16, to + i * 1024);
+    }
 }
 
 // ----------------------------------------------------------------------------- forward
@@ -366,13 +447,14 @@ __device__ __forceinline__ void stage_wave(char* a, const T* A, long lda, char* 
 template <typename T, int DH, bool CAUSAL>
 __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
     const int qa = q0 + wave * 32, qi = qa + (lane & 31);
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
     Kept<T, DH> q;
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, qi < n);
     const float sc = p.scale * LOG2E;
+    const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
     Softmax sm;
     const auto rescale = [&](float alpha) {
@@ -390,12 +472,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         }
         const auto scores = [&](int u, int how) {
             f32x16 x = product<DH>(Ks, 32 * u, q, lane);
-            if (how == 1) {
-                const int j = k0 + 32 * u + 4 * (lane >> 5);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!visible<CAUSAL>(qi, j + 8 * (r >> 2) + (r & 3), n, p.window, p.sinks)) x[r] = -INFINITY;
-            }
+            if (how == 1) hide(x, sp, k0 + 32 * u + 4 * (lane >> 5), k0 + 32 * u < p.sinks, -INFINITY);
             return x;
         };
         if (SUBS == 2 && cov[0] && cov[SUBS - 1]) {
@@ -430,7 +507,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
 template <typename T, int DH>
 __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h, int b, int n) {
     using S = Shape<T, DH>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
     const int chunk = x % p.chunks, qa = x / p.chunks * 32, qi = qa + (lane & 31);
     char* Ks = lds + wave * 2 * 32 * S::ROW;
     char* Vs = Ks + 32 * S::ROW;
@@ -446,12 +523,12 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
-        stage_wave<T, DH>(Ks, K, p.k_n, Vs, V, p.v_n, k0, n, lane);
+        start_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
+        start_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
+        dma_wait();
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if (!mine || k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= n) s[r] = -INFINITY;
+        hide(s, Span{0, mine ? n : 0, 0}, k0 + 4 * (lane >> 5), false, -INFINITY);
         sm.step<1>(&s, sc, [&](float alpha) {
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
@@ -499,7 +576,7 @@ template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) vo
 }
 
 // ----------------------------------------------------------------------------- backward
-// delta = dO . o, one wave per four rows of a (sequence, head); o in 32 bits, so that what the rounded output lost is
+// delta = -dO . o, one wave per four rows of a (sequence, head); o in 32 bits, so that what the rounded output lost is
 // not multiplied by the cancellation in dP - delta.
 template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta_kernel(Slide p, const float* o32) {
     const int lane = threadIdx.x & 15;
@@ -521,13 +598,13 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (r < rows && lane == 0) p.delta[((long)b * p.Hq + h) * p.N + i] = s;
+    if (r < rows && lane == 0) p.delta[((long)b * p.Hq + h) * p.N + i] = -s;
 }
 
 template <typename T, int DH, bool CAUSAL>
 __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
     const int qa = q0 + wave * 32, qi = qa + (lane & 31);
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
@@ -535,8 +612,9 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, qi < n);
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, qi < n);
     const long st = ((long)b * p.Hq + h) * p.N + qi;
-    const float lse = qi < n ? p.lse[st] : INFINITY, delta = qi < n ? p.delta[st] : 0.f;
+    const float lse = qi < n ? p.lse[st] : INFINITY, delta = qi < n ? p.delta[st] : 0.f;      // delta: negative
     const float sc = p.scale * LOG2E;
+    const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&](const char* Ks, const char* Vs, int k0) {
@@ -548,12 +626,8 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
             f32x16 s = product<DH>(Ks, sub, q, lane);
             const f32x16 dp = product<DH>(Vs, sub, d_o, lane);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] - delta);
-            if (cov == 1) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!visible<CAUSAL>(qi, ka + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), n, p.window, p.sinks)) s[r] = 0.f;
-            }
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
+            if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, 0.f);
             gather<DH>(acc, Ks, sub, s, lane, T{});
         }
     });
@@ -566,7 +640,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
 template <typename T, int DH>
 __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, int b, int n) {
     using S = Shape<T, DH>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hk = h / p.G;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
     const int chunk = x % p.chunks, qa = x / p.chunks * 32, qi = qa + (lane & 31);
     char* Ks = lds + wave * 2 * 32 * S::ROW;
     char* Vs = Ks + 32 * S::ROW;
@@ -584,15 +658,15 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
-        stage_wave<T, DH>(Ks, K, p.k_n, Vs, V, p.v_n, k0, n, lane);
+        start_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
+        start_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
+        dma_wait();
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
         const f32x16 dp = product<DH>(Vs, 0, d_o, lane);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] - delta);
-            s[r] = k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) < n ? x : 0.f;      // of no key it may be infinite
-        }
+        for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
+        hide(s, Span{0, n, 0}, k0 + 4 * (lane >> 5), false, 0.f);
         gather<DH>(acc, Ks, 0, s, lane, T{});
         wave_lds_fence();
     }
@@ -611,31 +685,27 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void slide_dq_kernel(S
 }
 
 // 32 x 32 scores, their probabilities and score gradients, and what they add to dV and dK: rows of the tile are queries,
-// columns keys; nls, nde: the rows' negative lse and delta (the second product starts from the latter).  `ok(row)`:
-// whether the pair is visible, asked only when `masked`.
-template <typename T, int DH, typename F>
-__device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const float* nls, const float* nde, int sub,
+// columns keys; lse, delta: the rows' (the second product starts from the negative delta).  x0: the query of the tile's
+// first row for this lane's half, for `masked` tiles.
+template <typename T, int DH>
+__device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const float* lse, const float* delta, int sub,
                                          const Kept<T, DH>& k, const Kept<T, DH>& v, f32x16* dk, f32x16* dv, float sc, int lane,
-                                         bool masked, F ok) {
+                                         bool masked, const Span& sp, int x0, bool first) {
     const int r0 = sub + 4 * (lane >> 5);
     f32x16 s = product<DH>(Qs, sub, k, lane), dp;
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(nde + r0 + 2 * r);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(delta + r0 + 2 * r);
         dp[r] = x[0]; dp[r + 1] = x[1]; dp[r + 2] = x[2]; dp[r + 3] = x[3];
     }
     dp = product<DH>(Os, sub, v, lane, dp);
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(nls + r0 + 2 * r);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(lse + r0 + 2 * r);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], sc, x[e]));
+        for (int e = 0; e < 4; ++e) s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], sc, -x[e]));
     }
-    if (masked) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if (!ok(r0 + 8 * (r >> 2) + (r & 3))) s[r] = 0.f;
-    }
+    if (masked) hide(s, sp, x0, first, 0.f);
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] *= s[r];
     gather<DH>(dv, Os, sub, s, lane, T{});
@@ -647,7 +717,7 @@ template <typename T, int DH, bool CAUSAL, int KG>
 __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int hk, int b, int n) {
     using S = Shape<T, DH>;
     constexpr int BYTES = S::KT * S::ROW, BUF = 2 * BYTES + 2 * S::KT * 4;      // Q, dO, -lse, -delta
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ka = k0 + wave % KG * 32, kj = ka + (lane & 31), part = wave / KG;
     Kept<T, DH> k, v;
     k.load((const T*)p.k + b * p.k_b + hk * p.k_h + (long)kj * p.k_n, lane >> 5, kj < n);
@@ -656,32 +726,27 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
     const int per = tl.count(), cnt = per * p.G;
-    Fetch<T, DH, S::KT, 256> fq, fo;
-    float fl = 0.f;
-    const auto load = [&](int t) {
-        const int h = hk * p.G + t / per, q0 = tl.at(t % per) * S::KT;
-        fq.load((const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, tid);
-        fo.load((const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n, q0, n, tid);
-        if (tid < 2 * S::KT) {
-            const int i = q0 + (tid < S::KT ? tid : tid - S::KT);
-            fl = -(tid < S::KT ? p.lse : p.delta)[((long)b * p.Hq + h) * p.N + (i < n ? i : n - 1)];
-            if (i >= n) fl = tid < S::KT ? -INFINITY : 0.f;
+    const Span sp = queries_of<CAUSAL>(kj, n, p.window, p.sinks);
+    const Stage<T, DH> fq(p.q_n, tid), fo(p.do_n, tid);
+    int next_g = 0, next_t = 0;
+    const auto start = [&](char* buf) {                 // the tiles in order, head after head
+        const int h = hk * p.G + next_g, q0 = tl.at(next_t) * S::KT;
+        fq.start(buf, (const T*)p.q + b * p.q_b + h * p.q_h, q0, n, tid);
+        fo.start(buf + BYTES, (const T*)p.d_o + b * p.do_b + h * p.do_h, q0, n, tid);
+        if (wave < 2 * S::KT / 64) {                    // the rows' lse, delta: rows behind the sequence are masked
+            const int x = wave * 64 + lane, i = q0 + x % S::KT;
+            const float* from = (x < S::KT ? p.lse : p.delta) + ((long)b * p.Hq + h) * p.N + (i < n ? i : n - 1);
+            dma4(from, __builtin_amdgcn_readfirstlane(lds_addr(buf + 2 * BYTES) + wave * 256));
         }
+        if (++next_t == per) { next_t = 0; ++next_g; }
     };
-    const auto store = [&](char* buf) {
-        fq.store(buf, tid);
-        fo.store(buf + BYTES, tid);
-        if (tid < 2 * S::KT) reinterpret_cast<float*>(buf + 2 * BYTES)[tid] = fl;
-    };
-    if (cnt > 0) {
-        load(0);
-        store(lds);
-    }
-    for (int t = 0; t < cnt; ++t) {
+    if (cnt > 0) start(lds);
+    for (int t = 0, tt = 0; t < cnt; ++t, tt = tt + 1 == per ? 0 : tt + 1) {
         const char* now = lds + (t & 1) * BUF;
+        dma_wait();
         __syncthreads();
-        if (t + 1 < cnt) load(t + 1);
-        const int q0 = tl.at(t % per) * S::KT;
+        if (t + 1 < cnt) start(lds + (~t & 1) * BUF);
+        const int q0 = tl.at(tt) * S::KT;
         const float* Ls = reinterpret_cast<const float*>(now + 2 * BYTES);
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
@@ -689,30 +754,27 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
             const int qa = q0 + sub;
             const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
             if (cov == 0) continue;
-            dkv_tile<T, DH>(now, now + BYTES, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1,
-                            [&](int r) { return visible<CAUSAL>(q0 + r, kj, n, p.window, p.sinks); });
+            dkv_tile<T, DH>(now, now + BYTES, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1, sp, qa + 4 * (lane >> 5),
+                            !CAUSAL && qa < p.sinks);
         }
-        if (t + 1 < cnt) store(lds + (~t & 1) * BUF);
     }
     if constexpr (KG == 2) {
         constexpr int W = DH + 4;
-        static_assert(64 * 2 * W * 4 <= 2 * BUF, "the halves meet in the tiles' buffers");
-        float* at = reinterpret_cast<float*>(lds) + (wave % 2 * 32 + (lane & 31)) * 2 * W;
-        __syncthreads();
-        if (part) {
-            put<float, DH>(at, dk, 1.f, lane);
-            put<float, DH>(at + W, dv, 1.f, lane);
-        }
-        __syncthreads();
+        static_assert(64 * W * 4 <= 2 * BUF, "the halves meet in the tiles' buffers");
+        float* at = reinterpret_cast<float*>(lds) + (wave % 2 * 32 + (lane & 31)) * W;
+        const auto meet = [&](f32x16* acc) {
+            __syncthreads();
+            if (part) put<float, DH>(at, acc, 1.f, lane);
+            __syncthreads();
+            if (part) return;
+#pragma unroll
+            for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] += at[32 * d + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3)];
+        };
+        meet(dk);
+        meet(dv);
         if (part) return;
-#pragma unroll
-        for (int d = 0; d < DH / 32; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int c = 32 * d + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                dk[d][r] += at[c];
-                dv[d][r] += at[W + c];
-            }
     }
     if (kj >= p.N) return;
     if (kj < p.rows) {
@@ -728,7 +790,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
 template <typename T, int DH, bool CAUSAL>
 __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk, int b, int n) {
     using S = Shape<T, DH>;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int chunk = x % p.chunks, ka = x / p.chunks * 32, kj = ka + (lane & 31);
     char* Qs = lds + wave * (2 * 32 * S::ROW + 256);
     char* Os = Qs + 32 * S::ROW;
@@ -746,12 +808,13 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     for (int t = chunk * 4 + wave; t < per * p.G; t += p.chunks * 4) {
         const int h = hk * p.G + t / per, q0 = from + t % per * 32;
         const long st = ((long)b * p.Hq + h) * p.N + q0;
-        stage_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, Os, (const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n,
-                          q0, n, lane);
+        start_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, lane);
+        start_wave<T, DH>(Os, (const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n, q0, n, lane);
         const int r = lane & 31;
-        Ls[lane] = q0 + r < n ? -(lane < 32 ? p.lse : p.delta)[st + r] : (lane < 32 ? -INFINITY : 0.f);
+        Ls[lane] = (lane < 32 ? p.lse : p.delta)[st + (q0 + r < n ? r : n - 1 - q0)];
+        dma_wait();
         wave_lds_fence();
-        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, !mine, [](int) { return false; });
+        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, Span{0, mine ? n : 0, 0}, q0 + 4 * (lane >> 5), false);
         wave_lds_fence();
     }
     const long stride = (long)(p.chunks + 1) * 2 * DH;
@@ -760,7 +823,7 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     add_waves<DH>(lds, dv, rec + DH, stride, tid);
 }
 template <typename T, int DH, bool CAUSAL, int KG>
-__global__ __launch_bounds__(256, 1) void slide_dkv_kernel(Slide p) {
+__global__ __launch_bounds__(256, sizeof(T) == 2 && DH < 128 ? 2 : 1) void slide_dkv_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
     const Item it = item_of(p, p.Hkv, (p.N + 32 * KG - 1) / (32 * KG));
     if (it.none) return;
@@ -804,7 +867,7 @@ template <typename T, int DH>
 __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
     using S = Shape<T, DH>;
     extern __shared__ __align__(16) char lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int groups = (p.G + 31) / 32;
     const int split = blockIdx.x, hk = blockIdx.y / groups, g0 = (blockIdx.y % groups) * 32, b = blockIdx.z;
     const int g = g0 + (lane & 31);
@@ -825,7 +888,11 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
     for (int t = split * 4 + wave; t < tf + tw; t += p.splits * 4) {
         const int k0 = t < tf ? t * 32 : back + (t - tf) * 32;
         const int end = t < tf ? f : n;
-        stage_wave<T, DH>(Ks, K, p.k_n, Vs, V, p.v_n, k0, end, lane);
+        Fetch<T, DH> fk, fv;
+        fk.load(K, p.k_n, k0, end, lane);
+        fv.load(V, p.v_n, k0, end, lane);
+        fk.store(Ks, lane);
+        fv.store(Vs, lane);
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
         if (k0 + 32 > end) {
@@ -1004,6 +1071,9 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     p.k_b = a->k_b; p.k_n = a->k_n; p.k_h = a->k_h;
     p.v_b = a->v_b; p.v_n = a->v_n; p.v_h = a->v_h;
     reach(a, p.window, p.sinks);
+    // a tile's rows are addressed with 32 bits from its first one on
+    for (long ld : {a->q_n, a->k_n, a->v_n, backward ? a->do_n : 0L})
+        if (ld < 0 || ld >= (1L << 23)) return VITK_ERR_SHAPE;
     if ((uintptr_t)a->workspace % 16) return VITK_ERR_SHAPE;
     // items of a launch are counted in 31 bits
     if (((long)a->N / TQ + 2) * a->Hq * a->B > (1L << 30)) return VITK_ERR_SHAPE;

@@ -46,9 +46,10 @@ def _one_device(what, *ts):
 
 
 def _rows(t):
-    """`t` as the kernels address it: consecutive elements inside a head, pointer and strides multiples of 16 bytes."""
+    """`t` as the kernels address it: consecutive elements inside a head, pointer and strides multiples of 16 bytes, tokens
+    less than 2^23 elements apart."""
     e = t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in t.stride()[:-1]):
+    if t.stride(-1) == 1 and t.stride(1) < 1 << 23 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in t.stride()[:-1]):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
