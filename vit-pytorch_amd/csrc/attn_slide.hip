@@ -68,6 +68,7 @@ template <bool CAUSAL> __device__ __forceinline__ Span queries_of(int j, int n, 
 // s[r] of the rows that are not seen; register r holds row x0 + 8 (r / 4) + r % 4.  `first`: whether rows before f may be
 // among them.
 __device__ __forceinline__ void hide(f32x16& s, const Span& v, int x0, bool first, float with) {
+    asm volatile("");          // a branch, not selects: most tiles have nothing to hide
     const int d = x0 - v.lo;
     if (first) {
 #pragma unroll
@@ -136,6 +137,20 @@ template <typename T, int DH> struct Shape {
     }
     static __device__ __forceinline__ int at(int r, int chunk) { return r * ROW + ((chunk ^ mix(r)) << 4); }
 };
+// x has arrived.  Without this the compiler would wait for it at its first use inside a loop, and with it, at every turn, for
+// all that the loop has on its way into LDS.
+template <typename X> __device__ __forceinline__ void arrived(X& x) { asm volatile("" : "+v"(x)); }
+// The order of a run of N products that each read READS times from LDS: a few reads ahead of the products.
+template <int N, int READS> __device__ __forceinline__ void reads_ahead() {
+    constexpr int AHEAD = N < 4 ? N : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD * READS, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
 // What a wave keeps of its 32 rows: column lane & 31, half h of the reduction.
 template <typename T, int DH> struct Kept;
 template <int DH> struct Kept<bf16_t, DH> {
@@ -147,6 +162,10 @@ template <int DH> struct Kept<bf16_t, DH> {
             if (ok) z = *reinterpret_cast<const u32x4*>(row + 16 * c + 8 * h);
             f[c] = __builtin_bit_cast(bf16x8, z);
         }
+    }
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) arrived(f[c]);
     }
 };
 template <int DH> struct Kept<float, DH> {
@@ -160,6 +179,10 @@ template <int DH> struct Kept<float, DH> {
             for (int i = 0; i < 4; ++i) f[4 * t + i] = z[i];
         }
     }
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int i = 0; i < DH / 2; ++i) arrived(f[i]);
+    }
 };
 // 32 tile rows from r0 times the kept rows, over the head, on top of acc: C[row][column].
 template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<bf16_t, DH>& kept, int lane, f32x16 acc = {}) {
@@ -168,6 +191,7 @@ template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, in
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c)
         acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(tile + (a ^ (c << 5))), kept.f[c], acc, 0, 0, 0);
+    reads_ahead<DH / 16, 1>();
     return acc;
 }
 template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<float, DH>& kept, int lane, f32x16 acc = {}) {
@@ -206,6 +230,7 @@ template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char
                                                              b[c], acc[d], 0, 0, 0);
         }
     }
+    reads_ahead<DH / 16, 2>();
 }
 template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, float) {
     using S = Shape<float, DH>;
@@ -223,11 +248,12 @@ template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char
 //
 // Straight into LDS, 16 bytes a lane in the order of the lanes: each lane fetches the chunk that belongs at its place.  By all
 // four waves (`voff`: where this thread's chunks lie from the tile's first row on.
+// (s_nop: the base may come from a vector instruction, which the compiler does not see either.)
 __device__ __forceinline__ void dma16(const void* base, int off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
 __device__ __forceinline__ void dma4(const void* from, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(VITK_LDS const char*)p; }
@@ -301,22 +327,22 @@ __device__ __forceinline__ int length_of(const Slide& p, int b) {
 
 // ----------------------------------------------------------------------------- softmax of a column, tile after tile
 // m: a maximum of the raw scores, l: running sum of exp2((s - m) sc), of this lane half's rows only until total().
-__device__ __forceinline__ float max3_raw(float a, float b, float c) {      // fmaxf() would quiet every input first
+// fmaxf() would quiet every input first.  The compiler does not wait for a matrix instruction's result in front of assembly:
+// `a` has to come from an instruction of its own that read the same result.
+__device__ __forceinline__ float max3_raw(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
 struct Softmax {
     float m = -INFINITY, l = 0.f;
-    // NS score tiles -> probabilities relative to m.  m follows the maximum only once that is 8 binary orders above it (in
-    // some column of the wave): until then probabilities stay below 2^8, and the accumulators need no factor, which for a
-    // head of 128 costs more than the exponentials.  `rescale(alpha)` applies it to everything before.
-    template <int NS, typename F> __device__ __forceinline__ void step(f32x16* s, float sc, F rescale) {
-        float t = -INFINITY;
+    // Scores -> probabilities relative to m.  m follows the maximum only once that is 8 binary orders above it (in some
+    // column of the wave): until then probabilities stay below 2^8, and the accumulators need no factor, which for a head
+    // of 128 costs more than the exponentials.  `rescale(alpha)` applies it to everything before.
+    template <typename F> __device__ __forceinline__ void step(f32x16& s, float sc, F rescale) {
+        float t = fmaxf(s[0], s[1]);
 #pragma unroll
-        for (int k = 0; k < NS; ++k)
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) t = max3_raw(t, s[k][r], s[k][r + 1]);
+        for (int r = 2; r < 16; r += 2) t = max3_raw(t, s[r], s[r + 1]);
         if (__any(t * sc > m * sc + 8.f)) {           // a row that has seen nothing: 0 > -inf, or -inf > -inf, which waits
             t = fmaxf(t, __shfl_xor(t, 32, 64));
             const float mn = fmaxf(m, t);
@@ -326,16 +352,13 @@ struct Softmax {
             rescale(alpha);
         }
         const float nb = m == -INFINITY ? 0.f : -m * sc;          // nothing visible yet: every term is exp2(-inf) = 0
+        float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < NS; ++k) {
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[k][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][r], sc, nb));
-                sum += s[k][r];
-            }
-            l += sum;
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, nb));
+            sum += s[r];
         }
+        l += sum;
     }
     __device__ __forceinline__ float total() const { return l + __shfl_xor(l, 32, 64); }
 };
@@ -453,6 +476,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
     Kept<T, DH> q;
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, qi < n);
+    q.settle();
     const float sc = p.scale * LOG2E;
     const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
@@ -463,28 +487,15 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
     };
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&](const char* Ks, const char* Vs, int k0) {
-        constexpr int SUBS = S::KT / 32;
-        int cov[SUBS];
 #pragma unroll
-        for (int u = 0; u < SUBS; ++u) {
-            const int ka = k0 + 32 * u;
-            cov[u] = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
-        }
-        const auto scores = [&](int u, int how) {
-            f32x16 x = product<DH>(Ks, 32 * u, q, lane);
-            if (how == 1) hide(x, sp, k0 + 32 * u + 4 * (lane >> 5), k0 + 32 * u < p.sinks, -INFINITY);
-            return x;
-        };
-        if (SUBS == 2 && cov[0] && cov[SUBS - 1]) {
-            f32x16 s[2] = {scores(0, cov[0]), scores(1, cov[SUBS - 1])};
-            sm.step<2>(s, sc, rescale);
-            gather<DH>(acc, Vs, 0, s[0], lane, T{});
-            gather<DH>(acc, Vs, 32, s[1], lane, T{});
-        } else if (cov[0] || cov[SUBS - 1]) {
-            const int u = cov[0] ? 0 : SUBS - 1;
-            f32x16 s = scores(u, cov[0] ? cov[0] : cov[SUBS - 1]);
-            sm.step<1>(&s, sc, rescale);
-            gather<DH>(acc, Vs, 32 * u, s, lane, T{});
+        for (int sub = 0; sub < S::KT; sub += 32) {
+            const int ka = k0 + sub;
+            const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
+            if (cov == 0) continue;
+            f32x16 s = product<DH>(Ks, sub, q, lane);
+            if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, -INFINITY);
+            sm.step(s, sc, rescale);
+            gather<DH>(acc, Vs, sub, s, lane, T{});
         }
     });
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
@@ -529,7 +540,7 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
         hide(s, Span{0, mine ? n : 0, 0}, k0 + 4 * (lane >> 5), false, -INFINITY);
-        sm.step<1>(&s, sc, [&](float alpha) {
+        sm.step(s, sc, [&](float alpha) {
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
         });
@@ -576,6 +587,17 @@ template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) vo
 }
 
 // ----------------------------------------------------------------------------- backward
+// Register r of a score tile belongs to row 8 (r / 4) + r % 4 (+ 4 in the upper half of the wave): the rows' numbers in
+// that order.
+__device__ __forceinline__ f32x16 rows_of(const float* x, int r0) {
+    f32x16 y;
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+        const f32x4 z = *reinterpret_cast<const f32x4*>(x + r0 + 2 * r);
+        y[r] = z[0]; y[r + 1] = z[1]; y[r + 2] = z[2]; y[r + 3] = z[3];
+    }
+    return y;
+}
 // delta = -dO . o, one wave per four rows of a (sequence, head); o in 32 bits, so that what the rounded output lost is
 // not multiplied by the cancellation in dP - delta.
 template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta_kernel(Slide p, const float* o32) {
@@ -612,7 +634,11 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, qi < n);
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, qi < n);
     const long st = ((long)b * p.Hq + h) * p.N + qi;
-    const float lse = qi < n ? p.lse[st] : INFINITY, delta = qi < n ? p.delta[st] : 0.f;      // delta: negative
+    float lse = qi < n ? p.lse[st] : INFINITY, delta = qi < n ? p.delta[st] : 0.f;      // delta: negative
+    q.settle();
+    d_o.settle();
+    arrived(lse);
+    arrived(delta);
     const float sc = p.scale * LOG2E;
     const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
@@ -627,7 +653,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
             const f32x16 dp = product<DH>(Vs, sub, d_o, lane);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
-            if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, 0.f);
+            if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, 0.f);      // of hidden pairs it may be infinite
             gather<DH>(acc, Ks, sub, s, lane, T{});
         }
     });
@@ -663,10 +689,10 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
         dma_wait();
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
+        hide(s, Span{0, n, 0}, k0 + 4 * (lane >> 5), false, -INFINITY);
         const f32x16 dp = product<DH>(Vs, 0, d_o, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
-        hide(s, Span{0, n, 0}, k0 + 4 * (lane >> 5), false, 0.f);
         gather<DH>(acc, Ks, 0, s, lane, T{});
         wave_lds_fence();
     }
@@ -692,19 +718,11 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const f
                                          const Kept<T, DH>& k, const Kept<T, DH>& v, f32x16* dk, f32x16* dv, float sc, int lane,
                                          bool masked, const Span& sp, int x0, bool first) {
     const int r0 = sub + 4 * (lane >> 5);
-    f32x16 s = product<DH>(Qs, sub, k, lane), dp;
+    f32x16 s = product<DH>(Qs, sub, k, lane);
+    f32x16 dp = product<DH>(Os, sub, v, lane, rows_of(delta, r0));
+    const f32x16 ls = rows_of(lse, r0);
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(delta + r0 + 2 * r);
-        dp[r] = x[0]; dp[r + 1] = x[1]; dp[r + 2] = x[2]; dp[r + 3] = x[3];
-    }
-    dp = product<DH>(Os, sub, v, lane, dp);
-#pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(lse + r0 + 2 * r);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], sc, -x[e]));
-    }
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -ls[r]));
     if (masked) hide(s, sp, x0, first, 0.f);
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] *= s[r];
@@ -722,6 +740,8 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
     Kept<T, DH> k, v;
     k.load((const T*)p.k + b * p.k_b + hk * p.k_h + (long)kj * p.k_n, lane >> 5, kj < n);
     v.load((const T*)p.v + b * p.v_b + hk * p.v_h + (long)kj * p.v_n, lane >> 5, kj < n);
+    k.settle();
+    v.settle();
     const float sc = p.scale * LOG2E;
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
@@ -900,7 +920,7 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
             for (int r = 0; r < 16; ++r)
                 if (k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= end) s[r] = -INFINITY;
         }
-        sm.step<1>(&s, sc, [&](float alpha) {
+        sm.step(s, sc, [&](float alpha) {
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
         });
