@@ -415,8 +415,8 @@ int vitk_sgd_step(const void* table, int n_entries, int n_blocks, const float* s
                   float lr, float momentum, float dampening, float weight_decay, void* stream);
 
 /* ---- AdamW over many tensors (no counterpart in the reference, whose loop uses SGD) ----
- * A device-resident table as above (block0 counts blocks of 8192 elements; a call on a later part of a table counts from
- * its first entry's block0); all tensors fp32 except 8-bit states.
+ * A device-resident table; entry e owns blocks [block0, block0 + ceil(n / 8192)), and entry_of[block] (device) is the entry
+ * of each block.  All tensors fp32 except 8-bit states.
  * flags: bit 0 = the states hold nothing yet and are taken as zero; bit 1 = every pointer of the entry allows 16-byte
  * (8-bit states: 4-byte) accesses.
  * state_bits 32: m, v fp32 [n].  state_bits 8: m, v e4m3 codes [n], m_scale, v_scale fp32 [ceil(n / 256)]: an element of
@@ -428,16 +428,17 @@ typedef struct vitk_adamw_entry {
     int block0;
     int flags;
 } vitk_adamw_entry;
-/* slots (device, VITK_ADAMW_SLOTS doubles owned by the caller): slots[0] := sum of squares of every gradient in the
- * table, in 64 bits and in a fixed order; norm (device, may be NULL) := its root. */
-#define VITK_ADAMW_SLOTS (1 + 1024)
-int vitk_adamw_norm(const void* table, int n_entries, int n_blocks, double* slots, float* norm, void* stream);
-/* g = coef * grad, coef = slots ? min(1, max_norm / (sqrt(slots[0]) + 1e-6)) : 1
+/* norm (device, may be NULL) := 2-norm of every gradient in blocks [0, n_blocks), summed in 64 bits and in a fixed order;
+ * slots (device, VITK_ADAMW_SLOTS doubles owned by the caller): slots[0] := min(1, max_norm / (norm + 1e-6)). */
+#define VITK_ADAMW_SLOTS (1 + 8192)
+int vitk_adamw_norm(const void* table, const int* entry_of, int n_blocks, double max_norm, double* slots, float* norm,
+                    void* stream);
+/* Blocks [first_block, first_block + n_blocks):  g = grad * (slots ? slots[0] : 1)
  * m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  * param = param (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * `step` counts from 1.  Eight-bit states are rounded at random from the word of (seed, step, element): the expectation
  * of what is held is the moment itself. */
-int vitk_adamw_step(const void* table, int n_entries, int n_blocks, const double* slots, double max_norm, double lr,
+int vitk_adamw_step(const void* table, const int* entry_of, int first_block, int n_blocks, const double* slots, double lr,
                     double beta1, double beta2, double eps, double weight_decay, long step, int state_bits, uint32_t seed,
                     void* stream);
 

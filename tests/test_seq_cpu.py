@@ -105,10 +105,12 @@ def test_c_entry_of_axial_rope_refuses(change, code):
 
 def test_c_entries_of_adamw_refuse():
     lib = vitk.lib
-    assert lib.vitk_adamw_norm(None, 1, 1, 4096, None, None) == -3
-    assert lib.vitk_adamw_norm(4096, 0, 1, 4096, None, None) == -1
-    good = [4096, 1, 1, None, 1.0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32, 0, None]
-    for at, value, code in ((0, None, -3), (1, 0, -1), (2, 0, -1), (6, 1.0, -1), (7, -0.1, -1), (8, -1.0, -1), (10, 0, -1), (11, 16, -4)):
+    good = [4096, 4096, 1, 1.0, 4096, None, None]
+    for at, value, code in ((0, None, -3), (1, None, -3), (2, 0, -1), (3, -1.0, -1), (4, None, -3)):
+        assert lib.vitk_adamw_norm(*(good[:at] + [value] + good[at + 1:])) == code, at
+    good = [4096, 4096, 0, 1, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32, 0, None]
+    for at, value, code in ((0, None, -3), (1, None, -3), (2, -1, -1), (3, 0, -1), (6, 1.0, -1), (7, -0.1, -1), (8, -1.0, -1),
+                            (10, 0, -1), (11, 16, -4)):
         assert lib.vitk_adamw_step(*(good[:at] + [value] + good[at + 1:])) == code, at
 
 

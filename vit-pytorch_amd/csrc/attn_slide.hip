@@ -598,29 +598,41 @@ __device__ __forceinline__ f32x16 rows_of(const float* x, int r0) {
     }
     return y;
 }
-// delta = -dO . o, one wave per four rows of a (sequence, head); o in 32 bits, so that what the rounded output lost is
-// not multiplied by the cancellation in dP - delta.
-template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta_kernel(Slide p, const float* o32) {
-    const int lane = threadIdx.x & 15;
-    const long r = (long)blockIdx.x * 16 + (threadIdx.x >> 4);           // (b, i, h)
-    const long rows = (long)p.B * p.N * p.Hq;
+// delta = -dO . o of a kept row; o in 32 bits, so that what the rounded output lost is not multiplied by the cancellation in
+// dP - delta.
+template <int DH> __device__ __forceinline__ float delta_of(const Kept<bf16_t, DH>& d_o, const float* o, int h, bool ok) {
     float s = 0.f;
-    const int h = (int)(r % p.Hq);
-    const long bi = r / p.Hq;
-    const int i = (int)(bi % p.N), b = (int)(bi / p.N);
-    if (r < rows && i < length_of(p, b)) {
-        const T* d_o = (const T*)p.d_o + b * p.do_b + (long)i * p.do_n + h * p.do_h;
-        const float* o = o32 + r * DH;
-        for (int c = lane * 4; c < DH; c += 64) {
-            float x[4], y[4];
-            Vec4<T>::load(d_o + c, x);
-            Vec4<float>::load(o + c, y);
-            s += x[0] * y[0] + x[1] * y[1] + x[2] * y[2] + x[3] * y[3];
-        }
-    }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
-    if (r < rows && lane == 0) p.delta[((long)b * p.Hq + h) * p.N + i] = -s;
+    for (int c = 0; c < DH / 16; ++c) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+        if (ok) {
+            x = *reinterpret_cast<const f32x4*>(o + 16 * c + 8 * h);
+            y = *reinterpret_cast<const f32x4*>(o + 16 * c + 8 * h + 4);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += (float)d_o.f[c][e] * x[e] + (float)d_o.f[c][4 + e] * y[e];
+    }
+    return -(s + __shfl_xor(s, 32, 64));
+}
+template <int DH> __device__ __forceinline__ float delta_of(const Kept<float, DH>& d_o, const float* o, int h, bool ok) {
+    float s = 0.f;
+#pragma unroll
+    for (int t = 0; t < DH / 8; ++t) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (ok) x = *reinterpret_cast<const f32x4*>(o + h * (DH / 2) + 4 * t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += d_o.f[4 * t + e] * x[e];
+    }
+    return -(s + __shfl_xor(s, 32, 64));
+}
+// The deltas alone, for a call that wants no dQ (whose kernel leaves them behind otherwise).
+template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta_kernel(Slide p) {
+    const int lane = threadIdx.x & 63, h = blockIdx.y, b = blockIdx.z, i = blockIdx.x * TQ + (threadIdx.x >> 6) * 32 + (lane & 31);
+    const bool ok = i < length_of(p, b);
+    Kept<T, DH> d_o;
+    d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)i * p.do_n, lane >> 5, ok);
+    const float d = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + i) * p.Hq + h) * DH, lane >> 5, ok);
+    if (i < p.N && lane < 32) p.delta[((long)b * p.Hq + h) * p.N + i] = d;
 }
 
 template <typename T, int DH, bool CAUSAL>
@@ -634,7 +646,9 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, qi < n);
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, qi < n);
     const long st = ((long)b * p.Hq + h) * p.N + qi;
-    float lse = qi < n ? p.lse[st] : INFINITY, delta = qi < n ? p.delta[st] : 0.f;      // delta: negative
+    float lse = qi < n ? p.lse[st] : INFINITY;
+    float delta = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, qi < n);
+    if (qi < p.N && lane < 32) p.delta[st] = delta;
     q.settle();
     d_o.settle();
     arrived(lse);
@@ -677,7 +691,8 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, mine);
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, mine);
     const long st = ((long)b * p.Hq + h) * p.N + qi;
-    const float lse = mine ? p.lse[st] : INFINITY, delta = mine ? p.delta[st] : 0.f;      // not mine: probabilities of 0
+    const float lse = mine ? p.lse[st] : INFINITY;                       // not mine: probabilities of 0
+    const float delta = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, mine);
     const float sc = p.scale * LOG2E;
     f32x16 acc[DH / 32] = {};
     const int q0 = qa / TQ * TQ;
@@ -851,24 +866,35 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && DH < 128 ? 2 : 1) void slide
     if (it.far) dkv_far<T, DH, CAUSAL>(p, lds, it.x, it.h, it.b, n);
     else dkv_band<T, DH, CAUSAL, KG>(p, lds, it.x * (32 * KG), it.h, it.b, n);
 }
-// The records of the first rows become gradients: blockIdx.y < Hkv dk and dv, behind them dq (if it has records).
-template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_bwd_join_kernel(Slide p, int kv_heads) {
-    const int i = blockIdx.x, b = blockIdx.z, d = threadIdx.x;
-    if (d >= DH) return;
+// The records of the first rows become gradients: blockIdx.y < kv_heads dk and dv, behind them dq.  256 / DH shares of the
+// records, each in its order, then the shares in theirs.
+template <typename T, int DH> __global__ __launch_bounds__(256) void slide_bwd_join_kernel(Slide p, int kv_heads, int rows, int k_recs, int q_recs) {
+    constexpr int SHARES = 256 / DH;
+    __shared__ float part[2][256];
+    const int i = blockIdx.x, b = blockIdx.z, d = threadIdx.x % DH, share = threadIdx.x / DH;
+    const int h = (int)blockIdx.y - kv_heads, hk = blockIdx.y;
+    const bool keys = h < 0;
+    const int recs = keys ? k_recs : q_recs, width = keys ? 2 * DH : DH;
+    const float* rec = (keys ? p.ws + (((long)b * p.Hkv + hk) * rows + i) * recs * width
+                             : p.ws_q + (((long)b * p.Hq + h) * rows + i) * recs * width) + d;
+    float x = 0.f, y = 0.f;
+#pragma unroll 4
+    for (int s = share; s < recs; s += SHARES) {
+        x += rec[(long)s * width];
+        if (keys) y += rec[(long)s * width + DH];
+    }
+    part[0][threadIdx.x] = x;
+    part[1][threadIdx.x] = y;
+    __syncthreads();
+    if (share) return;
+#pragma unroll
+    for (int s = 1; s < SHARES; ++s) { x += part[0][s * DH + d]; y += part[1][s * DH + d]; }
     const bool there = i < length_of(p, b);
-    const int h = (int)blockIdx.y - kv_heads;
-    if (h < 0) {
-        const int hk = blockIdx.y;
-        const float* rec = p.ws + (((long)b * p.Hkv + hk) * p.rows + i) * (p.chunks + 1) * (2 * DH) + d;
-        float k = 0.f, v = 0.f;
-        for (int s = 0; s <= p.chunks; ++s) { k += rec[s * 2 * DH]; v += rec[s * 2 * DH + DH]; }
-        ((T*)p.dk)[b * p.dk_b + i * p.dk_n + hk * p.dk_h + d] = (T)(there ? k * p.scale : 0.f);
-        ((T*)p.dv)[b * p.dv_b + i * p.dv_n + hk * p.dv_h + d] = (T)(there ? v : 0.f);
+    if (keys) {
+        ((T*)p.dk)[b * p.dk_b + (long)i * p.dk_n + hk * p.dk_h + d] = (T)(there ? x * p.scale : 0.f);
+        ((T*)p.dv)[b * p.dv_b + (long)i * p.dv_n + hk * p.dv_h + d] = (T)(there ? y : 0.f);
     } else {
-        const float* rec = p.ws_q + (((long)b * p.Hq + h) * p.rows + i) * (p.chunks + 1) * DH + d;
-        float q = 0.f;
-        for (int s = 0; s <= p.chunks; ++s) q += rec[s * DH];
-        ((T*)p.dq)[b * p.dq_b + i * p.dq_n + h * p.dq_h + d] = (T)(there ? q * p.scale : 0.f);
+        ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(there ? x * p.scale : 0.f);
     }
 }
 
@@ -1013,7 +1039,7 @@ template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipSt
     }
     return 0;
 }
-template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, const float* o32, float* ws, hipStream_t st) {
+template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipStream_t st) {
     const Records rk = records_of(p.B, p.N, p.Hkv, p.G, 2 * DH, p.window, p.sinks);
     const Records rq = CAUSAL ? Records{0, 0, 0} : records_of(p.B, p.N, p.Hq, 1, DH, p.window, p.sinks);
     if (rk.rows && !ws) return VITK_ERR_NULL;
@@ -1021,13 +1047,16 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, const float* o32
     if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL>, bytes)) return e;
     if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, 4>, bytes)) return e;
     if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, 2>, bytes)) return e;
-    const long rows = (long)p.B * p.N * p.Hq;
-    hipLaunchKernelGGL((slide_delta_kernel<T, DH>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, p, o32);
-    VITK_CHECK_LAUNCH();
     p.ws = ws;
     p.ws_q = ws + rk.floats;
-    const dim3 join(DH < 64 ? 64 : DH);
-    const unsigned first = (unsigned)(rk.rows < p.N ? rk.rows : p.N);
+    if (p.dq) {
+        p.rows = rq.rows; p.chunks = rq.chunks;
+        const unsigned grid = grid_of(p, p.Hq, rq.rows > 0);
+        hipLaunchKernelGGL((slide_dq_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
+    } else {
+        hipLaunchKernelGGL((slide_delta_kernel<T, DH>), dim3(vitk_ceil_div(p.N, TQ), p.Hq, p.B), dim3(256), 0, st, p);
+    }
+    VITK_CHECK_LAUNCH();
     if (p.dk) {
         p.rows = rk.rows; p.chunks = rk.chunks;
         // few key heads leave CUs without a band of 128 keys: bands of 64 below two of them for each CU
@@ -1037,20 +1066,12 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, const float* o32
         if (narrow) hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, 2>), dim3(grid), dim3(256), bytes, st, p);
         else hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, 4>), dim3(grid), dim3(256), bytes, st, p);
         VITK_CHECK_LAUNCH();
-        if (p.rows) {
-            hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(first, p.Hkv, p.B), join, 0, st, p, p.Hkv);
-            VITK_CHECK_LAUNCH();
-        }
     }
-    if (p.dq) {
-        p.rows = rq.rows; p.chunks = rq.chunks;
-        const unsigned grid = grid_of(p, p.Hq, rq.rows > 0);
-        hipLaunchKernelGGL((slide_dq_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
+    const int kv_heads = p.dk ? p.Hkv : 0, q_heads = p.dq && rq.rows ? p.Hq : 0;
+    if (rk.rows && kv_heads + q_heads) {
+        hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(rk.rows < p.N ? rk.rows : p.N, kv_heads + q_heads, p.B), dim3(256), 0, st,
+                           p, kv_heads, rk.rows, rk.chunks + 1, rq.chunks + 1);
         VITK_CHECK_LAUNCH();
-        if (p.rows) {
-            hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(first, p.Hq, p.B), join, 0, st, p, 0);
-            VITK_CHECK_LAUNCH();
-        }
     }
     return 0;
 }
@@ -1104,6 +1125,7 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     }
     if (!a->d_o || !a->lse || !a->delta || !a->dk != !a->dv || !(a->dq || a->dk)) return VITK_ERR_NULL;
     if (dtype == VITK_BF16 ? !a->o_f32 : !a->o) return VITK_ERR_NULL;
+    if (!aligned(dtype == VITK_BF16 ? a->o_f32 : a->o, 4, {})) return VITK_ERR_SHAPE;
     if (!aligned(a->d_o, e, {a->do_b, a->do_n, a->do_h}) || !aligned(a->dq, e, {a->dq_b, a->dq_n, a->dq_h}) ||
         !aligned(a->dk, e, {a->dk_b, a->dk_n, a->dk_h}) || !aligned(a->dv, e, {a->dv_b, a->dv_n, a->dv_h})) return VITK_ERR_SHAPE;
     p.d_o = a->d_o; p.delta = a->delta; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
@@ -1152,8 +1174,8 @@ extern "C" int vitk_slide_attn_bwd(const vitk_slide_attn* a, int dtype, void* st
     Slide p;
     if (int e = fill(a, dtype, true, p)) return e;
     hipStream_t st = (hipStream_t)stream;
-    const float* o32 = dtype == VITK_BF16 ? a->o_f32 : (const float*)a->o;
-#define BWD(T, DH, C) run_bwd<T, DH, C>(p, o32, a->workspace, st)
+    p.o32 = dtype == VITK_BF16 ? a->o_f32 : (float*)a->o;
+#define BWD(T, DH, C) run_bwd<T, DH, C>(p, a->workspace, st)
     SLIDE_FORMS(BWD);
 }
 

@@ -132,7 +132,7 @@ class FusedSGD(torch.optim.Optimizer):
 
 _ADAMW_ENTRY = np.dtype([("param", "<u8"), ("grad", "<u8"), ("m", "<u8"), ("v", "<u8"), ("m_scale", "<u8"),
                          ("v_scale", "<u8"), ("n", "<i8"), ("block0", "<i4"), ("flags", "<i4")])
-_ADAMW_SLOTS = 1 + 1024      # VITK_ADAMW_SLOTS (include/vitk.h)
+_ADAMW_SLOTS = 1 + 8192      # VITK_ADAMW_SLOTS (include/vitk.h)
 _SCALE_BLOCK = 256           # elements of an 8-bit state that share a scale
 assert _ADAMW_ENTRY.itemsize == 64
 
@@ -175,31 +175,41 @@ class FusedAdamW(torch.optim.Optimizer):
                         st[name] = torch.empty(value.shape, dtype=torch.float32 if name.endswith("_scale") else kind,
                                                device=p.device).copy_(value)
 
-    def _row(self, p, block0):
-        g, st = p.grad, self.state[p]
-        if not (p.is_cuda and p.dtype == torch.float32 and g.dtype == torch.float32 and not g.is_sparse
-                and p.is_contiguous() and g.is_contiguous()):
-            raise ValueError("FusedAdamW needs contiguous fp32 parameters and gradients on the GPU")
-        n = p.numel()
-        if not st:
-            kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
-            st["step"] = 0
-            st["exp_avg"] = torch.empty(p.shape, dtype=kind, device=p.device)
-            st["exp_avg_sq"] = torch.empty(p.shape, dtype=kind, device=p.device)
-            if self.state_bits == 8:
-                for name in ("exp_avg_scale", "exp_avg_sq_scale"):
-                    st[name] = torch.empty(-(-n // _SCALE_BLOCK), dtype=torch.float32, device=p.device)
-        m, v = st["exp_avg"].data_ptr(), st["exp_avg_sq"].data_ptr()
-        ms, vs = (st["exp_avg_scale"].data_ptr(), st["exp_avg_sq_scale"].data_ptr()) if self.state_bits == 8 else (0, 0)
-        vec = (p.data_ptr() | g.data_ptr()) % 16 == 0 and (m | v) % (4 if self.state_bits == 8 else 16) == 0
-        return (p.data_ptr(), g.data_ptr(), m, v, ms, vs, n, block0, (1 if st["step"] == 0 else 0) | (2 if vec else 0))
+    def _begin(self, p, st):
+        """Empty states of a parameter: the first step takes them as zeros."""
+        kind = torch.float8_e4m3fn if self.state_bits == 8 else torch.float32
+        st["step"] = 0
+        st["exp_avg"] = torch.empty(p.shape, dtype=kind, device=p.device)
+        st["exp_avg_sq"] = torch.empty(p.shape, dtype=kind, device=p.device)
+        if self.state_bits == 8:
+            for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+                st[name] = torch.empty(-(-p.numel() // _SCALE_BLOCK), dtype=torch.float32, device=p.device)
 
-    def _upload(self, host, dev):
-        """The table on the device; uploads go through a ring of pinned buffers, each guarded by an event, so the host
-        never waits for the step it has just enqueued."""
+    def _table(self, ps, grads, sts):
+        """The rows of all tensors, column by column, with blocks counted from 0; (table, number of blocks)."""
+        host = np.zeros(len(ps), dtype=_ADAMW_ENTRY)
+        host["param"] = [p.data_ptr() for p in ps]
+        host["grad"] = [g.data_ptr() for g in grads]
+        host["m"] = [s["exp_avg"].data_ptr() for s in sts]
+        host["v"] = [s["exp_avg_sq"].data_ptr() for s in sts]
+        if self.state_bits == 8:
+            host["m_scale"] = [s["exp_avg_scale"].data_ptr() for s in sts]
+            host["v_scale"] = [s["exp_avg_sq_scale"].data_ptr() for s in sts]
+        host["n"] = [p.numel() for p in ps]
+        blocks = np.cumsum((host["n"] + (_CHUNK - 1)) // _CHUNK)
+        host["block0"][1:] = blocks[:-1]
+        vec = ((host["param"] | host["grad"]) % 16 == 0) & ((host["m"] | host["v"]) % (4 if self.state_bits == 8 else 16) == 0)
+        host["flags"] = vec * 2
+        host["flags"] |= np.array([s["step"] == 0 for s in sts])
+        return host, blocks
+
+    def _upload(self, host, blocks, dev):
+        """The table and, behind it, the entry of each block, on the device; uploads go through a ring of pinned buffers,
+        each guarded by an event, so the host never waits for the step it has just enqueued."""
         if self._last is not None and self._last.shape == host.shape and np.array_equal(self._last, host):
             return
-        nbytes = host.nbytes
+        entry_of = np.repeat(np.arange(len(host), dtype=np.int32), np.diff(blocks, prepend=0))
+        nbytes = host.nbytes + entry_of.nbytes
         if self._dev is None or self._dev.numel() < nbytes:
             self._dev = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         if not self._ring or self._ring[0][0].numel() < nbytes:
@@ -209,7 +219,8 @@ class FusedAdamW(torch.optim.Optimizer):
         else:
             self._ring[self._turn][1].synchronize()
         buf, ev = self._ring[self._turn]
-        buf.numpy()[:nbytes] = host.view(np.uint8)
+        buf.numpy()[:host.nbytes] = host.view(np.uint8)
+        buf.numpy()[host.nbytes:nbytes] = entry_of.view(np.uint8)
         self._dev[:nbytes].copy_(buf[:nbytes], non_blocking=True)
         ev.record()
         self._turn = (self._turn + 1) % 4
@@ -224,46 +235,52 @@ class FusedAdamW(torch.optim.Optimizer):
         if max_grad_norm is not None and not max_grad_norm >= 0.0:
             raise ValueError("max_grad_norm must be non-negative")
         # one launch for the tensors of a group that have taken the same number of steps
-        runs = []
+        state, f32 = self.state, torch.float32
+        all_ps, all_grads, all_sts, spans = [], [], [], []
         for group in self.param_groups:
-            by_step = {}
-            for p in group["params"]:
-                if p.grad is not None and p.numel():
-                    by_step.setdefault(self.state[p].get("step", 0), []).append(p)
-            runs += [(group, t, ps) for t, ps in by_step.items()]
-        if not runs:
+            ps = [p for p in group["params"] if p.grad is not None and p.numel()]
+            sts = [state[p] for p in ps]
+            for p, st in zip(ps, sts):
+                if not st:
+                    self._begin(p, st)
+            steps = [st["step"] for st in sts]
+            for t in dict.fromkeys(steps):
+                at = [i for i, x in enumerate(steps) if x == t] if steps.count(t) != len(steps) else range(len(steps))
+                spans.append((group, t, len(all_ps), len(at)))
+                all_ps += [ps[i] for i in at]
+                all_sts += [sts[i] for i in at]
+        if not all_ps:
             return None
-        dev = runs[0][2][0].device
-        if any(p.device != dev for _, _, ps in runs for p in ps):
-            raise ValueError("FusedAdamW updates tensors of one device")
+        dev = all_ps[0].device
+        all_grads = [p.grad for p in all_ps]
+        at = all_ps[0].get_device()
+        if not (dev.type == "cuda" and all(p.dtype is f32 and p.get_device() == at and p.is_contiguous() for p in all_ps)
+                and all(g.dtype is f32 and g.get_device() == at and not g.is_sparse and g.is_contiguous() for g in all_grads)):
+            raise ValueError("FusedAdamW needs contiguous fp32 parameters and gradients on one GPU")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW.step counts steps on the host and is not captured into a graph")
-        rows, spans, blocks = [], [], 0
-        for group, t, ps in runs:
-            first, at = len(rows), blocks
-            for p in ps:
-                rows.append(self._row(p, blocks))
-                blocks += (p.numel() + _CHUNK - 1) // _CHUNK
-            spans.append((first, len(rows) - first, blocks - at))
+        host, blocks = self._table(all_ps, all_grads, all_sts)
         with torch.cuda.device(dev):
-            self._upload(np.array(rows, dtype=_ADAMW_ENTRY), dev)
+            self._upload(host, blocks, dev)
             if self._slots is None:
                 self._slots = torch.empty(_ADAMW_SLOTS, dtype=torch.float64, device=dev)
-            stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-            base = self._dev.data_ptr()
+            stream = torch.cuda.current_stream(dev).cuda_stream
+            table, entry_of = self._dev.data_ptr(), self._dev.data_ptr() + host.nbytes
             slots = norm = None
             if max_grad_norm is not None:
                 norm = torch.empty((), dtype=torch.float32, device=dev)
                 slots = self._slots.data_ptr()
-                vitk.check(vitk.lib.vitk_adamw_norm(base, len(rows), blocks, slots, norm.data_ptr(), stream), "adamw_norm")
-            for (group, t, ps), (first, cnt, nblk) in zip(runs, spans):
+                vitk.check(vitk.lib.vitk_adamw_norm(table, entry_of, int(blocks[-1]), float(max_grad_norm), slots, norm.data_ptr(),
+                                                    stream), "adamw_norm")
+            for group, t, first, cnt in spans:
                 b1, b2 = group["betas"]
-                vitk.check(vitk.lib.vitk_adamw_step(base + first * _ADAMW_ENTRY.itemsize, cnt, nblk, slots,
-                                                    float(max_grad_norm or 0.0), float(group["lr"]), float(b1), float(b2),
-                                                    float(group["eps"]), float(group["weight_decay"]), t + 1,
-                                                    self.state_bits, self.seed, stream), "adamw_step")
-                for p in ps:
-                    self.state[p]["step"] = t + 1
+                block = int(host["block0"][first])
+                vitk.check(vitk.lib.vitk_adamw_step(table, entry_of, block, int(blocks[first + cnt - 1]) - block, slots,
+                                                    float(group["lr"]), float(b1), float(b2), float(group["eps"]),
+                                                    float(group["weight_decay"]), t + 1, self.state_bits, self.seed, stream),
+                           "adamw_step")
+            for st in all_sts:
+                st["step"] += 1
             # the parameters were written through raw pointers: renew the GEMM operands kept with them (one launch)
-            vitk.ops.refresh_operands([p for _, _, ps in runs for p in ps])
+            vitk.ops.refresh_operands(all_ps)
         return norm

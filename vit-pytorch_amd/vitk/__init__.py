@@ -100,8 +100,8 @@ PROTOTYPES = {
     "vitk_slide_attn_bwd": [ctypes.POINTER(SlideAttn), _i, _vp],
     "vitk_slide_decode": [ctypes.POINTER(SlideCache), _i, _vp],
     "vitk_axial_rope": [ctypes.POINTER(Rope), _i, _vp],
-    "vitk_adamw_norm": [_vp, _i, _i, _vp, _vp, _vp],
-    "vitk_adamw_step": [_vp, _i, _i, _vp] + [ctypes.c_double] * 6 + [_l, _i, ctypes.c_uint32, _vp],
+    "vitk_adamw_norm": [_vp, _vp, _i, ctypes.c_double, _vp, _vp, _vp],
+    "vitk_adamw_step": [_vp, _vp, _i, _i, _vp] + [ctypes.c_double] * 5 + [_l, _i, ctypes.c_uint32, _vp],
     "vitk_comm_unique_id": [_vp, ctypes.c_size_t],
     "vitk_comm_init": [_i, _i, _vp, ctypes.POINTER(ctypes.c_void_p)],
     "vitk_allreduce": [_vp, _vp, ctypes.c_size_t, _i, _i, _vp],

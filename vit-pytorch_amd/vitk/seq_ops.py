@@ -26,7 +26,7 @@ class _On:
         self.before = torch.cuda.current_device()
         if self.before != self.device:
             torch.cuda.set_device(self.device)
-        self.stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        self.stream = torch._C._cuda_getCurrentRawStream(self.device)
         return self
 
     def __exit__(self, *_):
@@ -34,23 +34,26 @@ class _On:
             torch.cuda.set_device(self.before)
 
 
-def _one_device(what, *ts):
-    first = ts[0]
+def _one_device(what, first, *ts):
+    if not first.is_cuda:
+        raise VitkError(f"{what}: vitk kernels run on the GPU only: got a tensor on {first.device}")
+    device = first.device
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise VitkError(f"{what}: vitk kernels run on the GPU only: got a tensor on {t.device}")
-        if t.device != first.device:
-            raise VitkError(f"{what}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise VitkError(f"{what}: tensors on {device} and {t.device}")
 
 
 def _rows(t):
     """`t` as the kernels address it: consecutive elements inside a head, pointer and strides multiples of 16 bytes, tokens
-    less than 2^23 elements apart."""
-    e = t.element_size()
-    if t.stride(-1) == 1 and t.stride(1) < 1 << 23 and t.data_ptr() % 16 == 0 and all(s * e % 16 == 0 for s in t.stride()[:-1]):
-        return t
+    less than 2^23 elements apart.  (A contiguous head of 32 elements or more is such a multiple.)"""
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            if t.dim() < 4 or t.stride(1) < 1 << 23:
+                return t
+        else:
+            st, unit = t.stride(), 16 // t.element_size()
+            if st[-1] == 1 and not any(s % unit for s in st[:-1]) and st[1] < 1 << 23:
+                return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -97,29 +100,27 @@ def _rope_args(x, positions, pairs, base):
     return positions.contiguous(), pairs, float(base)
 
 
+def _rope_new(x, pos, pairs, base, interleaved, inverse):
+    x = x if x.stride(-1) == 1 else x.contiguous()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if y.numel():
+        with _On(x.device) as on:
+            _rope_call(x, y, pos, pairs, base, interleaved, inverse, on)
+    return y
+
+
 class AxialRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, pos, pairs, base, interleaved):
         ctx.save_for_backward(pos)
         ctx.meta = (pairs, base, interleaved)
-        x = x if x.stride(-1) == 1 else x.contiguous()
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if y.numel():
-            with _On(x.device) as on:
-                _rope_call(x, y, pos, pairs, base, interleaved, False, on)
-        return y
+        return _rope_new(x, pos, pairs, base, interleaved, False)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         (pos,) = ctx.saved_tensors
-        pairs, base, interleaved = ctx.meta
-        dy = dy if dy.stride(-1) == 1 else dy.contiguous()
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-        if dx.numel():
-            with _On(dy.device) as on:
-                _rope_call(dy, dx, pos, pairs, base, interleaved, True, on)
-        return dx, None, None, None, None
+        return _rope_new(dy, pos, *ctx.meta, True), None, None, None, None
 
 
 def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
@@ -132,8 +133,11 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     Returns a new contiguous tensor, or writes ``out`` (same shape and type, consecutive elements inside a head; it may be
     x itself, in a part of a cache, ...; not differentiable)."""
     pos, pairs, base = _rope_args(x, positions, pairs, base)
+    interleaved = bool(interleaved)
     if out is None:
-        return AxialRopeFn.apply(x, pos, pairs, base, bool(interleaved))
+        if torch.is_grad_enabled() and x.requires_grad:
+            return AxialRopeFn.apply(x, pos, pairs, base, interleaved)
+        return _rope_new(x, pos, pairs, base, interleaved, False)
     if torch.is_grad_enabled() and (x.requires_grad or out.requires_grad):
         raise VitkError("axial_rope: out= is not differentiable")
     if out.shape != x.shape or out.dtype != x.dtype or out.stride(-1) != 1:
@@ -142,13 +146,13 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     x = x if x.stride(-1) == 1 else x.contiguous()
     if out.numel():
         with _On(x.device) as on:
-            _rope_call(x, out, pos, pairs, base, bool(interleaved), False, on)
+            _rope_call(x, out, pos, pairs, base, interleaved, False, on)
     return out
 
 
 # ----------------------------------------------------------------------------- attention with a window and sinks
 def _heads(what, q, k, v):
-    B, N, Hq, dh = q.shape
+    B, Hq, dh = q.shape[0], q.shape[-2], q.shape[-1]
     if k.dim() != 4 or v.shape != k.shape or k.shape[0] != B or k.shape[3] != dh:
         raise VitkError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not go together")
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -267,7 +271,10 @@ def sliding_attention(q, k, v, window, sinks=0, causal=False, lengths=None, scal
     if lengths is not None:
         lengths = _lengths(what, lengths, q.shape[0])
     _one_device(what, q, k, v, lengths)
-    return SlidingAttentionFn.apply(q, k, v, lengths, (window, sinks, bool(causal), scale))
+    meta = (window, sinks, bool(causal), scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return SlidingAttentionFn.apply(q, k, v, lengths, meta)
+    return _slide_forward(_rows(q), _rows(k), _rows(v), lengths, meta, False)[0]
 
 
 class SlidingAttentionQkvFn(torch.autograd.Function):
@@ -330,9 +337,14 @@ def sliding_attention_qkv(qkv, B, N, H, window, sinks=0, causal=False, scale=Non
     return SlidingAttentionQkvFn.apply(qkv, (B, N, H), (window, sinks, bool(causal), scale), rope)
 
 
+_CUS = {}         # compute units of each device
+
+
 def _splits(B, Hkv, G, reach, device):
     """Workgroups that share the keys of one (sequence, key head)."""
-    cus = torch.cuda.get_device_properties(device).multi_processor_count
+    cus = _CUS.get(device.index)
+    if cus is None:
+        cus = _CUS[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
     groups = B * Hkv * ((G + 31) // 32)
     tiles = -(-reach // 128)                     # 4 waves of 32 keys
     return max(1, min(tiles, -(-2 * cus // groups), 64))
@@ -349,7 +361,7 @@ def sliding_attention_decode(q, k_cache, v_cache, lengths, window, sinks=0, scal
         raise VitkError(f"{what}: q is [batch, heads, head size], got {tuple(q.shape)}")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise VitkError(f"{what}: not differentiable; call it under torch.no_grad()")
-    _heads(what, q[:, None], k_cache, v_cache)
+    _heads(what, q, k_cache, v_cache)
     B, Hq, dh = q.shape
     cap, Hkv = k_cache.shape[1:3]
     window, sinks, scale = _reach(what, window, sinks, scale, cap, dh)
