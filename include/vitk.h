@@ -229,7 +229,7 @@ typedef struct vitk_slide_attn {
     float scale;
 } vitk_slide_attn;
 /* Bytes of `workspace` (16-byte aligned, contents undefined) that the forward or the backward call needs; 0: it may be NULL. */
-size_t vitk_slide_attn_workspace(const vitk_slide_attn* a, int backward);
+size_t vitk_slide_attn_workspace(const vitk_slide_attn* a, int dtype, int backward);
 int vitk_slide_attn_fwd(const vitk_slide_attn* a, int dtype, void* stream);
 int vitk_slide_attn_bwd(const vitk_slide_attn* a, int dtype, void* stream);
 /* One query per sequence, the last of its lengths[b] cached tokens: it sees j < sinks and j >= lengths[b] - window.

@@ -41,7 +41,6 @@ struct Slide {
     int chunks;                // far items of each 32 of them; a row has chunks + 1 records, the band's last
     float* ws;                 // forward: records of dh + 2; backward: dk | dv, then dq, records of dh
     float* ws_q;
-    int tk;                    // keys of a band of the dK / dV kernel
     int far_items, items;      // of this launch: far ones come first, then bands
 };
 
@@ -194,6 +193,18 @@ template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, in
     reads_ahead<DH / 16, 1>();
     return acc;
 }
+// The same with the kept rows in an LDS tile.
+template <typename T, int DH> struct KeptInLds { const char* rows; };
+template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const KeptInLds<bf16_t, DH>& kept, int lane, f32x16 acc = {}) {
+    const int a = Shape<bf16_t, DH>::at(lane & 31, lane >> 5);
+    tile += r0 * Shape<bf16_t, DH>::ROW;
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(tile + (a ^ (c << 5))),
+                                                      *reinterpret_cast<const bf16x8*>(kept.rows + (a ^ (c << 5))), acc, 0, 0, 0);
+    reads_ahead<DH / 16, 2>();
+    return acc;
+}
 template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, int r0, const Kept<float, DH>& kept, int lane, f32x16 acc = {}) {
     const int a = Shape<float, DH>::at(lane & 31, (lane >> 5) * (DH / 8));
     tile += r0 * Shape<float, DH>::ROW;
@@ -257,12 +268,12 @@ __device__ __forceinline__ void dma4(const void* from, unsigned lds) {
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(VITK_LDS const char*)p; }
-template <typename T, int DH> struct Stage {
+template <typename T, int DH, int NT = 256> struct Stage {
     using S = Shape<T, DH>;
-    static constexpr int PARTS = S::KT * S::CHUNKS / 256;
+    static constexpr int PARTS = S::KT * S::CHUNKS / NT;
     int voff[PARTS];
     int ld;
-    __device__ __forceinline__ static int place(int i, int tid) { return i * 256 + tid; }
+    __device__ __forceinline__ static int place(int i, int tid) { return i * NT + tid; }
     __device__ __forceinline__ int offset(int i, int tid, int last) const {
         const int pl = place(i, tid), r = pl / S::CHUNKS, ch = (pl % S::CHUNKS) ^ S::mix(r);
         return (r < last ? r : last) * ld * (int)sizeof(T) + ch * 16;
@@ -276,10 +287,10 @@ template <typename T, int DH> struct Stage {
         const unsigned to = __builtin_amdgcn_readfirstlane(lds_addr(tile) + (tid & ~63) * 16);
         if (r0 + S::KT <= n) {
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i) dma16(from, voff[i], to + i * 4096);
+            for (int i = 0; i < PARTS; ++i) dma16(from, voff[i], to + i * NT * 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i) dma16(from, offset(i, tid, n - 1 - r0), to + i * 4096);
+            for (int i = 0; i < PARTS; ++i) dma16(from, offset(i, tid, n - 1 - r0), to + i * NT * 16);
         }
     }
 };
@@ -385,8 +396,8 @@ __device__ __forceinline__ Item item_of(const Slide& p, int heads, int tiles) {
     it.b = k / tiles / heads;
     return it;
 }
-// Sums of the four waves, [32 columns][DH] each, in LDS; `extra` behind them.
-template <int DH> constexpr int join_bytes() { return 4 * 32 * (DH + 4) * (int)sizeof(float); }
+// Sums of the waves, [32 columns][DH + 4] each, in LDS.
+template <int DH> constexpr int join_bytes(int waves = 4) { return waves * 32 * (DH + 4) * (int)sizeof(float); }
 
 // One record of the softmax of a row from the four waves': called by all threads, f(column, d, sum, maximum, total).
 template <int DH, typename F> __device__ __forceinline__ void join_waves(char* lds, const f32x16* acc, float m, float l, int tid, F f) {
@@ -414,18 +425,20 @@ template <int DH, typename F> __device__ __forceinline__ void join_waves(char* l
         f(c, d, x, top, sum);
     }
 }
-// The plain sum of the four waves', to records `stride` floats apart.
-template <int DH> __device__ __forceinline__ void add_waves(char* lds, const f32x16* acc, float* rec, long stride, int tid) {
+// The plain sum of NW waves', to records `stride` floats apart.
+template <int DH, int NW = 4> __device__ __forceinline__ void add_waves(char* lds, const f32x16* acc, float* rec, long stride, int tid) {
     constexpr int W = DH + 4;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* out = reinterpret_cast<float*>(lds);
     __syncthreads();
     put<float, DH>(out + (wave * 32 + (lane & 31)) * W, acc, 1.f, lane);
     __syncthreads();
-    for (int idx = tid; idx < 32 * DH; idx += 256) {
+    for (int idx = tid; idx < 32 * DH; idx += NW * 64) {
         const int c = idx / DH, d = idx % DH;
-        const float* o = out + c * W + d;
-        rec[c * stride + d] = (o[0] + o[32 * W]) + (o[64 * W] + o[96 * W]);
+        float x = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) x += out[(w * 32 + c) * W + d];
+        rec[c * stride + d] = x;
     }
 }
 
@@ -728,9 +741,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void slide_dq_kernel(S
 // 32 x 32 scores, their probabilities and score gradients, and what they add to dV and dK: rows of the tile are queries,
 // columns keys; lse, delta: the rows' (the second product starts from the negative delta).  x0: the query of the tile's
 // first row for this lane's half, for `masked` tiles.
-template <typename T, int DH>
+template <typename T, int DH, typename K>
 __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const float* lse, const float* delta, int sub,
-                                         const Kept<T, DH>& k, const Kept<T, DH>& v, f32x16* dk, f32x16* dv, float sc, int lane,
+                                         const K& k, const K& v, f32x16* dk, f32x16* dv, float sc, int lane,
                                          bool masked, const Span& sp, int x0, bool first) {
     const int r0 = sub + 4 * (lane >> 5);
     f32x16 s = product<DH>(Qs, sub, k, lane);
@@ -744,59 +757,96 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const f
     gather<DH>(dv, Os, sub, s, lane, T{});
     gather<DH>(dk, Qs, sub, dp, lane, T{});
 }
-// Band: 32 KG keys of one (sequence, key head); the queries of every head that shares it stream through LDS.  Wave w keeps
-// keys 32 (w % KG); with KG = 2 the other two waves take every second 32 queries and the halves are added at the end.
-template <typename T, int DH, bool CAUSAL, int KG>
+// How a workgroup of the dK / dV kernel is laid out: NW waves, 32 KG keys; wave w keeps keys 32 (w % KG) and takes every
+// (NW / KG)-th 32 queries, and the parts are added at the end.  Four waves of 32 keys each where there are enough of them;
+// bands of 64 keys where heads are few; and for bf16 heads of 128, whose four operands and sums of a wave leave room for
+// one wave a SIMD only, eight waves with K and V in LDS, two to a SIMD (FIGURES).
+template <typename T, int DH, int NW, int KG> struct Layout {
+    using S = Shape<T, DH>;
+    static constexpr bool IN_LDS = NW == 8;
+    using Keep = typename std::conditional<IN_LDS, KeptInLds<T, DH>, Kept<T, DH>>::type;
+    static constexpr int PARTS = NW / KG, NT = NW * 64;
+    static constexpr int TILE = S::KT * S::ROW, BUF = 2 * TILE + 2 * S::KT * 4;      // Q, dO, lse, delta
+    static constexpr int WAVE = 2 * 32 * S::ROW + 256;                               // the same for 32 queries of one wave
+    static constexpr int KEEP = IN_LDS ? 32 * KG * S::ROW : 0, KEEP_FAR = IN_LDS ? 32 * S::ROW : 0;      // of K, of V
+    static constexpr int MEET = KG * 32 * (DH + 4) * 4;
+    static constexpr int most(int a, int b) { return a > b ? a : b; }
+    static constexpr int bytes(bool far) {
+        const int band = most(2 * BUF + 2 * KEEP, PARTS > 1 ? MEET : 0);
+        return far ? most(band, most(NW * WAVE + 2 * KEEP_FAR, join_bytes<DH>(NW))) : band;
+    }
+};
+// Rows of K or V into an LDS tile that stays, zeros from `end` on.
+template <typename T, int DH, int NT> __device__ __forceinline__ void keep_rows(char* tile, const T* base, long ld, int r0, int rows, int end, int tid) {
+    using S = Shape<T, DH>;
+    for (int idx = tid; idx < rows * S::CHUNKS; idx += NT) {
+        const int r = idx / S::CHUNKS, ch = idx % S::CHUNKS;
+        u32x4 x = {0, 0, 0, 0};
+        if (r0 + r < end) x = *reinterpret_cast<const u32x4*>(base + (long)(r0 + r) * ld + ch * (16 / (int)sizeof(T)));
+        *reinterpret_cast<u32x4*>(tile + S::at(r, ch)) = x;
+    }
+}
+// Band: the queries of every head that shares the keys stream through LDS.
+template <typename T, int DH, bool CAUSAL, int NW, int KG>
 __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int hk, int b, int n) {
     using S = Shape<T, DH>;
-    constexpr int BYTES = S::KT * S::ROW, BUF = 2 * BYTES + 2 * S::KT * 4;      // Q, dO, -lse, -delta
+    using L = Layout<T, DH, NW, KG>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int ka = k0 + wave % KG * 32, kj = ka + (lane & 31), part = wave / KG;
-    Kept<T, DH> k, v;
-    k.load((const T*)p.k + b * p.k_b + hk * p.k_h + (long)kj * p.k_n, lane >> 5, kj < n);
-    v.load((const T*)p.v + b * p.v_b + hk * p.v_h + (long)kj * p.v_n, lane >> 5, kj < n);
-    k.settle();
-    v.settle();
+    const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
+    const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
+    typename L::Keep k, v;
+    if constexpr (L::IN_LDS) {
+        char* keep = lds + 2 * L::BUF;
+        keep_rows<T, DH, L::NT>(keep, K, p.k_n, k0, 32 * KG, n, tid);
+        keep_rows<T, DH, L::NT>(keep + L::KEEP, V, p.v_n, k0, 32 * KG, n, tid);
+        k.rows = keep + wave % KG * 32 * S::ROW;
+        v.rows = k.rows + L::KEEP;
+    } else {
+        k.load(K + (long)kj * p.k_n, lane >> 5, kj < n);
+        v.load(V + (long)kj * p.v_n, lane >> 5, kj < n);
+        k.settle();
+        v.settle();
+    }
     const float sc = p.scale * LOG2E;
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
     const int per = tl.count(), cnt = per * p.G;
     const Span sp = queries_of<CAUSAL>(kj, n, p.window, p.sinks);
-    const Stage<T, DH> fq(p.q_n, tid), fo(p.do_n, tid);
+    const Stage<T, DH, L::NT> fq(p.q_n, tid), fo(p.do_n, tid);
     int next_g = 0, next_t = 0;
     const auto start = [&](char* buf) {                 // the tiles in order, head after head
         const int h = hk * p.G + next_g, q0 = tl.at(next_t) * S::KT;
         fq.start(buf, (const T*)p.q + b * p.q_b + h * p.q_h, q0, n, tid);
-        fo.start(buf + BYTES, (const T*)p.d_o + b * p.do_b + h * p.do_h, q0, n, tid);
+        fo.start(buf + L::TILE, (const T*)p.d_o + b * p.do_b + h * p.do_h, q0, n, tid);
         if (wave < 2 * S::KT / 64) {                    // the rows' lse, delta: rows behind the sequence are masked
             const int x = wave * 64 + lane, i = q0 + x % S::KT;
             const float* from = (x < S::KT ? p.lse : p.delta) + ((long)b * p.Hq + h) * p.N + (i < n ? i : n - 1);
-            dma4(from, __builtin_amdgcn_readfirstlane(lds_addr(buf + 2 * BYTES) + wave * 256));
+            dma4(from, __builtin_amdgcn_readfirstlane(lds_addr(buf + 2 * L::TILE) + wave * 256));
         }
         if (++next_t == per) { next_t = 0; ++next_g; }
     };
     if (cnt > 0) start(lds);
     for (int t = 0, tt = 0; t < cnt; ++t, tt = tt + 1 == per ? 0 : tt + 1) {
-        const char* now = lds + (t & 1) * BUF;
+        const char* now = lds + (t & 1) * L::BUF;
         dma_wait();
         __syncthreads();
-        if (t + 1 < cnt) start(lds + (~t & 1) * BUF);
+        if (t + 1 < cnt) start(lds + (~t & 1) * L::BUF);
         const int q0 = tl.at(tt) * S::KT;
-        const float* Ls = reinterpret_cast<const float*>(now + 2 * BYTES);
+        const float* Ls = reinterpret_cast<const float*>(now + 2 * L::TILE);
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
-            if (KG == 2 && (((S::KT > 32 ? sub / 32 : t) + part) & 1)) continue;
+            if (L::PARTS == 2 && (((S::KT > 32 ? sub / 32 : t) + part) & 1)) continue;
             const int qa = q0 + sub;
             const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
             if (cov == 0) continue;
-            dkv_tile<T, DH>(now, now + BYTES, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1, sp, qa + 4 * (lane >> 5),
-                            !CAUSAL && qa < p.sinks);
+            const int x0 = qa + 4 * (lane >> 5);
+            const bool first = !CAUSAL && qa < p.sinks;
+            dkv_tile<T, DH>(now, now + L::TILE, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1, sp, x0, first);
         }
     }
-    if constexpr (KG == 2) {
-        constexpr int W = DH + 4;
-        static_assert(64 * W * 4 <= 2 * BUF, "the halves meet in the tiles' buffers");
-        float* at = reinterpret_cast<float*>(lds) + (wave % 2 * 32 + (lane & 31)) * W;
+    if constexpr (L::PARTS == 2) {
+        float* at = reinterpret_cast<float*>(lds) + (wave % KG * 32 + (lane & 31)) * (DH + 4);
         const auto meet = [&](f32x16* acc) {
             __syncthreads();
             if (part) put<float, DH>(at, acc, 1.f, lane);
@@ -821,26 +871,38 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
         put<T, DH>((T*)p.dv + b * p.dv_b + (long)kj * p.dv_n + hk * p.dv_h, dv, kj < n ? 1.f : 0.f, lane);
     }
 }
-// Far: 32 first keys against every (4 chunks)-th 32 queries behind their band, of every head that shares them.
-template <typename T, int DH, bool CAUSAL>
+// Far: 32 first keys against every (NW chunks)-th 32 queries behind their band, of every head that shares them.
+template <typename T, int DH, bool CAUSAL, int NW, int KG>
 __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk, int b, int n) {
     using S = Shape<T, DH>;
+    using L = Layout<T, DH, NW, KG>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int chunk = x % p.chunks, ka = x / p.chunks * 32, kj = ka + (lane & 31);
-    char* Qs = lds + wave * (2 * 32 * S::ROW + 256);
+    char* Qs = lds + wave * L::WAVE;
     char* Os = Qs + 32 * S::ROW;
     float* Ls = reinterpret_cast<float*>(Os + 32 * S::ROW);             // [32] lse, [32] delta
     const bool mine = kj < n && kj < p.sinks;
-    Kept<T, DH> k, v;
-    k.load((const T*)p.k + b * p.k_b + hk * p.k_h + (long)kj * p.k_n, lane >> 5, mine);
-    v.load((const T*)p.v + b * p.v_b + hk * p.v_h + (long)kj * p.v_n, lane >> 5, mine);
+    const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
+    const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
+    typename L::Keep k, v;
+    if constexpr (L::IN_LDS) {
+        char* keep = lds + NW * L::WAVE;
+        keep_rows<T, DH, L::NT>(keep, K, p.k_n, ka, 32, least(n, p.sinks), tid);
+        keep_rows<T, DH, L::NT>(keep + L::KEEP_FAR, V, p.v_n, ka, 32, least(n, p.sinks), tid);
+        k.rows = keep;
+        v.rows = keep + L::KEEP_FAR;
+        __syncthreads();
+    } else {
+        k.load(K + (long)kj * p.k_n, lane >> 5, mine);
+        v.load(V + (long)kj * p.v_n, lane >> 5, mine);
+    }
     const float sc = p.scale * LOG2E;
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
-    const int k0 = ka / p.tk * p.tk;
-    const Tiles tl = query_tiles<CAUSAL>(k0, k0 + p.tk - 1, n, p.window, p.sinks, S::KT);
+    const int k0 = ka / (32 * KG) * (32 * KG);
+    const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
     const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     const int per = ka < n && from < n ? (n - from + 31) / 32 : 0;
-    for (int t = chunk * 4 + wave; t < per * p.G; t += p.chunks * 4) {
+    for (int t = chunk * NW + wave; t < per * p.G; t += p.chunks * NW) {
         const int h = hk * p.G + t / per, q0 = from + t % per * 32;
         const long st = ((long)b * p.Hq + h) * p.N + q0;
         start_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, lane);
@@ -849,22 +911,23 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
         Ls[lane] = (lane < 32 ? p.lse : p.delta)[st + (q0 + r < n ? r : n - 1 - q0)];
         dma_wait();
         wave_lds_fence();
-        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, Span{0, mine ? n : 0, 0}, q0 + 4 * (lane >> 5), false);
+        const Span sp{0, mine ? n : 0, 0};
+        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, sp, q0 + 4 * (lane >> 5), false);
         wave_lds_fence();
     }
     const long stride = (long)(p.chunks + 1) * 2 * DH;
     float* rec = p.ws + (((long)b * p.Hkv + hk) * p.rows + ka) * stride + chunk * 2 * DH;
-    add_waves<DH>(lds, dk, rec, stride, tid);
-    add_waves<DH>(lds, dv, rec + DH, stride, tid);
+    add_waves<DH, NW>(lds, dk, rec, stride, tid);
+    add_waves<DH, NW>(lds, dv, rec + DH, stride, tid);
 }
-template <typename T, int DH, bool CAUSAL, int KG>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && DH < 128 ? 2 : 1) void slide_dkv_kernel(Slide p) {
+template <typename T, int DH, bool CAUSAL, int NW, int KG>
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && (DH < 128 || NW == 8) ? 2 : 1) void slide_dkv_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
     const Item it = item_of(p, p.Hkv, (p.N + 32 * KG - 1) / (32 * KG));
     if (it.none) return;
     const int n = length_of(p, it.b);
-    if (it.far) dkv_far<T, DH, CAUSAL>(p, lds, it.x, it.h, it.b, n);
-    else dkv_band<T, DH, CAUSAL, KG>(p, lds, it.x * (32 * KG), it.h, it.b, n);
+    if (it.far) dkv_far<T, DH, CAUSAL, NW, KG>(p, lds, it.x, it.h, it.b, n);
+    else dkv_band<T, DH, CAUSAL, NW, KG>(p, lds, it.x * (32 * KG), it.h, it.b, n);
 }
 // The records of the first rows become gradients: blockIdx.y < kv_heads dk and dv, behind them dq.  256 / DH shares of the
 // records, each in its order, then the shares in theirs.
@@ -988,16 +1051,17 @@ template <typename K> int allow_lds(K kernel, int bytes) {
     if (bytes <= 64 * 1024) return 0;
     return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
+constexpr int dkv_waves(bool bf16, int dh) { return bf16 && dh == 128 ? 8 : 4; }
 // Records of the first tokens: rows (a multiple of 32; 0: none needed), chunks of far items for each 32 of them, and floats
-// of workspace.  A chunk gives each wave about 8 far tiles, fewer chunks where there are items enough without them.
+// of workspace.  A chunk gives each of its waves about 4 far tiles; fewer chunks where there are items enough without them.
 struct Records { int rows, chunks; long floats; };
-Records records_of(int B, int N, int heads, int G, int width, int window, int sinks) {
+Records records_of(int B, int N, int heads, int G, int width, int window, int sinks, int waves) {
     Records r{0, 0, 0};
     if (sinks <= 0 || window >= N) return r;
     r.rows = (sinks + 31) / 32 * 32;
     const long far = (long)G * ((N + 31) / 32), items = (long)B * heads * (r.rows / 32);
     const long most = (2048 + items - 1) / items;
-    r.chunks = (int)((far + 31) / 32);
+    r.chunks = (int)((far + 4 * waves - 1) / (4 * waves));
     if (r.chunks > most) r.chunks = (int)most;
     if (r.chunks > 512) r.chunks = 512;
     r.floats = (long)B * heads * r.rows * (r.chunks + 1) * width;
@@ -1016,19 +1080,26 @@ unsigned grid_of(Slide& p, int heads, bool far, int rows = TQ) {
     p.items = (int)(p.far_items + bands);
     return (unsigned)(p.far_items + (bands + 7) / 8 * 8);
 }
-template <typename T, int DH> constexpr int lds_bytes(bool far, bool backward) {
-    const int band = 2 * (2 * Shape<T, DH>::KT * Shape<T, DH>::ROW + (backward ? 2 * Shape<T, DH>::KT * 4 : 0));
-    const int staged = 4 * (2 * 32 * Shape<T, DH>::ROW + (backward ? 256 : 0));
+template <typename T, int DH> constexpr int lds_bytes(bool far) {      // of the forward and the dQ kernel
+    const int band = 4 * Shape<T, DH>::KT * Shape<T, DH>::ROW, staged = 4 * 2 * 32 * Shape<T, DH>::ROW;
     const int joined = join_bytes<DH>(), wide = staged > joined ? staged : joined;
     return far && wide > band ? wide : band;
 }
+template <typename T, int DH, bool CAUSAL, int NW, int KG> int launch_dkv(Slide& p, hipStream_t st) {
+    const int bytes = Layout<T, DH, NW, KG>::bytes(p.rows > 0);
+    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, NW, KG>, bytes)) return e;
+    const unsigned grid = grid_of(p, p.Hkv, p.rows > 0, 32 * KG);
+    hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, NW, KG>), dim3(grid), dim3(NW * 64), bytes, st, p);
+    VITK_CHECK_LAUNCH();
+    return 0;
+}
 template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipStream_t st) {
     if (!CAUSAL) {
-        const Records r = records_of(p.B, p.N, p.Hq, 1, DH + 4, p.window, p.sinks);
+        const Records r = records_of(p.B, p.N, p.Hq, 1, DH + 4, p.window, p.sinks, 4);
         p.rows = r.rows; p.chunks = r.chunks; p.ws = ws;
         if (r.rows && !ws) return VITK_ERR_NULL;
     }
-    const int bytes = lds_bytes<T, DH>(p.rows > 0, false);
+    const int bytes = lds_bytes<T, DH>(p.rows > 0);
     if (int e = allow_lds(slide_fwd_kernel<T, DH, CAUSAL>, bytes)) return e;
     const unsigned grid = grid_of(p, p.Hq, p.rows > 0);
     hipLaunchKernelGGL((slide_fwd_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
@@ -1040,13 +1111,11 @@ template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipSt
     return 0;
 }
 template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipStream_t st) {
-    const Records rk = records_of(p.B, p.N, p.Hkv, p.G, 2 * DH, p.window, p.sinks);
-    const Records rq = CAUSAL ? Records{0, 0, 0} : records_of(p.B, p.N, p.Hq, 1, DH, p.window, p.sinks);
+    const Records rk = records_of(p.B, p.N, p.Hkv, p.G, 2 * DH, p.window, p.sinks, dkv_waves(sizeof(T) == 2, DH));
+    const Records rq = CAUSAL ? Records{0, 0, 0} : records_of(p.B, p.N, p.Hq, 1, DH, p.window, p.sinks, 4);
     if (rk.rows && !ws) return VITK_ERR_NULL;
-    const int bytes = lds_bytes<T, DH>(rk.rows > 0, true);
+    const int bytes = lds_bytes<T, DH>(rq.rows > 0);
     if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL>, bytes)) return e;
-    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, 4>, bytes)) return e;
-    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, 2>, bytes)) return e;
     p.ws = ws;
     p.ws_q = ws + rk.floats;
     if (p.dq) {
@@ -1059,13 +1128,12 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipSt
     VITK_CHECK_LAUNCH();
     if (p.dk) {
         p.rows = rk.rows; p.chunks = rk.chunks;
+        int e;
+        if constexpr (dkv_waves(sizeof(T) == 2, DH) == 8) e = launch_dkv<T, DH, CAUSAL, 8, 4>(p, st);
         // few key heads leave CUs without a band of 128 keys: bands of 64 below two of them for each CU
-        const bool narrow = (long)vitk_ceil_div(p.N, TQ) * p.Hkv * p.B < 512;
-        p.tk = narrow ? 64 : 128;
-        const unsigned grid = grid_of(p, p.Hkv, rk.rows > 0, p.tk);
-        if (narrow) hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, 2>), dim3(grid), dim3(256), bytes, st, p);
-        else hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, 4>), dim3(grid), dim3(256), bytes, st, p);
-        VITK_CHECK_LAUNCH();
+        else if ((long)vitk_ceil_div(p.N, TQ) * p.Hkv * p.B < 512) e = launch_dkv<T, DH, CAUSAL, 4, 2>(p, st);
+        else e = launch_dkv<T, DH, CAUSAL, 4, 4>(p, st);
+        if (e) return e;
     }
     const int kv_heads = p.dk ? p.Hkv : 0, q_heads = p.dq && rq.rows ? p.Hq : 0;
     if (rk.rows && kv_heads + q_heads) {
@@ -1148,16 +1216,16 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     if (a->dh == 64) return a->causal ? CALL(float, 64, true) : CALL(float, 64, false);                               \
     return a->causal ? CALL(float, 128, true) : CALL(float, 128, false)
 
-extern "C" size_t vitk_slide_attn_workspace(const vitk_slide_attn* a, int backward) {
+extern "C" size_t vitk_slide_attn_workspace(const vitk_slide_attn* a, int dtype, int backward) {
     if (!a || a->B <= 0 || a->N <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->dh <= 0) return 0;
     int window, sinks;
     reach(a, window, sinks);
     long n = 0;
     if (!backward) {
-        if (!a->causal) n = records_of(a->B, a->N, a->Hq, 1, a->dh + 4, window, sinks).floats;
+        if (!a->causal) n = records_of(a->B, a->N, a->Hq, 1, a->dh + 4, window, sinks, 4).floats;
     } else {
-        n = records_of(a->B, a->N, a->Hkv, a->Hq / a->Hkv, 2 * a->dh, window, sinks).floats;
-        if (!a->causal) n += records_of(a->B, a->N, a->Hq, 1, a->dh, window, sinks).floats;
+        n = records_of(a->B, a->N, a->Hkv, a->Hq / a->Hkv, 2 * a->dh, window, sinks, dkv_waves(dtype == VITK_BF16, a->dh)).floats;
+        if (!a->causal) n += records_of(a->B, a->N, a->Hq, 1, a->dh, window, sinks, 4).floats;
     }
     return (size_t)n * sizeof(float);
 }

@@ -125,7 +125,7 @@ lib.vitk_layernorm_bwd_workspace.argtypes = [ctypes.c_int, ctypes.c_int]
 lib.vitk_groupnorm_workspace.restype = ctypes.c_size_t
 lib.vitk_groupnorm_workspace.argtypes = [ctypes.c_int] * 4
 lib.vitk_slide_attn_workspace.restype = ctypes.c_size_t
-lib.vitk_slide_attn_workspace.argtypes = [ctypes.POINTER(SlideAttn), ctypes.c_int]
+lib.vitk_slide_attn_workspace.argtypes = [ctypes.POINTER(SlideAttn), ctypes.c_int, ctypes.c_int]
 for _name, _args in PROTOTYPES.items():
     _fn = getattr(lib, _name)
     _fn.argtypes = _args

@@ -194,9 +194,9 @@ def _slide_args(q, k, v, o, o32, lse, lengths, meta, d_o=None, delta=None, dq=No
                      None, *st, q.shape[0], q.shape[1], q.shape[2], k.shape[2], q.shape[3], window, sinks, int(causal), scale)
 
 
-def _slide_workspace(a, backward, device):
+def _slide_workspace(a, code, backward, device):
     """The records of the first tokens (16-byte aligned memory of this call and stream)."""
-    n = lib.vitk_slide_attn_workspace(ctypes.byref(a), int(backward))
+    n = lib.vitk_slide_attn_workspace(ctypes.byref(a), code, int(backward))
     if not n:
         return None
     ws = torch.empty(n // 4, dtype=torch.float32, device=device)
@@ -213,8 +213,9 @@ def _slide_forward(q, k, v, lengths, meta, keep):
     if o.numel():
         with _On(q.device) as on:
             a = _slide_args(q, k, v, o, o32, lse, lengths, meta)
-            ws = _slide_workspace(a, False, q.device)  # noqa: F841  (lives until the launch is enqueued)
-            check(lib.vitk_slide_attn_fwd(ctypes.byref(a), dtype_code(q.dtype), on.stream), "vitk_slide_attn_fwd")
+            code = dtype_code(q.dtype)
+            ws = _slide_workspace(a, code, False, q.device)  # noqa: F841  (lives until the launch is enqueued)
+            check(lib.vitk_slide_attn_fwd(ctypes.byref(a), code, on.stream), "vitk_slide_attn_fwd")
     return o, o32, lse
 
 
@@ -225,8 +226,9 @@ def _slide_backward(q, k, v, o, o32, lse, lengths, meta, d_o, dq, dk, dv):
     delta = torch.empty_like(lse)
     with _On(q.device) as on:
         a = _slide_args(q, k, v, o, o32, lse, lengths, meta, d_o, delta, dq, dk, dv)
-        ws = _slide_workspace(a, True, q.device)  # noqa: F841
-        check(lib.vitk_slide_attn_bwd(ctypes.byref(a), dtype_code(q.dtype), on.stream), "vitk_slide_attn_bwd")
+        code = dtype_code(q.dtype)
+        ws = _slide_workspace(a, code, True, q.device)  # noqa: F841
+        check(lib.vitk_slide_attn_bwd(ctypes.byref(a), code, on.stream), "vitk_slide_attn_bwd")
 
 
 class SlidingAttentionFn(torch.autograd.Function):
