@@ -18,6 +18,7 @@
 // ordinary rows, the few first tokens on the other side), and what the first tokens see beyond their band is cut into
 // chunks of FAR items: 32 first tokens against a share of the far rows, dealt out to four waves that meet in LDS.
 // Bands and chunks of a first token leave 32-bit records in a workspace, which a last small launch adds in a fixed order.
+// Where the whole sequence is not much longer than a band, one item does all of 32 first tokens and nothing is left to add.
 // (Without the split one workgroup per head walked the whole sequence: 6.9 ms instead of the time below at 16384 tokens.)
 #include <initializer_list>
 
@@ -37,8 +38,9 @@ struct Slide {
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, do_b, do_n, do_h, dq_b, dq_n, dq_h, dk_b, dk_n, dk_h, dv_b, dv_n, dv_h;
     int window, sinks;
     float scale;
-    int rows;                  // first tokens with records, a multiple of 32 (0: none)
-    int chunks;                // far items of each 32 of them; a row has chunks + 1 records, the band's last
+    int rows;                  // first tokens in items of their own, a multiple of 32 (0: none)
+    int chunks;                // far items of each 32 of them; a row has chunks + 1 records, the band's last.  0: one item
+                               // for all that 32 of them see, and no records
     float* ws;                 // forward: records of dh + 2; backward: dk | dv, then dq, records of dh
     float* ws_q;
     int far_items, items;      // of this launch: far ones come first, then bands
@@ -385,7 +387,7 @@ __device__ __forceinline__ Item item_of(const Slide& p, int heads, int tiles) {
     int k;
     if (it.far) {
         k = id;
-        tiles = p.chunks * (p.rows / 32);
+        tiles = (p.chunks ? p.chunks : 1) * (p.rows / 32);
     } else {
         const int m = p.items - p.far_items, each = (m + 7) / 8, r = id - p.far_items;
         k = (r & 7) * each + (r >> 3);
@@ -425,8 +427,8 @@ template <int DH, typename F> __device__ __forceinline__ void join_waves(char* l
         f(c, d, x, top, sum);
     }
 }
-// The plain sum of NW waves', to records `stride` floats apart.
-template <int DH, int NW = 4> __device__ __forceinline__ void add_waves(char* lds, const f32x16* acc, float* rec, long stride, int tid) {
+// The plain sum of NW waves': called by all threads, f(column, d, sum).
+template <int DH, int NW, typename F> __device__ __forceinline__ void add_waves(char* lds, const f32x16* acc, int tid, F f) {
     constexpr int W = DH + 4;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* out = reinterpret_cast<float*>(lds);
@@ -438,7 +440,7 @@ template <int DH, int NW = 4> __device__ __forceinline__ void add_waves(char* ld
         float x = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) x += out[(w * 32 + c) * W + d];
-        rec[c * stride + d] = x;
+        f(c, d, x);
     }
 }
 
@@ -479,6 +481,15 @@ template <typename T, int DH> __device__ __forceinline__ void start_wave(char* t
 }
 
 // ----------------------------------------------------------------------------- forward
+// Element d of an output row from its sums, the maximum behind them (base 2) and their total.
+template <typename T, int DH>
+__device__ __forceinline__ void write_row(const Slide& p, int b, int h, int i, int d, float sum, float top, float total) {
+    const float x = total > 0.f ? sum / total : 0.f;
+    const long row = ((long)b * p.N + i) * p.Hq + h;
+    ((T*)p.o)[row * DH + d] = (T)x;
+    if (p.o32) p.o32[row * DH + d] = x;
+    if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.N + i] = total > 0.f ? top + __log2f(total) : INFINITY;
+}
 // Band: 128 queries of one (sequence, head), each wave 32 of them; key tiles stream through LDS.
 template <typename T, int DH, bool CAUSAL>
 __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
@@ -490,6 +501,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
     Kept<T, DH> q;
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, qi < n);
     q.settle();
+    const bool elsewhere = !CAUSAL && qa < p.rows && !p.chunks;          // an item of its own does these rows
     const float sc = p.scale * LOG2E;
     const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
@@ -504,7 +516,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
             const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
-            if (cov == 0) continue;
+            if (cov == 0 || elsewhere) continue;
             f32x16 s = product<DH>(Ks, sub, q, lane);
             if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, -INFINITY);
             sm.step(s, sc, rescale);
@@ -512,7 +524,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         }
     });
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
-    if (qi < p.N) {
+    if (qi < p.N && !elsewhere) {
         if (!CAUSAL && qi < p.rows) {
             float* rec = p.ws + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * (DH + 4);
             put<float, DH>(rec, acc, 1.f, lane);
@@ -527,32 +539,35 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         if (p.lse && lane < 32) p.lse[((long)b * p.Hq + h) * p.N + qi] = l > 0.f ? m + __log2f(l) : INFINITY;
     }
 }
-// Far: 32 first queries against every (4 chunks)-th 32 keys behind their band.
+// Far: 32 first queries against every (4 chunks)-th 32 keys behind their band; or, without chunks, against all they see.
 template <typename T, int DH>
 __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h, int b, int n) {
     using S = Shape<T, DH>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
-    const int chunk = x % p.chunks, qa = x / p.chunks * 32, qi = qa + (lane & 31);
+    const bool all = !p.chunks;
+    const int chunks = all ? 1 : p.chunks, chunk = x % chunks, qa = x / chunks * 32, qi = qa + (lane & 31);
     char* Ks = lds + wave * 2 * 32 * S::ROW;
     char* Vs = Ks + 32 * S::ROW;
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
-    const bool mine = qi < n && qi < p.sinks;
+    const bool mine = qi < n && (all || qi < p.sinks);
     Kept<T, DH> q;
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, mine);
     const float sc = p.scale * LOG2E;
+    const Span sp = all ? keys_of<false>(qi, n, p.window, p.sinks) : Span{0, mine ? n : 0, 0};
     f32x16 acc[DH / 32] = {};
     Softmax sm;
     const int q0 = qa / TQ * TQ;
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
-    for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
+    const int from = all ? 0 : (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += chunks * 4 * 32) {
+        if (all && coverage<false>(qa, qa + 31, k0, k0 + 31, n, p.window, p.sinks) == 0) continue;
         start_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
         start_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
         dma_wait();
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
-        hide(s, Span{0, mine ? n : 0, 0}, k0 + 4 * (lane >> 5), false, -INFINITY);
+        hide(s, sp, k0 + 4 * (lane >> 5), k0 < p.sinks, -INFINITY);
         sm.step(s, sc, [&](float alpha) {
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
@@ -561,9 +576,13 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
         wave_lds_fence();
     }
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
-    float* base = p.ws + ((((long)b * p.Hq + h) * p.rows + qa) * (p.chunks + 1) + chunk) * (DH + 4);
+    float* base = p.ws + ((((long)b * p.Hq + h) * p.rows + qa) * (chunks + 1) + chunk) * (DH + 4);
     join_waves<DH>(lds, acc, m, l, tid, [&](int c, int d, float sum, float top, float total) {
-        float* rec = base + (long)c * (p.chunks + 1) * (DH + 4);
+        if (all) {
+            if (qa + c < p.N) write_row<T, DH>(p, b, h, qa + c, d, sum, top, total);
+            return;
+        }
+        float* rec = base + (long)c * (chunks + 1) * (DH + 4);
         rec[d] = sum;
         if (d == 0) { rec[DH] = top; rec[DH + 1] = total; }
     });
@@ -592,11 +611,7 @@ template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) vo
         x += r[d] * e;
         sum += r[DH + 1] * e;
     }
-    x = sum > 0.f ? x / sum : 0.f;
-    const long row = ((long)b * p.N + i) * p.Hq + h;
-    ((T*)p.o)[row * DH + d] = (T)x;
-    if (p.o32) p.o32[row * DH + d] = x;
-    if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.N + i] = sum > 0.f ? top + __log2f(sum) : INFINITY;
+    write_row<T, DH>(p, b, h, i, d, x, top, sum);
 }
 
 // ----------------------------------------------------------------------------- backward
@@ -666,6 +681,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     d_o.settle();
     arrived(lse);
     arrived(delta);
+    const bool elsewhere = !CAUSAL && qa < p.rows && !p.chunks;
     const float sc = p.scale * LOG2E;
     const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
@@ -675,7 +691,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
             const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
-            if (cov == 0) continue;
+            if (cov == 0 || elsewhere) continue;
             f32x16 s = product<DH>(Ks, sub, q, lane);
             const f32x16 dp = product<DH>(Vs, sub, d_o, lane);
 #pragma unroll
@@ -684,7 +700,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
             gather<DH>(acc, Ks, sub, s, lane, T{});
         }
     });
-    if (qi >= p.N) return;
+    if (qi >= p.N || elsewhere) return;
     if (!CAUSAL && qi < p.rows)
         put<float, DH>(p.ws_q + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * DH, acc, 1.f, lane);
     else
@@ -694,12 +710,13 @@ template <typename T, int DH>
 __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, int b, int n) {
     using S = Shape<T, DH>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
-    const int chunk = x % p.chunks, qa = x / p.chunks * 32, qi = qa + (lane & 31);
+    const bool all = !p.chunks;
+    const int chunks = all ? 1 : p.chunks, chunk = x % chunks, qa = x / chunks * 32, qi = qa + (lane & 31);
     char* Ks = lds + wave * 2 * 32 * S::ROW;
     char* Vs = Ks + 32 * S::ROW;
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
-    const bool mine = qi < n && qi < p.sinks;
+    const bool mine = qi < n && (all || qi < p.sinks);
     Kept<T, DH> q, d_o;
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, mine);
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, mine);
@@ -707,25 +724,30 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     const float lse = mine ? p.lse[st] : INFINITY;                       // not mine: probabilities of 0
     const float delta = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, mine);
     const float sc = p.scale * LOG2E;
+    const Span sp = all ? keys_of<false>(qi, n, p.window, p.sinks) : Span{0, n, 0};
     f32x16 acc[DH / 32] = {};
     const int q0 = qa / TQ * TQ;
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
-    for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += p.chunks * 4 * 32) {
+    const int from = all ? 0 : (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += chunks * 4 * 32) {
+        if (all && coverage<false>(qa, qa + 31, k0, k0 + 31, n, p.window, p.sinks) == 0) continue;
         start_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
         start_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
         dma_wait();
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
-        hide(s, Span{0, n, 0}, k0 + 4 * (lane >> 5), false, -INFINITY);
         const f32x16 dp = product<DH>(Vs, 0, d_o, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
+        hide(s, sp, k0 + 4 * (lane >> 5), k0 < p.sinks, 0.f);
         gather<DH>(acc, Ks, 0, s, lane, T{});
         wave_lds_fence();
     }
-    const long stride = (long)(p.chunks + 1) * DH;
-    add_waves<DH>(lds, acc, p.ws_q + (((long)b * p.Hq + h) * p.rows + qa) * stride + chunk * DH, stride, tid);
+    add_waves<DH, 4>(lds, acc, tid, [&](int c, int d, float sum) {
+        const int i = qa + c;
+        if (!all) p.ws_q[((((long)b * p.Hq + h) * p.rows + i) * (chunks + 1) + chunk) * DH + d] = sum;
+        else if (i < p.N) ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(i < n ? sum * p.scale : 0.f);
+    });
 }
 template <typename T, int DH, bool CAUSAL>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void slide_dq_kernel(Slide p) {
@@ -813,6 +835,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
     const int per = tl.count(), cnt = per * p.G;
     const Span sp = queries_of<CAUSAL>(kj, n, p.window, p.sinks);
+    const bool elsewhere = ka < p.rows && !p.chunks;
     const Stage<T, DH, L::NT> fq(p.q_n, tid), fo(p.do_n, tid);
     int next_g = 0, next_t = 0;
     const auto start = [&](char* buf) {                 // the tiles in order, head after head
@@ -839,7 +862,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
             if (L::PARTS == 2 && (((S::KT > 32 ? sub / 32 : t) + part) & 1)) continue;
             const int qa = q0 + sub;
             const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
-            if (cov == 0) continue;
+            if (cov == 0 || elsewhere) continue;
             const int x0 = qa + 4 * (lane >> 5);
             const bool first = !CAUSAL && qa < p.sinks;
             dkv_tile<T, DH>(now, now + L::TILE, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1, sp, x0, first);
@@ -861,7 +884,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
         meet(dv);
         if (part) return;
     }
-    if (kj >= p.N) return;
+    if (kj >= p.N || elsewhere) return;
     if (kj < p.rows) {
         float* rec = p.ws + ((((long)b * p.Hkv + hk) * p.rows + kj) * (p.chunks + 1) + p.chunks) * (2 * DH);
         put<float, DH>(rec, dk, 1.f, lane);
@@ -877,18 +900,20 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     using S = Shape<T, DH>;
     using L = Layout<T, DH, NW, KG>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int chunk = x % p.chunks, ka = x / p.chunks * 32, kj = ka + (lane & 31);
+    const bool all = !p.chunks;
+    const int chunks = all ? 1 : p.chunks, chunk = x % chunks, ka = x / chunks * 32, kj = ka + (lane & 31);
     char* Qs = lds + wave * L::WAVE;
     char* Os = Qs + 32 * S::ROW;
     float* Ls = reinterpret_cast<float*>(Os + 32 * S::ROW);             // [32] lse, [32] delta
-    const bool mine = kj < n && kj < p.sinks;
+    const int last = all ? n : least(n, p.sinks);
+    const bool mine = kj < last;
     const T* K = (const T*)p.k + b * p.k_b + hk * p.k_h;
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
     typename L::Keep k, v;
     if constexpr (L::IN_LDS) {
         char* keep = lds + NW * L::WAVE;
-        keep_rows<T, DH, L::NT>(keep, K, p.k_n, ka, 32, least(n, p.sinks), tid);
-        keep_rows<T, DH, L::NT>(keep + L::KEEP_FAR, V, p.v_n, ka, 32, least(n, p.sinks), tid);
+        keep_rows<T, DH, L::NT>(keep, K, p.k_n, ka, 32, last, tid);
+        keep_rows<T, DH, L::NT>(keep + L::KEEP_FAR, V, p.v_n, ka, 32, last, tid);
         k.rows = keep;
         v.rows = keep + L::KEEP_FAR;
         __syncthreads();
@@ -900,10 +925,12 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
     const int k0 = ka / (32 * KG) * (32 * KG);
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
-    const int from = (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    const int from = all ? 0 : (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    const Span sp = all ? queries_of<CAUSAL>(kj, n, p.window, p.sinks) : Span{0, mine ? n : 0, 0};
     const int per = ka < n && from < n ? (n - from + 31) / 32 : 0;
-    for (int t = chunk * NW + wave; t < per * p.G; t += p.chunks * NW) {
+    for (int t = chunk * NW + wave; t < per * p.G; t += chunks * NW) {
         const int h = hk * p.G + t / per, q0 = from + t % per * 32;
+        if (all && coverage<CAUSAL>(q0, q0 + 31, ka, ka + 31, n, p.window, p.sinks) == 0) continue;
         const long st = ((long)b * p.Hq + h) * p.N + q0;
         start_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, lane);
         start_wave<T, DH>(Os, (const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n, q0, n, lane);
@@ -911,14 +938,22 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
         Ls[lane] = (lane < 32 ? p.lse : p.delta)[st + (q0 + r < n ? r : n - 1 - q0)];
         dma_wait();
         wave_lds_fence();
-        const Span sp{0, mine ? n : 0, 0};
-        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, sp, q0 + 4 * (lane >> 5), false);
+        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, sp, q0 + 4 * (lane >> 5), !CAUSAL && q0 < p.sinks);
         wave_lds_fence();
     }
-    const long stride = (long)(p.chunks + 1) * 2 * DH;
-    float* rec = p.ws + (((long)b * p.Hkv + hk) * p.rows + ka) * stride + chunk * 2 * DH;
-    add_waves<DH, NW>(lds, dk, rec, stride, tid);
-    add_waves<DH, NW>(lds, dv, rec + DH, stride, tid);
+    const auto leave = [&](f32x16* acc, bool values) {
+        add_waves<DH, NW>(lds, acc, tid, [&](int c, int d, float sum) {
+            const int j = ka + c;
+            if (!all) {
+                p.ws[((((long)b * p.Hkv + hk) * p.rows + j) * (chunks + 1) + chunk) * (2 * DH) + (values ? DH : 0) + d] = sum;
+            } else if (j < p.N) {
+                if (values) ((T*)p.dv)[b * p.dv_b + (long)j * p.dv_n + hk * p.dv_h + d] = (T)(j < n ? sum : 0.f);
+                else ((T*)p.dk)[b * p.dk_b + (long)j * p.dk_n + hk * p.dk_h + d] = (T)(j < n ? sum * p.scale : 0.f);
+            }
+        });
+    };
+    leave(dk, false);
+    leave(dv, true);
 }
 template <typename T, int DH, bool CAUSAL, int NW, int KG>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && (DH < 128 || NW == 8) ? 2 : 1) void slide_dkv_kernel(Slide p) {
@@ -1052,16 +1087,19 @@ template <typename K> int allow_lds(K kernel, int bytes) {
     return (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 constexpr int dkv_waves(bool bf16, int dh) { return bf16 && dh == 128 ? 8 : 4; }
-// Records of the first tokens: rows (a multiple of 32; 0: none needed), chunks of far items for each 32 of them, and floats
-// of workspace.  A chunk gives each of its waves about 4 far tiles; fewer chunks where there are items enough without them.
+// Items of the first tokens: rows (a multiple of 32; 0: none needed), chunks of far items for each 32 of them, floats of
+// workspace for their records.  One item for all (no records, no second launch) while that is at most 24 turns of its waves,
+// of a microsecond or so each (FIGURES); else a chunk gives each of its waves about 4 far tiles, and fewer chunks do
+// where there are items enough without them.
 struct Records { int rows, chunks; long floats; };
 Records records_of(int B, int N, int heads, int G, int width, int window, int sinks, int waves) {
     Records r{0, 0, 0};
     if (sinks <= 0 || window >= N) return r;
     r.rows = (sinks + 31) / 32 * 32;
-    const long far = (long)G * ((N + 31) / 32), items = (long)B * heads * (r.rows / 32);
-    const long most = (2048 + items - 1) / items;
-    r.chunks = (int)((far + 4 * waves - 1) / (4 * waves));
+    const long tiles = (long)G * ((N + 31) / 32);
+    if (tiles <= 24 * waves) return r;
+    const long items = (long)B * heads * (r.rows / 32), most = (2048 + items - 1) / items;
+    r.chunks = (int)((tiles + 4 * waves - 1) / (4 * waves));
     if (r.chunks > most) r.chunks = (int)most;
     if (r.chunks > 512) r.chunks = 512;
     r.floats = (long)B * heads * r.rows * (r.chunks + 1) * width;
@@ -1075,7 +1113,7 @@ void reach(const vitk_slide_attn* a, int& window, int& sinks) {
     if (window >= a->N) sinks = 0;
 }
 unsigned grid_of(Slide& p, int heads, bool far, int rows = TQ) {
-    p.far_items = far ? p.chunks * (p.rows / 32) * heads * p.B : 0;
+    p.far_items = far ? (p.chunks ? p.chunks : 1) * (p.rows / 32) * heads * p.B : 0;
     const long bands = (long)vitk_ceil_div(p.N, rows) * heads * p.B;
     p.items = (int)(p.far_items + bands);
     return (unsigned)(p.far_items + (bands + 7) / 8 * 8);
@@ -1097,14 +1135,14 @@ template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipSt
     if (!CAUSAL) {
         const Records r = records_of(p.B, p.N, p.Hq, 1, DH + 4, p.window, p.sinks, 4);
         p.rows = r.rows; p.chunks = r.chunks; p.ws = ws;
-        if (r.rows && !ws) return VITK_ERR_NULL;
+        if (r.floats && !ws) return VITK_ERR_NULL;
     }
     const int bytes = lds_bytes<T, DH>(p.rows > 0);
     if (int e = allow_lds(slide_fwd_kernel<T, DH, CAUSAL>, bytes)) return e;
     const unsigned grid = grid_of(p, p.Hq, p.rows > 0);
     hipLaunchKernelGGL((slide_fwd_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
     VITK_CHECK_LAUNCH();
-    if (p.rows) {
+    if (p.chunks) {
         hipLaunchKernelGGL((slide_fwd_join_kernel<T, DH>), dim3(p.rows < p.N ? p.rows : p.N, p.Hq, p.B), dim3(DH < 64 ? 64 : DH), 0, st, p);
         VITK_CHECK_LAUNCH();
     }
@@ -1113,7 +1151,7 @@ template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipSt
 template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipStream_t st) {
     const Records rk = records_of(p.B, p.N, p.Hkv, p.G, 2 * DH, p.window, p.sinks, dkv_waves(sizeof(T) == 2, DH));
     const Records rq = CAUSAL ? Records{0, 0, 0} : records_of(p.B, p.N, p.Hq, 1, DH, p.window, p.sinks, 4);
-    if (rk.rows && !ws) return VITK_ERR_NULL;
+    if (rk.floats + rq.floats && !ws) return VITK_ERR_NULL;
     const int bytes = lds_bytes<T, DH>(rq.rows > 0);
     if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL>, bytes)) return e;
     p.ws = ws;
@@ -1135,8 +1173,8 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipSt
         else e = launch_dkv<T, DH, CAUSAL, 4, 4>(p, st);
         if (e) return e;
     }
-    const int kv_heads = p.dk ? p.Hkv : 0, q_heads = p.dq && rq.rows ? p.Hq : 0;
-    if (rk.rows && kv_heads + q_heads) {
+    const int kv_heads = p.dk && rk.chunks ? p.Hkv : 0, q_heads = p.dq && rq.chunks ? p.Hq : 0;
+    if (kv_heads + q_heads) {
         hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(rk.rows < p.N ? rk.rows : p.N, kv_heads + q_heads, p.B), dim3(256), 0, st,
                            p, kv_heads, rk.rows, rk.chunks + 1, rq.chunks + 1);
         VITK_CHECK_LAUNCH();
