@@ -144,6 +144,16 @@ def test_what_lies_behind_a_sequence_is_not_looked_at(dt, causal):
 
 
 @pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,window,sinks,causal,lengths", [(1, 1, 0, True, None), (1, 9, 2, False, None), (150, 1, 0, True, None),
+                                                           (150, 1, 0, False, (150, 33)), (3000, 0, 1, True, None), (90, 20, 3, False, (1, 1))])
+def test_scores_of_queries_that_see_one_key_have_no_gradient(dt, N, window, sinks, causal, lengths):
+    q, k, v, d_o = _case(dt, N=N)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    o, dq, dk, dv = _grads(q, k, v, d_o, window=window, sinks=sinks, causal=causal, lengths=n)
+    assert not dq.any() and not dk.any() and dv.any()
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("level", [-900.0, 900.0])
 def test_scores_far_from_zero(dt, causal, level):

@@ -38,6 +38,7 @@ struct Slide {
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, do_b, do_n, do_h, dq_b, dq_n, dq_h, dk_b, dk_n, dk_h, dv_b, dv_n, dv_h;
     int window, sinks;
     float scale;
+    int single;                // whether every query sees one key only, however long the sequence
     int rows;                  // first tokens in items of their own, a multiple of 32 (0: none)
     int chunks;                // far items of each 32 of them; a row has chunks + 1 records, the band's last.  0: one item
                                // for all that 32 of them see, and no records
@@ -327,6 +328,9 @@ template <typename T, int DH> __device__ __forceinline__ void put(T* row, const 
             Vec4<T>::store(row + 32 * d + 8 * b + 4 * (lane >> 5), x);
         }
 }
+// What the sums of dQ and dK are multiplied with.  A query that sees one key only has the probability 1 whatever its score:
+// where all do, the gradients of the scores are exactly 0, and not what dP - delta leaves after rounding.
+__device__ __forceinline__ float score_scale(const Slide& p, int n) { return p.single || n == 1 ? 0.f : p.scale; }
 // LDS written by other lanes of this wave may be read behind it (a wave's LDS accesses take effect in order).
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -401,8 +405,8 @@ __device__ __forceinline__ Item item_of(const Slide& p, int heads, int tiles) {
 // Sums of the waves, [32 columns][DH + 4] each, in LDS.
 template <int DH> constexpr int join_bytes(int waves = 4) { return waves * 32 * (DH + 4) * (int)sizeof(float); }
 
-// One record of the softmax of a row from the four waves': called by all threads, f(column, d, sum, maximum, total).
-template <int DH, typename F> __device__ __forceinline__ void join_waves(char* lds, const f32x16* acc, float m, float l, int tid, F f) {
+// One record of the softmax of a row from NW waves': called by all threads, f(column, d, sum, maximum, total).
+template <int DH, int NW, typename F> __device__ __forceinline__ void join_waves(char* lds, const f32x16* acc, float m, float l, int tid, F f) {
     constexpr int W = DH + 4;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float* out = reinterpret_cast<float*>(lds);
@@ -411,14 +415,14 @@ template <int DH, typename F> __device__ __forceinline__ void join_waves(char* l
     put<float, DH>(mine, acc, 1.f, lane);
     if (lane < 32) { mine[DH] = m; mine[DH + 1] = l; }
     __syncthreads();
-    for (int idx = tid; idx < 32 * DH; idx += 256) {
+    for (int idx = tid; idx < 32 * DH; idx += NW * 64) {
         const int c = idx / DH, d = idx % DH;
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, out[(w * 32 + c) * W + DH]);
+        for (int w = 0; w < NW; ++w) top = fmaxf(top, out[(w * 32 + c) * W + DH]);
         float x = 0.f, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < NW; ++w) {
             const float* rec = out + (w * 32 + c) * W;
             const float e = rec[DH] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(rec[DH] - top);
             x += rec[d] * e;
@@ -577,7 +581,7 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
     }
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
     float* base = p.ws + ((((long)b * p.Hq + h) * p.rows + qa) * (chunks + 1) + chunk) * (DH + 4);
-    join_waves<DH>(lds, acc, m, l, tid, [&](int c, int d, float sum, float top, float total) {
+    join_waves<DH, 4>(lds, acc, m, l, tid, [&](int c, int d, float sum, float top, float total) {
         if (all) {
             if (qa + c < p.N) write_row<T, DH>(p, b, h, qa + c, d, sum, top, total);
             return;
@@ -704,7 +708,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     if (!CAUSAL && qi < p.rows)
         put<float, DH>(p.ws_q + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * DH, acc, 1.f, lane);
     else
-        put<T, DH>((T*)p.dq + b * p.dq_b + (long)qi * p.dq_n + h * p.dq_h, acc, qi < n ? p.scale : 0.f, lane);
+        put<T, DH>((T*)p.dq + b * p.dq_b + (long)qi * p.dq_n + h * p.dq_h, acc, qi < n ? score_scale(p, n) : 0.f, lane);
 }
 template <typename T, int DH>
 __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, int b, int n) {
@@ -746,7 +750,7 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     add_waves<DH, 4>(lds, acc, tid, [&](int c, int d, float sum) {
         const int i = qa + c;
         if (!all) p.ws_q[((((long)b * p.Hq + h) * p.rows + i) * (chunks + 1) + chunk) * DH + d] = sum;
-        else if (i < p.N) ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(i < n ? sum * p.scale : 0.f);
+        else if (i < p.N) ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(i < n ? sum * score_scale(p, n) : 0.f);
     });
 }
 template <typename T, int DH, bool CAUSAL>
@@ -890,7 +894,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
         put<float, DH>(rec, dk, 1.f, lane);
         put<float, DH>(rec + DH, dv, 1.f, lane);
     } else {
-        put<T, DH>((T*)p.dk + b * p.dk_b + (long)kj * p.dk_n + hk * p.dk_h, dk, kj < n ? p.scale : 0.f, lane);
+        put<T, DH>((T*)p.dk + b * p.dk_b + (long)kj * p.dk_n + hk * p.dk_h, dk, kj < n ? score_scale(p, n) : 0.f, lane);
         put<T, DH>((T*)p.dv + b * p.dv_b + (long)kj * p.dv_n + hk * p.dv_h, dv, kj < n ? 1.f : 0.f, lane);
     }
 }
@@ -948,7 +952,7 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
                 p.ws[((((long)b * p.Hkv + hk) * p.rows + j) * (chunks + 1) + chunk) * (2 * DH) + (values ? DH : 0) + d] = sum;
             } else if (j < p.N) {
                 if (values) ((T*)p.dv)[b * p.dv_b + (long)j * p.dv_n + hk * p.dv_h + d] = (T)(j < n ? sum : 0.f);
-                else ((T*)p.dk)[b * p.dk_b + (long)j * p.dk_n + hk * p.dk_h + d] = (T)(j < n ? sum * p.scale : 0.f);
+                else ((T*)p.dk)[b * p.dk_b + (long)j * p.dk_n + hk * p.dk_h + d] = (T)(j < n ? sum * score_scale(p, n) : 0.f);
             }
         });
     };
@@ -987,12 +991,13 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_bwd_j
     if (share) return;
 #pragma unroll
     for (int s = 1; s < SHARES; ++s) { x += part[0][s * DH + d]; y += part[1][s * DH + d]; }
-    const bool there = i < length_of(p, b);
+    const int n = length_of(p, b);
+    const bool there = i < n;
     if (keys) {
-        ((T*)p.dk)[b * p.dk_b + (long)i * p.dk_n + hk * p.dk_h + d] = (T)(there ? x * p.scale : 0.f);
+        ((T*)p.dk)[b * p.dk_b + (long)i * p.dk_n + hk * p.dk_h + d] = (T)(there ? x * score_scale(p, n) : 0.f);
         ((T*)p.dv)[b * p.dv_b + (long)i * p.dv_n + hk * p.dv_h + d] = (T)(there ? y : 0.f);
     } else {
-        ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(there ? x * p.scale : 0.f);
+        ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(there ? x * score_scale(p, n) : 0.f);
     }
 }
 
@@ -1004,11 +1009,11 @@ struct Decode {
     int window, sinks;
     float scale;
 };
-// The heads that share a key head are the 32 MFMA columns.  Each wave stages its own 32 keys at a time (no barrier in
-// the loop) and keeps a softmax of its own; the four are joined through LDS, the splits through the workspace:
+// The heads that share a key head are the 32 MFMA columns.  Memory-bound: each of NW waves stages its own 32 keys at a time (no
+// barrier in the loop) and keeps a softmax of its own; the waves are joined through LDS, the splits through the workspace:
 // [B, Hq, splits] records of DH sums, a maximum (scaled, base 2) and a sum.
-template <typename T, int DH>
-__global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
+template <typename T, int DH, int NW>
+__global__ __launch_bounds__(NW * 64, 1) void slide_decode_kernel(Decode p) {
     using S = Shape<T, DH>;
     extern __shared__ __align__(16) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1029,7 +1034,7 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
     const int back = n - p.window > 0 ? n - p.window : 0;              // first key of the window
     const int f = p.sinks < back ? p.sinks : back;                     // first tokens in front of it
     const int tf = (f + 31) / 32, tw = (n - back + 31) / 32;
-    for (int t = split * 4 + wave; t < tf + tw; t += p.splits * 4) {
+    for (int t = split * NW + wave; t < tf + tw; t += p.splits * NW) {
         const int k0 = t < tf ? t * 32 : back + (t - tf) * 32;
         const int end = t < tf ? f : n;
         Fetch<T, DH> fk, fv;
@@ -1039,11 +1044,7 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
         fv.store(Vs, lane);
         wave_lds_fence();
         f32x16 s = product<DH>(Ks, 0, q, lane);
-        if (k0 + 32 > end) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (k0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) >= end) s[r] = -INFINITY;
-        }
+        if (k0 + 32 > end) hide(s, Span{0, end, 0}, k0 + 4 * (lane >> 5), false, -INFINITY);
         sm.step(s, sc, [&](float alpha) {
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
@@ -1052,7 +1053,7 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
         wave_lds_fence();
     }
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
-    join_waves<DH>(lds, acc, m, l, tid, [&](int c, int d, float x, float top, float sum) {
+    join_waves<DH, NW>(lds, acc, m, l, tid, [&](int c, int d, float x, float top, float sum) {
         if (g0 + c >= p.G) return;
         const long row = (long)b * p.Hq + hk * p.G + g0 + c;
         if (p.splits == 1) {
@@ -1065,18 +1066,35 @@ __global__ __launch_bounds__(256, 1) void slide_decode_kernel(Decode p) {
     });
 }
 template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_join_kernel(Decode p) {
+    constexpr int U = 8;                       // records in flight
     const long row = blockIdx.x;
     const int d = threadIdx.x;
     if (d >= DH) return;
     const float* rec = p.ws + row * p.splits * (DH + 2);
-    float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, rec[s * (DH + 2) + DH]);
-    float x = 0.f, sum = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float* r = rec + s * (DH + 2);
-        const float e = r[DH] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[DH] - top);
-        x += r[d] * e;
-        sum += r[DH + 1] * e;
+    float top = -INFINITY, x = 0.f, sum = 0.f;
+    for (int s0 = 0; s0 < p.splits; s0 += U) {
+        float m[U], l[U], v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float* r = rec + (long)least(s0 + u, p.splits - 1) * (DH + 2);
+            m[u] = s0 + u < p.splits ? r[DH] : -INFINITY;
+            l[u] = r[DH + 1];
+            v[u] = r[d];
+        }
+        float t = top;
+#pragma unroll
+        for (int u = 0; u < U; ++u) t = fmaxf(t, m[u]);
+        if (t == -INFINITY) continue;
+        const float a = __builtin_amdgcn_exp2f(top - t);
+        x *= a;
+        sum *= a;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float e = __builtin_amdgcn_exp2f(m[u] - t);
+            x += e > 0.f ? v[u] * e : 0.f;
+            sum += e > 0.f ? l[u] * e : 0.f;
+        }
+        top = t;
     }
     ((T*)p.o)[row * DH + d] = (T)(sum > 0.f ? x / sum : 0.f);
 }
@@ -1182,10 +1200,10 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipSt
     return 0;
 }
 template <typename T, int DH> int run_decode(const Decode& p, hipStream_t st) {
-    const int tiles = 4 * 2 * 32 * Shape<T, DH>::ROW, join = join_bytes<DH>();
-    const int bytes = tiles > join ? tiles : join;
-    if (int e = allow_lds(slide_decode_kernel<T, DH>, bytes)) return e;
-    hipLaunchKernelGGL((slide_decode_kernel<T, DH>), dim3(p.splits, p.Hkv * ((p.G + 31) / 32), p.B), dim3(256), bytes, st, p);
+    constexpr int NW = sizeof(T) == 2 ? 8 : 4;                         // what LDS holds of a head of 128
+    constexpr int tiles = NW * 2 * 32 * Shape<T, DH>::ROW, join = join_bytes<DH>(NW), bytes = tiles > join ? tiles : join;
+    if (int e = allow_lds(slide_decode_kernel<T, DH, NW>, bytes)) return e;
+    hipLaunchKernelGGL((slide_decode_kernel<T, DH, NW>), dim3(p.splits, p.Hkv * ((p.G + 31) / 32), p.B), dim3(NW * 64), bytes, st, p);
     VITK_CHECK_LAUNCH();
     if (p.splits > 1) {
         hipLaunchKernelGGL((slide_join_kernel<T, DH>), dim3((unsigned)((long)p.B * p.Hq)), dim3(DH < 64 ? 64 : DH), 0, st, p);
@@ -1218,6 +1236,7 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     p.k_b = a->k_b; p.k_n = a->k_n; p.k_h = a->k_h;
     p.v_b = a->v_b; p.v_n = a->v_n; p.v_h = a->v_h;
     reach(a, p.window, p.sinks);
+    p.single = (p.window == 1 && p.sinks == 0) || (p.window == 0 && p.sinks == 1 && a->causal);
     // a tile's rows are addressed with 32 bits from its first one on
     for (long ld : {a->q_n, a->k_n, a->v_n, backward ? a->do_n : 0L})
         if (ld < 0 || ld >= (1L << 23)) return VITK_ERR_SHAPE;
