@@ -162,3 +162,39 @@ def adamw8(p, g, mc, ms, vc, vs, t, coef, lr, betas, eps, wd, seed=0,
             code = torch.where(y < 0, -code, code)
         out += [code.to(torch.float8_e4m3fn), scale]
     return [p] + out
+
+
+# ----------------------------------------------------------------------------- a ViT with rotary positions and a window
+def vit_logits(params, images, patch, layers, heads, grid, window, sinks, pairs, base):
+    """Logits of a pre-LN ViT (class token first) in the type of ``params`` (a state dict by the model's names)."""
+    P = {k.replace("transformer.", "", 1) if k.startswith("transformer.") else k: v for k, v in params.items()}
+    F = torch.nn.functional
+
+    def norm(x, name):
+        return F.layer_norm(x, x.shape[-1:], P[name + ".weight"], P[name + ".bias"], 1e-6)
+
+    def linear(x, name):
+        return F.linear(x, P[name + ".weight"], P[name + ".bias"])
+
+    x = F.conv2d(images, P["embeddings.patch_embeddings.weight"], P["embeddings.patch_embeddings.bias"], stride=patch)
+    B, D = x.shape[:2]
+    x = torch.cat([P["embeddings.cls_token"].expand(B, -1, -1), x.flatten(2).transpose(1, 2)], 1) + P["embeddings.position_embeddings"]
+    N, dh = x.shape[1], D // heads
+    at = torch.tensor([[0, 0]] + [[r, c] for r in range(grid[0]) for c in range(grid[1])], dtype=x.dtype)
+    angle = torch.cat([at[:, a:a + 1] * base ** (-torch.arange(n, dtype=x.dtype) / n) for a, n in enumerate(pairs)], 1)[:, None]
+    cos, sin, S = angle.cos(), angle.sin(), sum(pairs)
+
+    def turned(t):
+        a, b = t[..., :S], t[..., S:2 * S]
+        return torch.cat([a * cos - b * sin, b * cos + a * sin, t[..., 2 * S:]], -1)
+
+    seen = visible(N, N, window, sinks, False, N)
+    for i in range(layers):
+        L = f"encoder.layer.{i}."
+        h = norm(x, L + "attention_norm")
+        q, k, v = (linear(h, L + "attn." + n).view(B, N, heads, dh) for n in ("query", "key", "value"))
+        q, k, v = (t.transpose(1, 2) for t in (turned(q), turned(k), v))
+        p = torch.softmax((q @ k.transpose(-1, -2) / math.sqrt(dh)).masked_fill(~seen, -math.inf), -1)
+        x = x + linear((p @ v).transpose(1, 2).reshape(B, N, D), L + "attn.out")
+        x = x + linear(F.gelu(linear(norm(x, L + "ffn_norm"), L + "ffn.fc1")), L + "ffn.fc2")
+    return linear(norm(x, "encoder.encoder_norm")[:, 0], "head")

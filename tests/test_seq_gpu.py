@@ -587,3 +587,53 @@ def test_adamw_loads_torch_state_and_refuses():
         held += 1
         with pytest.raises(RuntimeError, match="captured"):
             opt.step()
+
+
+# ----------------------------------------------------------------------------- together
+@pytest.mark.parametrize("bits", [32, 8])
+def test_vit_with_rotary_positions_and_a_window_trains_with_adamw(bits):
+    """Positions, attention and update in one model, fp32 compute: loss and every gradient within 1e-5 of their scale
+    (the framework's fp32 bar), every updated parameter within the step's own rounding of the gradients it was given."""
+    import vitk
+    from models.config import get_tiny_config
+    from models.ViT.modeling import VisionTransformer
+    from utils.optim import FusedAdamW
+    torch.manual_seed(3)
+    cfg = get_tiny_config()
+    cfg.transformer.update(attention_window=4, attention_sinks=1, rope_pairs=(12, 20), rope_base=100.0)
+    kw = dict(lr=1e-3, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.05)
+    with vitk.compute_dtype(FP):
+        model = VisionTransformer(cfg, (48, 80), num_classes=7).to(DEV).train()
+        assert not any("positions" in k and "embeddings" not in k for k in model.state_dict())
+        with torch.no_grad():
+            for p in model.parameters():
+                p.add_(0.05 * torch.randn_like(p))
+        opt = FusedAdamW(model.parameters(), state_bits=bits, **kw)
+        for step in (1, 2):
+            images, labels = _rand(3, 3, 48, 80, seed=step), torch.tensor([1, 5, 2])
+            loss = model(images.to(DEV), labels.to(DEV))
+            loss.backward()
+            ref = {k: v.detach().double().cpu().requires_grad_(True) for k, v in model.named_parameters()}
+            logits = SO.vit_logits(ref, images.double(), 16, 2, 2, (3, 5), 4, 1, (12, 20), 100.0)
+            want = torch.nn.functional.cross_entropy(logits, labels)
+            want.backward()
+            assert abs(float(loss) - float(want)) <= 1e-5 * abs(float(want))
+            for name, p in model.named_parameters():
+                g, r = p.grad.double().cpu(), ref[name].grad
+                scale = r.abs().max()
+                if name.endswith("attn.key.bias"):     # zero but for rounding: judged by the query bias's
+                    scale = torch.maximum(scale, ref[name.replace("key", "query")].grad.abs().max())
+                assert (g - r).abs().max() <= 1e-5 * scale + 1e-7, name
+            before = {k: (p.detach().double().cpu(), p.grad.double().cpu(),
+                          *((opt.state[p][n].double().cpu() for n in ("exp_avg", "exp_avg_sq")) if step > 1 and bits == 32 else
+                            (torch.zeros_like(p, dtype=torch.float64).cpu(),) * 2)) for k, p in model.named_parameters()}
+            norm = opt.step(max_grad_norm=1.0)
+            coef = float(torch.tensor(min(1.0, 1.0 / (float(norm.double()) + 1e-6)), dtype=FP))
+            if step == 1 or bits == 32:                # in 8 bits the second step starts from rounded moments
+                for name, p in model.named_parameters():
+                    # the norm was rounded to 32 bits on its way here: one unit of the factor more
+                    (val, e), _, _ = SO.adamw(*before[name], step, coef, kw["lr"], kw["betas"], kw["eps"], kw["weight_decay"])
+                    _hold(name, p, val, e + 4 * SO.U * kw["lr"] * 10)
+            opt.zero_grad()
+    with pytest.raises(ValueError):
+        VisionTransformer(cfg, (48, 80), num_classes=7, vis=True)

@@ -90,6 +90,16 @@ class Attention(nn.Module):
         self.attn_dropout = nn.Dropout(rate)
         self.proj_dropout = nn.Dropout(rate)
         self.softmax = nn.Softmax(dim=-1)
+        # Not in the reference, for many tokens: `attention_window` (tokens see those nearer than it, and the first
+        # `attention_sinks`, by default the class token, see and are seen by all), and `rope_pairs` (rotary positions on the
+        # token grid: element pairs of a head for its rows and its columns; Transformer fills in the positions).
+        t = config.transformer
+        self.window, self.sinks = t.get("attention_window"), t.get("attention_sinks", 1)
+        self.rope_pairs, self.rope_base = t.get("rope_pairs"), t.get("rope_base", 10000.0)
+        self.register_buffer("positions", None, persistent=False)
+        self.sliding = self.window is not None or self.rope_pairs is not None
+        if self.sliding and (vis or rate > 0):
+            raise ValueError("attention_window / rope_pairs: no attention maps (vis) and no attention dropout")
 
     def forward(self, hidden_states, residual=None):
         """hidden_states [B,N,D] -> (attention_output [B,N,D], probs [B,H,N,N] or None).
@@ -101,8 +111,13 @@ class Attention(nn.Module):
         qkv = ops.linear(x.reshape(B * N, D),
                          (self.query.weight, self.key.weight, self.value.weight),
                          (self.query.bias, self.key.bias, self.value.bias))
-        ctx, lse = ops.attention(qkv, B, N, H, dropout_p=self.attn_dropout.p if self.training else 0.0)
-        weights = ops.attention_probs(qkv.detach(), lse, B, N, H) if self.vis else None
+        weights = None
+        if self.sliding:
+            ctx = ops.sliding_attention_qkv(qkv, B, N, H, self.window, sinks=self.sinks, positions=self.positions,
+                                            pairs=self.rope_pairs, base=self.rope_base)
+        else:
+            ctx, lse = ops.attention(qkv, B, N, H, dropout_p=self.attn_dropout.p if self.training else 0.0)
+            weights = ops.attention_probs(qkv.detach(), lse, B, N, H) if self.vis else None
         p = self.proj_dropout.p if self.training else 0.0
         out = ops.linear(ctx, (self.out.weight,), (self.out.bias,), residual=residual, dropout_p=p)
         return out.view(B, N, D), weights
@@ -257,6 +272,13 @@ class Transformer(nn.Module):
         super().__init__()
         self.embeddings = Embeddings(config, img_size=img_size)
         self.encoder = Encoder(config, vis)
+        if config.transformer.get("rope_pairs") is not None:
+            # the class token stays at the origin, patches are at their row and column
+            step = 16 if self.embeddings.hybrid else self.embeddings.patch_embeddings.kernel_size
+            grid = [n // s for n, s in zip(_pair(img_size), _pair(step))]
+            positions = ops.grid_positions(grid, lead=1, device="cpu")
+            for layer in self.encoder.layer:
+                layer.attn.positions = positions
 
     def forward(self, input_ids):
         return self.encoder(self.embeddings(input_ids))
