@@ -82,16 +82,38 @@ __device__ __forceinline__ void hide(f32x16& s, const Span& v, int x0, bool firs
             if ((unsigned)(d + 8 * (r >> 2) + (r & 3)) >= (unsigned)v.len) s[r] = with;
     }
 }
-// Of the rectangle [ia, ib] x [ja, jb]: 0 nothing is visible, 2 everything is, 1 look at each pair.
-template <bool CAUSAL> __device__ __forceinline__ int coverage(int ia, int ib, int ja, int jb, int n, int w, int f) {
-    if (ia >= n || ja >= n) return 0;
-    if constexpr (CAUSAL) {
-        if (ja > ib || (ia - jb >= w && ja >= f)) return 0;
-        return ib < n && jb < n && jb <= ia && (ib - ja < w || jb < f) ? 2 : 1;
-    } else {
-        if ((ia - jb >= w || ja - ib >= w) && ja >= f && ia >= f) return 0;
-        return ib < n && jb < n && ((ib - ja < w && jb - ia < w) || jb < f || ib < f) ? 2 : 1;
+// What 32 rows see of 32 rows [x, x + 31] of the other axis: 0 nothing, 2 everything, 1 some pairs.  Rows [lo, hi] are seen by
+// some of them and rows [flo, fhi] by all; of the rows before f some are seen, those before ff by all.  Four comparisons of
+// scalars a tile: what the general test of a rectangle costs showed in the time of the loops.
+struct Cover {
+    int lo, hi, flo, fhi, f, ff;
+    __device__ __forceinline__ int of(int x) const {
+        if (x >= f && (x + 31 < lo || x > hi)) return 0;
+        return (x >= flo && x + 31 <= fhi) || x + 31 < ff ? 2 : 1;
     }
+};
+__device__ __forceinline__ Cover only_some(Cover c, bool some) {      // nothing is seen by all
+    if (some) { c.flo = c.fhi + 1; c.ff = 0; }
+    return c;
+}
+// Of keys, by queries [a, a + 31]; no key is seen by a query behind the sequence.
+template <bool CAUSAL> __device__ __forceinline__ Cover keys_by(int a, int n, int w, int f) {
+    if (a >= n) return Cover{n, -1, n, -1, 0, 0};
+    const int z = a + 31, r = w > 0 ? w - 1 : -1;
+    f = least(f, n);
+    if (CAUSAL)
+        return only_some(Cover{a - r, w > 0 ? least(z, n - 1) : -1, z - r, w > 0 ? least(a, n - 1) : -1, least(f, z + 1), least(f, a + 1)}, z >= n);
+    if (a < f) return only_some(Cover{0, n - 1, z < f ? 0 : z - r, z < f ? n - 1 : least(a + r, n - 1), f, f}, z >= n);
+    return only_some(Cover{a - r, least(z + r, n - 1), z - r, least(a + r, n - 1), f, f}, z >= n);
+}
+// Of queries, by keys [a, a + 31].
+template <bool CAUSAL> __device__ __forceinline__ Cover queries_by(int a, int n, int w, int f) {
+    if (a >= n) return Cover{n, -1, n, -1, 0, 0};
+    const int z = a + 31, r = w > 0 ? w - 1 : -1;
+    f = least(f, n);
+    if (CAUSAL) return only_some(Cover{a, a < f ? n - 1 : least(z + r, n - 1), z, z < f ? n - 1 : least(a + r, n - 1), 0, 0}, z >= n);
+    if (a < f) return only_some(Cover{0, n - 1, z < f ? 0 : z - r, z < f ? n - 1 : least(a + r, n - 1), f, f}, z >= n);
+    return only_some(Cover{a - r, least(z + r, n - 1), z - r, least(a + r, n - 1), f, f}, z >= n);
 }
 // The tiles of `T` rows of the other axis that rows [a, b] of this one can touch: [0, first) and [lo, hi).
 struct Tiles { int first, lo, hi; __device__ __forceinline__ int count() const { return first + (hi > lo ? hi - lo : 0); }
@@ -262,9 +284,15 @@ template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char
 //
 // Straight into LDS, 16 bytes a lane in the order of the lanes: each lane fetches the chunk that belongs at its place.  By all
 // four waves (`voff`: where this thread's chunks lie from the tile's first row on.
-// (s_nop: the base may come from a vector instruction, which the compiler does not see either.)
+// A base for them: moved by a scalar instruction, which waits for a vector instruction that may have made it, as the loads in
+// assembly would not.
+template <typename X> __device__ __forceinline__ const X* settled(const X* p) {
+    const X* q;
+    asm volatile("s_mov_b64 %0, %1" : "=s"(q) : "s"(p));
+    return q;
+}
 __device__ __forceinline__ void dma16(const void* base, int off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 }
 __device__ __forceinline__ void dma4(const void* from, unsigned lds) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(lds) : "memory");
@@ -286,7 +314,7 @@ template <typename T, int DH, int NT = 256> struct Stage {
         for (int i = 0; i < PARTS; ++i) voff[i] = offset(i, tid, S::KT);
     }
     __device__ __forceinline__ void start(char* tile, const T* base, int r0, int n, int tid) const {
-        const T* from = base + (long)r0 * ld;
+        const T* from = settled(base + (long)r0 * ld);
         const unsigned to = __builtin_amdgcn_readfirstlane(lds_addr(tile) + (tid & ~63) * 16);
         if (r0 + S::KT <= n) {
 #pragma unroll
@@ -476,7 +504,7 @@ __device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T*
 template <typename T, int DH> __device__ __forceinline__ void start_wave(char* tile, const T* base, long ld, int r0, int n, int lane) {
     using S = Shape<T, DH>;
     const unsigned to = __builtin_amdgcn_readfirstlane(lds_addr(tile));
-    const T* from = base + r0 * ld;
+    const T* from = settled(base + r0 * ld);
 #pragma unroll
     for (int i = 0; i < 32 * S::CHUNKS / 64; ++i) {
         const int pl = i * 64 + lane, r = pl / S::CHUNKS, ch = (pl % S::CHUNKS) ^ S::mix(r);
@@ -508,6 +536,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
     const bool elsewhere = !CAUSAL && qa < p.rows && !p.chunks;          // an item of its own does these rows
     const float sc = p.scale * LOG2E;
     const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
+    const Cover cover = keys_by<CAUSAL>(qa, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
     Softmax sm;
     const auto rescale = [&](float alpha) {
@@ -519,7 +548,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
-            const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
+            const int cov = cover.of(ka);
             if (cov == 0 || elsewhere) continue;
             f32x16 s = product<DH>(Ks, sub, q, lane);
             if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, -INFINITY);
@@ -558,6 +587,7 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
     Kept<T, DH> q;
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, mine);
     const float sc = p.scale * LOG2E;
+    const Cover cover = keys_by<false>(qa, n, p.window, p.sinks);
     const Span sp = all ? keys_of<false>(qi, n, p.window, p.sinks) : Span{0, mine ? n : 0, 0};
     f32x16 acc[DH / 32] = {};
     Softmax sm;
@@ -565,7 +595,7 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     const int from = all ? 0 : (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += chunks * 4 * 32) {
-        if (all && coverage<false>(qa, qa + 31, k0, k0 + 31, n, p.window, p.sinks) == 0) continue;
+        if (all && cover.of(k0) == 0) continue;
         start_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
         start_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
         dma_wait();
@@ -688,13 +718,14 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     const bool elsewhere = !CAUSAL && qa < p.rows && !p.chunks;
     const float sc = p.scale * LOG2E;
     const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
+    const Cover cover = keys_by<CAUSAL>(qa, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&](const char* Ks, const char* Vs, int k0) {
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
-            const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
+            const int cov = cover.of(ka);
             if (cov == 0 || elsewhere) continue;
             f32x16 s = product<DH>(Ks, sub, q, lane);
             const f32x16 dp = product<DH>(Vs, sub, d_o, lane);
@@ -728,13 +759,14 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     const float lse = mine ? p.lse[st] : INFINITY;                       // not mine: probabilities of 0
     const float delta = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, mine);
     const float sc = p.scale * LOG2E;
+    const Cover cover = keys_by<false>(qa, n, p.window, p.sinks);
     const Span sp = all ? keys_of<false>(qi, n, p.window, p.sinks) : Span{0, n, 0};
     f32x16 acc[DH / 32] = {};
     const int q0 = qa / TQ * TQ;
     const Tiles tl = key_tiles<false>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
     const int from = all ? 0 : (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
     for (int k0 = from + (chunk * 4 + wave) * 32; k0 < n && qa < n; k0 += chunks * 4 * 32) {
-        if (all && coverage<false>(qa, qa + 31, k0, k0 + 31, n, p.window, p.sinks) == 0) continue;
+        if (all && cover.of(k0) == 0) continue;
         start_wave<T, DH>(Ks, K, p.k_n, k0, n, lane);
         start_wave<T, DH>(Vs, V, p.v_n, k0, n, lane);
         dma_wait();
@@ -839,6 +871,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
     const int per = tl.count(), cnt = per * p.G;
     const Span sp = queries_of<CAUSAL>(kj, n, p.window, p.sinks);
+    const Cover cover = queries_by<CAUSAL>(ka, n, p.window, p.sinks);
     const bool elsewhere = ka < p.rows && !p.chunks;
     const Stage<T, DH, L::NT> fq(p.q_n, tid), fo(p.do_n, tid);
     int next_g = 0, next_t = 0;
@@ -865,7 +898,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
         for (int sub = 0; sub < S::KT; sub += 32) {
             if (L::PARTS == 2 && (((S::KT > 32 ? sub / 32 : t) + part) & 1)) continue;
             const int qa = q0 + sub;
-            const int cov = coverage<CAUSAL>(qa, qa + 31, ka, ka + 31, n, p.window, p.sinks);
+            const int cov = cover.of(qa);
             if (cov == 0 || elsewhere) continue;
             const int x0 = qa + 4 * (lane >> 5);
             const bool first = !CAUSAL && qa < p.sinks;
@@ -930,11 +963,12 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     const int k0 = ka / (32 * KG) * (32 * KG);
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
     const int from = all ? 0 : (tl.hi > tl.first ? tl.hi : tl.first) * S::KT;
+    const Cover cover = queries_by<CAUSAL>(ka, n, p.window, p.sinks);
     const Span sp = all ? queries_of<CAUSAL>(kj, n, p.window, p.sinks) : Span{0, mine ? n : 0, 0};
     const int per = ka < n && from < n ? (n - from + 31) / 32 : 0;
     for (int t = chunk * NW + wave; t < per * p.G; t += chunks * NW) {
         const int h = hk * p.G + t / per, q0 = from + t % per * 32;
-        if (all && coverage<CAUSAL>(q0, q0 + 31, ka, ka + 31, n, p.window, p.sinks) == 0) continue;
+        if (all && cover.of(q0) == 0) continue;
         const long st = ((long)b * p.Hq + h) * p.N + q0;
         start_wave<T, DH>(Qs, (const T*)p.q + b * p.q_b + h * p.q_h, p.q_n, q0, n, lane);
         start_wave<T, DH>(Os, (const T*)p.d_o + b * p.do_b + h * p.do_h, p.do_n, q0, n, lane);
