@@ -631,21 +631,44 @@ __global__ __launch_bounds__(256, 2) void slide_fwd_kernel(Slide p) {
         if (it.far) return fwd_far<T, DH>(p, lds, it.x, it.h, it.b, n);
     fwd_band<T, DH, CAUSAL>(p, lds, it.x * TQ, it.h, it.b, n);
 }
+// One softmax from `count` records of `width` numbers, as element d sees it: several records are in flight at a time.
+template <int DH> struct Joined { float x, top, sum; };
+template <int DH> __device__ __forceinline__ Joined<DH> join_records(const float* rec, int count, int width, int d) {
+    constexpr int U = 8;
+    Joined<DH> j{0.f, -INFINITY, 0.f};
+    for (int s0 = 0; s0 < count; s0 += U) {
+        float m[U], l[U], v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float* r = rec + (long)least(s0 + u, count - 1) * width;
+            m[u] = s0 + u < count ? r[DH] : -INFINITY;
+            l[u] = r[DH + 1];
+            v[u] = r[d];
+        }
+        float t = j.top;
+#pragma unroll
+        for (int u = 0; u < U; ++u) t = fmaxf(t, m[u]);
+        if (t == -INFINITY) continue;
+        const float a = __builtin_amdgcn_exp2f(j.top - t);
+        j.x *= a;
+        j.sum *= a;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float e = __builtin_amdgcn_exp2f(m[u] - t);
+            j.x += e > 0.f ? v[u] * e : 0.f;
+            j.sum += e > 0.f ? l[u] * e : 0.f;
+        }
+        j.top = t;
+    }
+    return j;
+}
 // The records of the first rows become outputs.
 template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_fwd_join_kernel(Slide p) {
     const int i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, d = threadIdx.x;
     if (d >= DH) return;
     const float* rec = p.ws + (((long)b * p.Hq + h) * p.rows + i) * (p.chunks + 1) * (DH + 4);
-    float top = -INFINITY;
-    for (int s = 0; s <= p.chunks; ++s) top = fmaxf(top, rec[s * (DH + 4) + DH]);
-    float x = 0.f, sum = 0.f;
-    for (int s = 0; s <= p.chunks; ++s) {
-        const float* r = rec + s * (DH + 4);
-        const float e = r[DH] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(r[DH] - top);
-        x += r[d] * e;
-        sum += r[DH + 1] * e;
-    }
-    write_row<T, DH>(p, b, h, i, d, x, top, sum);
+    const Joined<DH> j = join_records<DH>(rec, p.chunks + 1, DH + 4, d);
+    write_row<T, DH>(p, b, h, i, d, j.x, j.top, j.sum);
 }
 
 // ----------------------------------------------------------------------------- backward
@@ -1100,37 +1123,11 @@ __global__ __launch_bounds__(NW * 64, 1) void slide_decode_kernel(Decode p) {
     });
 }
 template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) void slide_join_kernel(Decode p) {
-    constexpr int U = 8;                       // records in flight
     const long row = blockIdx.x;
     const int d = threadIdx.x;
     if (d >= DH) return;
-    const float* rec = p.ws + row * p.splits * (DH + 2);
-    float top = -INFINITY, x = 0.f, sum = 0.f;
-    for (int s0 = 0; s0 < p.splits; s0 += U) {
-        float m[U], l[U], v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float* r = rec + (long)least(s0 + u, p.splits - 1) * (DH + 2);
-            m[u] = s0 + u < p.splits ? r[DH] : -INFINITY;
-            l[u] = r[DH + 1];
-            v[u] = r[d];
-        }
-        float t = top;
-#pragma unroll
-        for (int u = 0; u < U; ++u) t = fmaxf(t, m[u]);
-        if (t == -INFINITY) continue;
-        const float a = __builtin_amdgcn_exp2f(top - t);
-        x *= a;
-        sum *= a;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float e = __builtin_amdgcn_exp2f(m[u] - t);
-            x += e > 0.f ? v[u] * e : 0.f;
-            sum += e > 0.f ? l[u] * e : 0.f;
-        }
-        top = t;
-    }
-    ((T*)p.o)[row * DH + d] = (T)(sum > 0.f ? x / sum : 0.f);
+    const Joined<DH> j = join_records<DH>(p.ws + row * p.splits * (DH + 2), p.splits, DH + 2, d);
+    ((T*)p.o)[row * DH + d] = (T)(j.sum > 0.f ? j.x / j.sum : 0.f);
 }
 
 // ----------------------------------------------------------------------------- host side
@@ -1140,16 +1137,20 @@ template <typename K> int allow_lds(K kernel, int bytes) {
 }
 constexpr int dkv_waves(bool bf16, int dh) { return bf16 && dh == 128 ? 8 : 4; }
 // Items of the first tokens: rows (a multiple of 32; 0: none needed), chunks of far items for each 32 of them, floats of
-// workspace for their records.  One item for all (no records, no second launch) while that is at most 24 turns of its waves,
-// of a microsecond or so each (FIGURES); else a chunk gives each of its waves about 4 far tiles, and fewer chunks do
-// where there are items enough without them.
+// workspace for their records.  One item for all (no records, no second launch) while it ends before the bands do, which
+// its turns, of a microsecond or so each, decide: up to 24 of its waves where there are four bands a CU and more (2305 tokens,
+// 8 sequences of 12 heads: forward 53 us, with chunks 63; backward 163, with chunks 172), up to 12 with fewer bands (577
+// tokens, 6 of 8 heads: backward 34 us, with chunks 37; 2305 tokens, one of 12 heads: 55 us, with chunks 38; 16384 causal
+// tokens, 2 key heads of 4 queries each: 663 us, with chunks 286).  Else a chunk gives each of its waves about 4 far tiles (that
+// backward: 2 tiles 299 us, 4 286, 8 291), and fewer chunks do where there are items enough without them.
 struct Records { int rows, chunks; long floats; };
 Records records_of(int B, int N, int heads, int G, int width, int window, int sinks, int waves) {
     Records r{0, 0, 0};
     if (sinks <= 0 || window >= N) return r;
     r.rows = (sinks + 31) / 32 * 32;
     const long tiles = (long)G * ((N + 31) / 32);
-    if (tiles <= 24 * waves) return r;
+    const long bands = (long)B * heads * ((N + TQ - 1) / TQ);
+    if (tiles <= (bands >= 1024 ? 24 : 12) * waves) return r;
     const long items = (long)B * heads * (r.rows / 32), most = (2048 + items - 1) / items;
     r.chunks = (int)((tiles + 4 * waves - 1) / (4 * waves));
     if (r.chunks > most) r.chunks = (int)most;
@@ -1258,7 +1259,7 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     if (!a || !a->q || !a->k || !a->v) return VITK_ERR_NULL;
     if (dtype != VITK_BF16 && dtype != VITK_F32) return VITK_ERR_DTYPE;
     if (a->dh != 32 && a->dh != 64 && a->dh != 128) return VITK_ERR_UNSUPPORTED;
-    if (a->B <= 0 || a->N <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->B > 65535 || a->Hq > 65535) return VITK_ERR_SHAPE;
+    if (a->B <= 0 || a->N <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->B > 65535 || a->Hq > 32767) return VITK_ERR_SHAPE;
     if (a->N > (1 << 30) || a->window < 0 || a->sinks < 0 || !(a->scale > 0.f)) return VITK_ERR_SHAPE;
     const int e = dtype == VITK_BF16 ? 2 : 4;
     if (!aligned(a->q, e, {a->q_b, a->q_n, a->q_h}) || !aligned(a->k, e, {a->k_b, a->k_n, a->k_h}) ||
