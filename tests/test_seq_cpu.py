@@ -24,7 +24,7 @@ DECODE = dict(q=_t(2, 4, 64), k_cache=_t(2, 9, 2, 64), v_cache=_t(2, 9, 2, 64), 
     dict(positions=torch.zeros(4, 2)), dict(positions=torch.zeros(5, 3)), dict(positions=torch.zeros(3, 5, 2)),
     dict(positions=torch.zeros(5, 2, dtype=torch.float16)), dict(positions=torch.zeros(5, 2, requires_grad=True)),
     dict(base=0.0), dict(base=float("inf")), dict(out=_t(2, 5, 3, 32)), dict(out=_t(2, 5, 3, 64, dtype=torch.float32)),
-    dict(out=_t(2, 5, 64, 3).transpose(2, 3)),
+    dict(out=_t(2, 5, 64, 3).transpose(2, 3)), dict(out=_t(2, 5, 1, 64).expand(2, 5, 3, 64)),
 ])
 def test_axial_rope_refuses(change):
     with pytest.raises(VitkError, match="axial_rope|unsupported dtype" if change else "GPU only"):
@@ -134,6 +134,38 @@ def test_adamw_refuses_what_it_cannot_update():
         opt.step(closure=lambda: 0)
     with pytest.raises(ValueError):
         opt.step(max_grad_norm=-1.0)
+
+
+def test_adamw_refuses_states_of_other_parameters():
+    from utils.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.zeros(300))
+    moments = {name: torch.zeros(300) for name in ("exp_avg", "exp_avg_sq")}
+    groups = torch.optim.AdamW([p]).state_dict()["param_groups"]
+
+    def load(bits=32, groups=groups, **change):
+        st = {k: v for k, v in {"step": 1, **moments, **change}.items() if v is not None}
+        FusedAdamW([p], state_bits=bits).load_state_dict(dict(state={0: st}, param_groups=groups))
+
+    load()
+    scales = dict(exp_avg_scale=torch.zeros(2), exp_avg_sq_scale=torch.zeros(2))
+    load(8, **scales)
+    for bits, change in ((32, dict(exp_avg=torch.zeros(299))), (32, dict(exp_avg_sq=torch.zeros(1, 300))), (32, dict(exp_avg=None)),
+                         (8, dict(scales, exp_avg_scale=torch.zeros(1))), (8, dict(scales, exp_avg_sq_scale=None)), (32, scales), (8, {})):
+        with pytest.raises(ValueError):
+            load(bits, **change)
+    for name in ("amsgrad", "maximize"):
+        with pytest.raises(ValueError):
+            load(groups=[dict(groups[0], **{name: True})])
+
+
+def test_adamw_refused_step_leaves_no_states():
+    from utils.optim import FusedAdamW
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = FusedAdamW([p])
+    p.grad = torch.zeros(3)
+    with pytest.raises(ValueError):
+        opt.step()
+    assert not opt.state[p]
 
 
 def test_grid_positions():

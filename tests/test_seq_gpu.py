@@ -193,6 +193,40 @@ def test_strides_orders_and_repeats_give_the_same_bits():
         got = _grads(q, k, v, d_o, **kw)
     torch.cuda.current_stream().wait_stream(side)
     same(got, "another stream")
+    one = [t[:1].contiguous() for t in (q, k, v, d_o)]
+    want = _grads(*one, **kw)
+    same(_grads(*[t.as_strided(t.shape, (7, *t.stride()[1:])) for t in one], **kw), "a batch of one, any stride")
+
+
+def test_two_captured_passes_replayed_at_once():
+    """Each graph holds the records of its first tokens in memory of its own: replayed side by side on two streams, with
+    other work of the same kind in between, both give what they give alone."""
+    from vitk import ops
+    first = _case(BF, B=1, N=3000)
+    cases = [first, tuple(t.flip(1) for t in first)]
+    kw = dict(window=40, sinks=3)
+    graphs, outs, want = [], [], []
+    with torch.no_grad():
+        for q, k, v, _ in cases:
+            want.append(ops.sliding_attention(q, k, v, **kw))
+        torch.cuda.synchronize()
+        for q, k, v, _ in cases:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs.append(ops.sliding_attention(q, k, v, **kw))
+            graphs.append(g)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for turn in range(4):
+            for o in outs:
+                o.zero_()
+            torch.cuda.synchronize()
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+            ops.sliding_attention(*cases[0][:3], **kw)
+            torch.cuda.synchronize()
+            for o, w in zip(outs, want):
+                assert torch.equal(o, w), turn
 
 
 def test_some_gradients_only_and_shared_inputs():
@@ -571,6 +605,10 @@ def test_adamw_loads_torch_state_and_refuses():
     ref.step()
     opt.step()
     _hold("p", q, p.detach().double().cpu(), 16 * SO.U * (p.detach().double().cpu().abs() + 1e-2))
+    with pytest.raises(ValueError, match="moments"):          # another tensor behind the same parameter
+        q.data = torch.zeros(101, device=DEV)
+        q.grad = torch.zeros(101, device=DEV)
+        opt.step()
     for bad in (torch.zeros(4, device=DEV, dtype=BF), torch.zeros(4, 6, device=DEV).t()):
         x = torch.nn.Parameter(bad)
         x.grad = torch.zeros_like(x)

@@ -165,6 +165,14 @@ class FusedAdamW(torch.optim.Optimizer):
         held = [s for s in state_dict["state"].values() if s]
         if any(("exp_avg_scale" in s) != (self.state_bits == 8) for s in held):
             raise ValueError(f"the state dict's moments are not in {self.state_bits} bits")
+        if any(g.get("amsgrad") or g.get("maximize") for g in state_dict["param_groups"]):
+            raise ValueError("FusedAdamW has no amsgrad and no maximize")
+        # (super() pairs groups and parameters in this order, and refuses others)
+        ours = [p for g in self.param_groups for p in g["params"]]
+        for key, p in zip([k for g in state_dict["param_groups"] for k in g["params"]], ours):
+            st = state_dict["state"].get(key)
+            if st and not self._fits(p, st):
+                raise ValueError(f"the state dict's moments do not belong to a parameter of shape {tuple(p.shape)}")
         super().load_state_dict(state_dict)
         for p, st in self.state.items():
             if st:
@@ -174,6 +182,13 @@ class FusedAdamW(torch.optim.Optimizer):
                     if name != "step":      # copies: the state dict's tensors may be another optimizer's
                         st[name] = torch.empty(value.shape, dtype=torch.float32 if name.endswith("_scale") else kind,
                                                device=p.device).copy_(value)
+
+    def _fits(self, p, st):
+        """Whether these states have the sizes that the kernel takes for granted."""
+        if not all(name in st and st[name].shape == p.shape for name in ("exp_avg", "exp_avg_sq")):
+            return False
+        return self.state_bits != 8 or all(name in st and st[name].numel() == -(-p.numel() // _SCALE_BLOCK)
+                                           for name in ("exp_avg_scale", "exp_avg_sq_scale"))
 
     def _begin(self, p, st):
         """Empty states of a parameter: the first step takes them as zeros."""
@@ -206,6 +221,9 @@ class FusedAdamW(torch.optim.Optimizer):
     def _upload(self, host, blocks, dev):
         """The table and, behind it, the entry of each block, on the device; uploads go through a ring of pinned buffers,
         each guarded by an event, so the host never waits for the step it has just enqueued."""
+        if self._dev is not None and self._dev.device != dev:          # the model has moved
+            self._dev = self._last = self._slots = None
+            self._ring = []
         if self._last is not None and self._last.shape == host.shape and np.array_equal(self._last, host):
             return
         entry_of = np.repeat(np.arange(len(host), dtype=np.int32), np.diff(blocks, prepend=0))
@@ -234,31 +252,36 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError("FusedAdamW does not re-evaluate the model")
         if max_grad_norm is not None and not max_grad_norm >= 0.0:
             raise ValueError("max_grad_norm must be non-negative")
-        # one launch for the tensors of a group that have taken the same number of steps
         state, f32 = self.state, torch.float32
-        all_ps, all_grads, all_sts, spans = [], [], [], []
-        for group in self.param_groups:
-            ps = [p for p in group["params"] if p.grad is not None and p.numel()]
+        groups = [[p for p in group["params"] if p.grad is not None and p.numel()] for group in self.param_groups]
+        first = next((ps[0] for ps in groups if ps), None)
+        if first is None:
+            return None
+        dev, at = first.device, first.get_device()
+        for ps in groups:
+            grads = [p.grad for p in ps]
+            if not (dev.type == "cuda" and all(p.dtype is f32 and p.get_device() == at and p.is_contiguous() for p in ps)
+                    and all(g.dtype is f32 and g.get_device() == at and not g.is_sparse and g.is_contiguous() for g in grads)):
+                raise ValueError("FusedAdamW needs contiguous fp32 parameters and gradients on one GPU")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW.step counts steps on the host and is not captured into a graph")
+        # one launch for the tensors of a group that have taken the same number of steps
+        all_ps, all_sts, spans = [], [], []
+        for group, ps in zip(self.param_groups, groups):
             sts = [state[p] for p in ps]
             for p, st in zip(ps, sts):
                 if not st:
                     self._begin(p, st)
             steps = [st["step"] for st in sts]
             for t in dict.fromkeys(steps):
-                at = [i for i, x in enumerate(steps) if x == t] if steps.count(t) != len(steps) else range(len(steps))
-                spans.append((group, t, len(all_ps), len(at)))
-                all_ps += [ps[i] for i in at]
-                all_sts += [sts[i] for i in at]
-        if not all_ps:
-            return None
-        dev = all_ps[0].device
+                of_t = [i for i, x in enumerate(steps) if x == t] if steps.count(t) != len(steps) else range(len(steps))
+                spans.append((group, t, len(all_ps), len(of_t)))
+                all_ps += [ps[i] for i in of_t]
+                all_sts += [sts[i] for i in of_t]
+        # a parameter may have got another tensor, or moved, since its states were made
+        if not all(st["exp_avg"].get_device() == at and st["exp_avg"].shape == p.shape for p, st in zip(all_ps, all_sts)):
+            raise ValueError("a parameter's shape or device is not that of its moments")
         all_grads = [p.grad for p in all_ps]
-        at = all_ps[0].get_device()
-        if not (dev.type == "cuda" and all(p.dtype is f32 and p.get_device() == at and p.is_contiguous() for p in all_ps)
-                and all(g.dtype is f32 and g.get_device() == at and not g.is_sparse and g.is_contiguous() for g in all_grads)):
-            raise ValueError("FusedAdamW needs contiguous fp32 parameters and gradients on one GPU")
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("FusedAdamW.step counts steps on the host and is not captured into a graph")
         host, blocks = self._table(all_ps, all_grads, all_sts)
         with torch.cuda.device(dev):
             self._upload(host, blocks, dev)

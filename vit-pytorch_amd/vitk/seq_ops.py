@@ -45,15 +45,10 @@ def _one_device(what, first, *ts):
 
 def _rows(t):
     """`t` as the kernels address it: consecutive elements inside a head, pointer and strides multiples of 16 bytes, tokens
-    less than 2^23 elements apart.  (A contiguous head of 32 elements or more is such a multiple.)"""
-    if t.data_ptr() % 16 == 0:
-        if t.is_contiguous():
-            if t.dim() < 4 or t.stride(1) < 1 << 23:
-                return t
-        else:
-            st, unit = t.stride(), 16 // t.element_size()
-            if st[-1] == 1 and not any(s % unit for s in st[:-1]) and st[1] < 1 << 23:
-                return t
+    less than 2^23 elements apart."""
+    st, unit = t.stride(), 16 // t.element_size()
+    if t.data_ptr() % 16 == 0 and st[-1] == 1 and st[1] < 1 << 23 and not any(s % unit for s in st[:-1]):
+        return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
@@ -142,6 +137,8 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
         raise VitkError("axial_rope: out= is not differentiable")
     if out.shape != x.shape or out.dtype != x.dtype or out.stride(-1) != 1:
         raise VitkError("axial_rope: out has x's shape and type and consecutive elements inside a head")
+    if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise VitkError("axial_rope: out holds an element in more than one place")
     _one_device("axial_rope", x, out)
     x = x if x.stride(-1) == 1 else x.contiguous()
     if out.numel():
