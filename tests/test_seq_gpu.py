@@ -95,7 +95,10 @@ ATTN = [  # (B, N, Hq, Hkv, dh, causal, window, sinks, lengths)
     (4, 200, 2, 2, 32, True, 64, 5, (200, 0, 1, 130)), (1, 300, 6, 2, 64, False, 20, 70, None), (1, 300, 3, 3, 128, True, 50, 140, None),
     (2, 257, 4, 1, 64, True, 1000, 0, (257, 250)), (1, 257, 4, 4, 64, False, None, 0, None), (2, 160, 2, 2, 64, True, 0, 2, (160, 9)),
     (1, 96, 2, 2, 64, False, 0, 0, None), (1, 96, 2, 2, 64, False, 0, 3, None), (1, 513, 2, 2, 128, False, 128, 0, None),
-    (1, 700, 5, 1, 64, True, 128, 4, None), (1, 1025, 1, 1, 64, False, 65, 33, (999,))]
+    (1, 700, 5, 1, 64, True, 128, 4, None), (1, 1025, 1, 1, 64, False, 65, 33, (999,)),
+    # few key heads, many queries a key: several workgroups to a band of keys
+    (2, 700, 8, 1, 64, False, 150, 3, (700, 90)), (1, 150, 8, 1, 32, False, 100, 4, None), (2, 390, 12, 2, 128, True, None, 0, (390, 0)),
+    (1, 520, 16, 1, 128, True, 100, 40, (333,)), (1, 1500, 2, 1, 64, True, None, 0, None), (1, 260, 20, 1, 128, False, 70, 2, None)]
 
 
 @pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])

@@ -44,6 +44,8 @@ struct Slide {
                                // for all that 32 of them see, and no records
     float* ws;                 // forward: records of dh + 2; backward: dk | dv, then dq, records of dh
     float* ws_q;
+    float* ws_b;               // of dK / dV bands that `shares` workgroups have in common: records of dk | dv, one of each share
+    int shares;
     int far_items, items;      // of this launch: far ones come first, then bands
 };
 
@@ -152,7 +154,10 @@ template <bool CAUSAL> __device__ __forceinline__ Tiles query_tiles(int ka, int 
 template <typename T, int DH> struct Shape {
     static constexpr int ROW = DH * (int)sizeof(T);
     static constexpr int CHUNKS = ROW / 16;
-    static constexpr int KT = sizeof(T) == 2 ? 64 : 32;           // rows of a staged tile
+    // Rows of a staged tile.  In fp32, 64 rows of a head of 32 (4 sequences of 4099 causal tokens, backward: 381 us with 32 rows, 338 us),
+    // but 32 of a head of 64, whose tiles of 64 would leave two workgroups a CU (the same: 702 and 663 us; 8 images of 2305
+    // tokens: 974 and 1016 us).
+    static constexpr int KT = ROW <= 128 || sizeof(T) == 2 ? 64 : 32;
     static constexpr int PER = ROW >= 256 ? 1 : 256 / ROW;        // rows in 64 banks
     static __device__ __forceinline__ int mix(int r) {
         if constexpr (sizeof(T) == 2) return ((r & 3) / PER << 2) | ((r >> 2) & 3);
@@ -841,7 +846,8 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const f
 // How a workgroup of the dK / dV kernel is laid out: NW waves, 32 KG keys; wave w keeps keys 32 (w % KG) and takes every
 // (NW / KG)-th 32 queries, and the parts are added at the end.  Four waves of 32 keys each where there are enough of them;
 // bands of 64 keys where heads are few; and for bf16 heads of 128, whose four operands and sums of a wave leave room for
-// one wave a SIMD only, eight waves with K and V in LDS, two to a SIMD (FIGURES).
+// one wave a SIMD only, eight waves with K and V in LDS, two to a SIMD (16384 causal tokens, 2 key heads, window 1024: 249 us with
+// four waves, 187 us, which is 711 TFLOP/s).
 template <typename T, int DH, int NW, int KG> struct Layout {
     using S = Shape<T, DH>;
     static constexpr bool IN_LDS = NW == 8;
@@ -869,7 +875,7 @@ template <typename T, int DH, int NT> __device__ __forceinline__ void keep_rows(
 }
 // Band: the queries of every head that shares the keys stream through LDS.
 template <typename T, int DH, bool CAUSAL, int NW, int KG>
-__device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int hk, int b, int n) {
+__device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int share, int hk, int b, int n) {
     using S = Shape<T, DH>;
     using L = Layout<T, DH, NW, KG>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -892,12 +898,19 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
     const float sc = p.scale * LOG2E;
     f32x16 dk[DH / 32] = {}, dv[DH / 32] = {};
     const Tiles tl = query_tiles<CAUSAL>(k0, k0 + 32 * KG - 1, n, p.window, p.sinks, S::KT);
-    const int per = tl.count(), cnt = per * p.G;
+    const int per = tl.count();
+    int cnt = per * p.G, next_g = 0, next_t = 0;                         // this share's turns, its first one's head and tile
+    if (p.shares > 1 && cnt > 0) {
+        const int from = (int)((long)cnt * share / p.shares);
+        cnt = (int)((long)cnt * (share + 1) / p.shares) - from;
+        next_g = from / per;
+        next_t = from - next_g * per;
+    }
+    int tt = next_t;
     const Span sp = queries_of<CAUSAL>(kj, n, p.window, p.sinks);
     const Cover cover = queries_by<CAUSAL>(ka, n, p.window, p.sinks);
     const bool elsewhere = ka < p.rows && !p.chunks;
     const Stage<T, DH, L::NT> fq(p.q_n, tid), fo(p.do_n, tid);
-    int next_g = 0, next_t = 0;
     const auto start = [&](char* buf) {                 // the tiles in order, head after head
         const int h = hk * p.G + next_g, q0 = tl.at(next_t) * S::KT;
         fq.start(buf, (const T*)p.q + b * p.q_b + h * p.q_h, q0, n, tid);
@@ -910,7 +923,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
         if (++next_t == per) { next_t = 0; ++next_g; }
     };
     if (cnt > 0) start(lds);
-    for (int t = 0, tt = 0; t < cnt; ++t, tt = tt + 1 == per ? 0 : tt + 1) {
+    for (int t = 0; t < cnt; ++t, tt = tt + 1 == per ? 0 : tt + 1) {
         const char* now = lds + (t & 1) * L::BUF;
         dma_wait();
         __syncthreads();
@@ -945,8 +958,9 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
         if (part) return;
     }
     if (kj >= p.N || elsewhere) return;
-    if (kj < p.rows) {
-        float* rec = p.ws + ((((long)b * p.Hkv + hk) * p.rows + kj) * (p.chunks + 1) + p.chunks) * (2 * DH);
+    if (kj < p.rows || p.shares > 1) {
+        float* rec = p.shares > 1 ? p.ws_b + ((((long)b * p.Hkv + hk) * p.N + kj) * p.shares + share) * (2 * DH)
+                                  : p.ws + ((((long)b * p.Hkv + hk) * p.rows + kj) * (p.chunks + 1) + p.chunks) * (2 * DH);
         put<float, DH>(rec, dk, 1.f, lane);
         put<float, DH>(rec + DH, dv, 1.f, lane);
     } else {
@@ -1019,29 +1033,37 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
 template <typename T, int DH, bool CAUSAL, int NW, int KG>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && (DH < 128 || NW == 8) ? 2 : 1) void slide_dkv_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
-    const Item it = item_of(p, p.Hkv, (p.N + 32 * KG - 1) / (32 * KG));
+    const Item it = item_of(p, p.Hkv, (p.N + 32 * KG - 1) / (32 * KG) * p.shares);
     if (it.none) return;
     const int n = length_of(p, it.b);
     if (it.far) dkv_far<T, DH, CAUSAL, NW, KG>(p, lds, it.x, it.h, it.b, n);
-    else dkv_band<T, DH, CAUSAL, NW, KG>(p, lds, it.x * (32 * KG), it.h, it.b, n);
+    else {
+        const int band = p.shares > 1 ? it.x / p.shares : it.x;
+        dkv_band<T, DH, CAUSAL, NW, KG>(p, lds, band * (32 * KG), it.x - band * p.shares, it.h, it.b, n);
+    }
 }
-// The records of the first rows become gradients: blockIdx.y < kv_heads dk and dv, behind them dq.  256 / DH shares of the
-// records, each in its order, then the shares in theirs.
-template <typename T, int DH> __global__ __launch_bounds__(256) void slide_bwd_join_kernel(Slide p, int kv_heads, int rows, int k_recs, int q_recs) {
+// Records become gradients.  Of the keys that are first tokens: their far items' and the band's; of all keys, where shares of
+// a band were done apart: the shares'.  Of the queries that are first tokens (the workgroups behind `keys` ones): their
+// items' and the band's.  256 / DH workgroup parts add some of them, each in its order, and then their sums in theirs.
+template <typename T, int DH> __global__ __launch_bounds__(256) void slide_bwd_join_kernel(Slide p, int keys, int rows, int k_chunks, int q_chunks) {
     constexpr int SHARES = 256 / DH;
     __shared__ float part[2][256];
-    const int i = blockIdx.x, b = blockIdx.z, d = threadIdx.x % DH, share = threadIdx.x / DH;
-    const int h = (int)blockIdx.y - kv_heads, hk = blockIdx.y;
-    const bool keys = h < 0;
-    const int recs = keys ? k_recs : q_recs, width = keys ? 2 * DH : DH;
-    const float* rec = (keys ? p.ws + (((long)b * p.Hkv + hk) * rows + i) * recs * width
-                             : p.ws_q + (((long)b * p.Hq + h) * rows + i) * recs * width) + d;
+    const bool key = (int)blockIdx.x < keys;
+    const int id = key ? blockIdx.x : blockIdx.x - keys, heads = key ? p.Hkv : p.Hq;
+    const int i = id / heads, h = id % heads, b = blockIdx.y, d = threadIdx.x % DH, share = threadIdx.x / DH;
+    const int width = key ? 2 * DH : DH, chunks = key ? k_chunks : q_chunks;
+    if (key && !chunks && i < rows) return;                   // done by items of their own
+    const bool split = key && p.shares > 1;
     float x = 0.f, y = 0.f;
+    const auto add = [&](const float* rec, int count) {
 #pragma unroll 4
-    for (int s = share; s < recs; s += SHARES) {
-        x += rec[(long)s * width];
-        if (keys) y += rec[(long)s * width + DH];
-    }
+        for (int s = share; s < count; s += SHARES) {
+            x += rec[(long)s * width + d];
+            if (key) y += rec[(long)s * width + DH + d];
+        }
+    };
+    if (i < rows) add((key ? p.ws : p.ws_q) + (((long)b * heads + h) * rows + i) * (chunks + 1) * width, chunks + !split);
+    if (split) add(p.ws_b + (((long)b * heads + h) * p.N + i) * p.shares * width, p.shares);
     part[0][threadIdx.x] = x;
     part[1][threadIdx.x] = y;
     __syncthreads();
@@ -1050,9 +1072,9 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_bwd_j
     for (int s = 1; s < SHARES; ++s) { x += part[0][s * DH + d]; y += part[1][s * DH + d]; }
     const int n = length_of(p, b);
     const bool there = i < n;
-    if (keys) {
-        ((T*)p.dk)[b * p.dk_b + (long)i * p.dk_n + hk * p.dk_h + d] = (T)(there ? x * score_scale(p, n) : 0.f);
-        ((T*)p.dv)[b * p.dv_b + (long)i * p.dv_n + hk * p.dv_h + d] = (T)(there ? y : 0.f);
+    if (key) {
+        ((T*)p.dk)[b * p.dk_b + (long)i * p.dk_n + h * p.dk_h + d] = (T)(there ? x * score_scale(p, n) : 0.f);
+        ((T*)p.dv)[b * p.dv_b + (long)i * p.dv_n + h * p.dv_h + d] = (T)(there ? y : 0.f);
     } else {
         ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(there ? x * score_scale(p, n) : 0.f);
     }
@@ -1158,6 +1180,24 @@ Records records_of(int B, int N, int heads, int G, int width, int window, int si
     r.floats = (long)B * heads * r.rows * (r.chunks + 1) * width;
     return r;
 }
+// Bands of the dK / dV kernel: 32 `groups` keys, `shares` workgroups each, floats of workspace for their records.  Bands of 64
+// keys where there are fewer than two of 128 for each CU (577 tokens, 6 of 4 key heads: 22 us, bands of 128 26 us; at 750 bands
+// 50 us against 41), and then as many shares as it takes to fill the chip, of 8 turns and more, behind which the records
+// are added (4096 causal tokens, 2 key heads of 4 queries each, 128 elements: 139 us unsplit, 76 us; 1024 tokens of 64: 48 us and 23 us,
+// and with shares of 2 turns 29 us).
+struct Bands { int groups, shares; long floats; };
+Bands bands_of(int B, int N, int Hkv, int G, bool causal, int window, bool bf16, int dh) {
+    Bands r{4, 1, 0};
+    const bool wide = dkv_waves(bf16, dh) == 8;
+    if (!wide && (long)vitk_ceil_div(N, TQ) * Hkv * B < 512) r.groups = 2;
+    const long bands = (long)vitk_ceil_div(N, 32 * r.groups) * Hkv * B;
+    const long reach = (causal ? window : 2L * window) + 32 * r.groups, turns = G * (((reach < N ? reach : N) + 63) / 64);
+    const long some = (wide ? 256 : 512) / bands, least = turns / 8;
+    r.shares = (int)(some < least ? some : least);
+    if (r.shares < 2) r.shares = 1;
+    else r.floats = (long)B * Hkv * N * r.shares * 2 * dh;
+    return r;
+}
 // Window and sinks of N tokens without what they cannot tell apart: all visible is a window of N.
 void reach(const vitk_slide_attn* a, int& window, int& sinks) {
     window = a->window < a->N ? a->window : a->N;
@@ -1165,9 +1205,9 @@ void reach(const vitk_slide_attn* a, int& window, int& sinks) {
     if (sinks >= a->N) window = a->N;
     if (window >= a->N) sinks = 0;
 }
-unsigned grid_of(Slide& p, int heads, bool far, int rows = TQ) {
+unsigned grid_of(Slide& p, int heads, bool far, int rows = TQ, int shares = 1) {
     p.far_items = far ? (p.chunks ? p.chunks : 1) * (p.rows / 32) * heads * p.B : 0;
-    const long bands = (long)vitk_ceil_div(p.N, rows) * heads * p.B;
+    const long bands = (long)vitk_ceil_div(p.N, rows) * heads * p.B * shares;
     p.items = (int)(p.far_items + bands);
     return (unsigned)(p.far_items + (bands + 7) / 8 * 8);
 }
@@ -1179,7 +1219,7 @@ template <typename T, int DH> constexpr int lds_bytes(bool far) {      // of the
 template <typename T, int DH, bool CAUSAL, int NW, int KG> int launch_dkv(Slide& p, hipStream_t st) {
     const int bytes = Layout<T, DH, NW, KG>::bytes(p.rows > 0);
     if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, NW, KG>, bytes)) return e;
-    const unsigned grid = grid_of(p, p.Hkv, p.rows > 0, 32 * KG);
+    const unsigned grid = grid_of(p, p.Hkv, p.rows > 0, 32 * KG, p.shares);
     hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, NW, KG>), dim3(grid), dim3(NW * 64), bytes, st, p);
     VITK_CHECK_LAUNCH();
     return 0;
@@ -1203,12 +1243,15 @@ template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipSt
 }
 template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipStream_t st) {
     const Records rk = records_of(p.B, p.N, p.Hkv, p.G, 2 * DH, p.window, p.sinks, dkv_waves(sizeof(T) == 2, DH));
+    const Bands bands = bands_of(p.B, p.N, p.Hkv, p.G, CAUSAL, p.window, sizeof(T) == 2, DH);
     const Records rq = CAUSAL ? Records{0, 0, 0} : records_of(p.B, p.N, p.Hq, 1, DH, p.window, p.sinks, 4);
-    if (rk.floats + rq.floats && !ws) return VITK_ERR_NULL;
+    if (rk.floats + bands.floats + rq.floats && !ws) return VITK_ERR_NULL;
     const int bytes = lds_bytes<T, DH>(rq.rows > 0);
     if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL>, bytes)) return e;
     p.ws = ws;
-    p.ws_q = ws + rk.floats;
+    p.ws_b = ws + rk.floats;
+    p.ws_q = p.ws_b + bands.floats;
+    p.shares = bands.shares;
     if (p.dq) {
         p.rows = rq.rows; p.chunks = rq.chunks;
         const unsigned grid = grid_of(p, p.Hq, rq.rows > 0);
@@ -1221,15 +1264,14 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipSt
         p.rows = rk.rows; p.chunks = rk.chunks;
         int e;
         if constexpr (dkv_waves(sizeof(T) == 2, DH) == 8) e = launch_dkv<T, DH, CAUSAL, 8, 4>(p, st);
-        // few key heads leave CUs without a band of 128 keys: bands of 64 below two of them for each CU
-        else if ((long)vitk_ceil_div(p.N, TQ) * p.Hkv * p.B < 512) e = launch_dkv<T, DH, CAUSAL, 4, 2>(p, st);
+        else if (bands.groups == 2) e = launch_dkv<T, DH, CAUSAL, 4, 2>(p, st);
         else e = launch_dkv<T, DH, CAUSAL, 4, 4>(p, st);
         if (e) return e;
     }
-    const int kv_heads = p.dk && rk.chunks ? p.Hkv : 0, q_heads = p.dq && rq.chunks ? p.Hq : 0;
-    if (kv_heads + q_heads) {
-        hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(rk.rows < p.N ? rk.rows : p.N, kv_heads + q_heads, p.B), dim3(256), 0, st,
-                           p, kv_heads, rk.rows, rk.chunks + 1, rq.chunks + 1);
+    const int first = rk.rows < p.N ? rk.rows : p.N;
+    const int keys = !p.dk ? 0 : (bands.shares > 1 ? p.N : rk.chunks ? first : 0) * p.Hkv, queries = p.dq && rq.chunks ? first * p.Hq : 0;
+    if (keys + queries) {
+        hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH>), dim3(keys + queries, p.B), dim3(256), 0, st, p, keys, rk.rows, rk.chunks, rq.chunks);
         VITK_CHECK_LAUNCH();
     }
     return 0;
@@ -1317,6 +1359,7 @@ extern "C" size_t vitk_slide_attn_workspace(const vitk_slide_attn* a, int dtype,
         if (!a->causal) n = records_of(a->B, a->N, a->Hq, 1, a->dh + 4, window, sinks, 4).floats;
     } else {
         n = records_of(a->B, a->N, a->Hkv, a->Hq / a->Hkv, 2 * a->dh, window, sinks, dkv_waves(dtype == VITK_BF16, a->dh)).floats;
+        n += bands_of(a->B, a->N, a->Hkv, a->Hq / a->Hkv, a->causal, window, dtype == VITK_BF16, a->dh).floats;
         if (!a->causal) n += records_of(a->B, a->N, a->Hq, 1, a->dh, window, sinks, 4).floats;
     }
     return (size_t)n * sizeof(float);
