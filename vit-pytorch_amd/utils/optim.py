@@ -14,6 +14,7 @@ torch.optim.SGD without Nesterov: the momentum buffer starts as the first (clipp
 There is no CPU path: the tensors must live on the GPU and the kernel library must load.
 """
 import ctypes
+from operator import attrgetter
 
 import numpy as np
 import torch
@@ -200,7 +201,7 @@ class FusedAdamW(torch.optim.Optimizer):
             for name in ("exp_avg_scale", "exp_avg_sq_scale"):
                 st[name] = torch.empty(-(-p.numel() // _SCALE_BLOCK), dtype=torch.float32, device=p.device)
 
-    def _table(self, ps, grads, sts):
+    def _table(self, ps, grads, sts, sizes):
         """The rows of all tensors, column by column, with blocks counted from 0; (table, number of blocks)."""
         host = np.zeros(len(ps), dtype=_ADAMW_ENTRY)
         host["param"] = [p.data_ptr() for p in ps]
@@ -210,7 +211,7 @@ class FusedAdamW(torch.optim.Optimizer):
         if self.state_bits == 8:
             host["m_scale"] = [s["exp_avg_scale"].data_ptr() for s in sts]
             host["v_scale"] = [s["exp_avg_sq_scale"].data_ptr() for s in sts]
-        host["n"] = [p.numel() for p in ps]
+        host["n"] = sizes
         blocks = np.cumsum((host["n"] + (_CHUNK - 1)) // _CHUNK)
         host["block0"][1:] = blocks[:-1]
         vec = ((host["param"] | host["grad"]) % 16 == 0) & ((host["m"] | host["v"]) % (4 if self.state_bits == 8 else 16) == 0)
@@ -252,37 +253,44 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError("FusedAdamW does not re-evaluate the model")
         if max_grad_norm is not None and not max_grad_norm >= 0.0:
             raise ValueError("max_grad_norm must be non-negative")
-        state, f32 = self.state, torch.float32
-        groups = [[p for p in group["params"] if p.grad is not None and p.numel()] for group in self.param_groups]
-        first = next((ps[0] for ps in groups if ps), None)
-        if first is None:
+        # (loops over bound methods of the class: with a few hundred small tensors this function is what a step costs)
+        state, Tensor = self.state, torch.Tensor
+        groups = []
+        for group in self.param_groups:
+            pairs = [(p, g) for p in group["params"] if (g := p.grad) is not None and g.numel()]
+            groups.append(([p for p, _ in pairs], [g for _, g in pairs]))
+        all_ps, all_grads = sum((ps for ps, _ in groups), []), sum((grads for _, grads in groups), [])
+        if not all_ps:
             return None
-        dev, at = first.device, first.get_device()
-        for ps in groups:
-            grads = [p.grad for p in ps]
-            if not (dev.type == "cuda" and all(p.dtype is f32 and p.get_device() == at and p.is_contiguous() for p in ps)
-                    and all(g.dtype is f32 and g.get_device() == at and not g.is_sparse and g.is_contiguous() for g in grads)):
-                raise ValueError("FusedAdamW needs contiguous fp32 parameters and gradients on one GPU")
+        dev, both = all_ps[0].device, all_ps + all_grads
+        if (dev.type != "cuda" or any(map(attrgetter("is_sparse"), all_grads)) or set(map(attrgetter("dtype"), both)) != {torch.float32}
+                or set(map(Tensor.get_device, both)) != {dev.index} or not all(map(Tensor.is_contiguous, both))):
+            raise ValueError("FusedAdamW needs contiguous fp32 parameters and gradients on one GPU")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW.step counts steps on the host and is not captured into a graph")
         # one launch for the tensors of a group that have taken the same number of steps
-        all_ps, all_sts, spans = [], [], []
-        for group, ps in zip(self.param_groups, groups):
+        all_ps, all_grads, all_sts, spans = [], [], [], []
+        for group, (ps, grads) in zip(self.param_groups, groups):
             sts = [state[p] for p in ps]
             for p, st in zip(ps, sts):
                 if not st:
                     self._begin(p, st)
             steps = [st["step"] for st in sts]
             for t in dict.fromkeys(steps):
-                of_t = [i for i, x in enumerate(steps) if x == t] if steps.count(t) != len(steps) else range(len(steps))
-                spans.append((group, t, len(all_ps), len(of_t)))
-                all_ps += [ps[i] for i in of_t]
-                all_sts += [sts[i] for i in of_t]
-        # a parameter may have got another tensor, or moved, since its states were made
-        if not all(st["exp_avg"].get_device() == at and st["exp_avg"].shape == p.shape for p, st in zip(all_ps, all_sts)):
-            raise ValueError("a parameter's shape or device is not that of its moments")
-        all_grads = [p.grad for p in all_ps]
-        host, blocks = self._table(all_ps, all_grads, all_sts)
+                of_t = (ps, grads, sts)
+                if steps.count(t) != len(steps):
+                    of_t = ([x for x, n in zip(xs, steps) if n == t] for xs in of_t)
+                at = len(all_ps)
+                for xs, more in zip((all_ps, all_grads, all_sts), of_t):
+                    xs += more
+                spans.append((group, t, at, len(all_ps) - at))
+        # a parameter may have got another tensor, or moved, since its gradient or its states were made
+        moments = [st["exp_avg"] for st in all_sts]
+        sizes = list(map(Tensor.numel, all_ps))
+        if (sizes != list(map(Tensor.numel, moments)) or sizes != list(map(Tensor.numel, all_grads))
+                or set(map(Tensor.get_device, moments)) != {dev.index}):
+            raise ValueError("a parameter's size or device is not that of its gradient or its moments")
+        host, blocks = self._table(all_ps, all_grads, all_sts, sizes)
         with torch.cuda.device(dev):
             self._upload(host, blocks, dev)
             if self._slots is None:
