@@ -482,9 +482,10 @@ template <int DH, int NW, typename F> __device__ __forceinline__ void add_waves(
 }
 
 // Tiles of two matrices through LDS, two buffers deep: while one tile is used, the next one is on its way, and one
-// barrier a tile orders the two.  use(first tile, second tile, first row).
-template <typename T, int DH, typename F>
-__device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T* B, long ldb, const Tiles& tl, int n, int tid, F use) {
+// barrier a tile orders the two.  use(first tile, second tile, first row); ready() waits for what the loop keeps with the first
+// tiles on their way (forward, 1024 tokens of 8 heads: 15.9 -> 15.1 us; in the backward kernels it gained nothing).
+template <typename T, int DH, typename R, typename F>
+__device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T* B, long ldb, const Tiles& tl, int n, int tid, R ready, F use) {
     using S = Shape<T, DH>;
     constexpr int BYTES = S::KT * S::ROW;
     const Stage<T, DH> fa(lda, tid), fb(ldb, tid);
@@ -493,6 +494,7 @@ __device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T*
         fa.start(lds, A, tl.at(0) * S::KT, n, tid);
         fb.start(lds + BYTES, B, tl.at(0) * S::KT, n, tid);
     }
+    ready();
     for (int t = 0; t < cnt; ++t) {
         char* now = lds + (t & 1) * 2 * BYTES;
         char* next = lds + (~t & 1) * 2 * BYTES;
@@ -537,7 +539,6 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
     const T* V = (const T*)p.v + b * p.v_b + hk * p.v_h;
     Kept<T, DH> q;
     q.load((const T*)p.q + b * p.q_b + h * p.q_h + (long)qi * p.q_n, lane >> 5, qi < n);
-    q.settle();
     const bool elsewhere = !CAUSAL && qa < p.rows && !p.chunks;          // an item of its own does these rows
     const float sc = p.scale * LOG2E;
     const Span sp = keys_of<CAUSAL>(qi, n, p.window, p.sinks);
@@ -549,7 +550,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
     };
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&](const char* Ks, const char* Vs, int k0) {
+    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&] { q.settle(); }, [&](const char* Ks, const char* Vs, int k0) {
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
@@ -749,7 +750,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     const Cover cover = keys_by<CAUSAL>(qa, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&](const char* Ks, const char* Vs, int k0) {
+    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [] {}, [&](const char* Ks, const char* Vs, int k0) {
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
