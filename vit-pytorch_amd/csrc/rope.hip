@@ -3,6 +3,8 @@
 // Memory-bound: every element is read and written once, 3 operations each.  A workgroup takes a few tokens; the angles of
 // a token are the same for all of its heads, so they are computed once, reduced to one turn in 64 bits (in 32 a position
 // of a million has lost its fraction of a turn), and kept in LDS as cosines and sines while the heads stream past.
+// 113 MB of bf16 read and as much written in 45 us, 206 MB of fp32 in 88 us (5.0 and 4.7 TB/s; a large copy reaches 4.9): 4 tokens a workgroup,
+// which is 2 to 4 vectors a thread of heads like these.
 #include "common.h"
 
 namespace {
@@ -29,7 +31,7 @@ __device__ __forceinline__ double position(const Rope& p, long at) {
     return reinterpret_cast<const double*>(p.pos)[at];
 }
 
-// V: elements moved at once.  Half pairing: V pairs from two places V elements wide; interleaved: V / 2 pairs in a row.
+// V: elements moved at once, 16 bytes where pairs, strides and addresses allow it.  Half pairing: V pairs from two places V elements wide; interleaved: V / 2 pairs in a row.
 template <typename T, int V, bool INTERLEAVED, int TOK>
 __global__ __launch_bounds__(256) void rope_kernel(Rope p) {
     __shared__ float cs[TOK][MAX_PAIRS], sn[TOK][MAX_PAIRS];
