@@ -210,14 +210,14 @@ int vitk_window_attn_bwd(const void* qkv, const float* bias_table, const void* o
  * lengths:[B] int32 on the device (NULL: N tokens each): tokens behind a sequence's length are neither read as keys nor
  * computed as queries, whatever memory holds there; their outputs and gradients are written as 0.
  * o:[B, N, Hq, dh] contiguous.  For a backward pass: lse:[B, Hq, N] (base-2 logarithm of each row's sum, +inf for a row
- * that sees nothing) and, in bf16, o_f32 (o unrounded, contiguous), both NULL without one.
- * vitk_slide_attn_bwd reads q, k, v, d_o, lse, o_f32 (fp32: o) and writes dq, dk, dv (strided; dq, or dk and dv together,
+ * that sees nothing) and, in bf16, o_rest (like o: what rounding o left, in units of 1/256 of its last place), both NULL without one.
+ * vitk_slide_attn_bwd reads q, k, v, d_o, lse, o, o_rest (bf16) and writes dq, dk, dv (strided; dq, or dk and dv together,
  * may be NULL: not wanted); delta:[B, Hq, N] is workspace.  Sums have a fixed order: equal inputs give equal bits.
  * dh 32, 64 or 128; every pointer 16-byte aligned, every stride a multiple of 16 bytes, *_n below 2^23; Hq % Hkv == 0; window, sinks >= 0;
  * scale > 0. */
 typedef struct vitk_slide_attn {
     const void* q; const void* k; const void* v;
-    void* o; float* o_f32; float* lse;
+    void* o; signed char* o_rest; float* lse;
     const int* lengths;
     const void* d_o; float* delta;
     void* dq; void* dk; void* dv;

@@ -41,7 +41,8 @@ def attention(q, k, v, seen, scale, r, d_o=None):
         delta = (p * dp).sum(1, keepdim=True)
         ds = p * (dp - delta)
         e_dp = dh * U * (d_o.abs() @ v.abs().t())
-        e_delta = (d_o.abs() * e_o).sum(1, keepdim=True) + (dh + 4) * U * (d_o.abs() * o.abs()).sum(1, keepdim=True)
+        # the output that delta reads holds 7 bits behind a rounded one's
+        e_delta = (d_o.abs() * e_o).sum(1, keepdim=True) + (r * 2.0 ** -7 + (dh + 4) * U) * (d_o.abs() * o.abs()).sum(1, keepdim=True)
         e_ds = e_p * (dp.abs() + delta.abs()) + p * (e_dp + e_delta) + (r + 4 * U) * ds.abs()
         for name, val, err in (("dq", ds @ k * scale, (e_ds + m * U * ds.abs()) @ k.abs() * scale),
                                ("dk", ds.t() @ q * scale, (e_ds + q.shape[0] * U * ds.abs()).t() @ q.abs() * scale),

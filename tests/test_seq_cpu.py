@@ -79,10 +79,10 @@ def test_c_entry_of_the_forward_pass_refuses(change, dtype, code):
 
 
 @pytest.mark.parametrize("change,dtype,code", [
-    (dict(d_o=None), 0, -3), (dict(lse=None), 0, -3), (dict(delta=None), 0, -3), (dict(o_f32=None), 0, -3), (dict(o=None), 1, -3),
+    (dict(d_o=None), 0, -3), (dict(lse=None), 0, -3), (dict(delta=None), 0, -3), (dict(o_rest=None), 0, -3), (dict(o=None), 0, -3), (dict(o=None), 1, -3),
     (dict(dk=None), 0, -3), (dict(dq=None, dk=None, dv=None), 0, -3), (dict(do_n=4), 0, -1), (dict(dq=4104), 0, -1)])
 def test_c_entry_of_the_backward_pass_refuses(change, dtype, code):
-    a = dict(d_o=4096, lse=4096, delta=4096, o_f32=4096, dq=4096, dk=4096, dv=4096)
+    a = dict(d_o=4096, lse=4096, delta=4096, o_rest=4096, dq=4096, dk=4096, dv=4096)
     assert vitk.lib.vitk_slide_attn_bwd(ctypes.byref(_attn(**{**a, **change})), dtype, None) == code
 
 

@@ -25,7 +25,7 @@
 //   8 x 2305 x 12 x 64, all visible:            forward 186 us (702 TFLOP/s), dQ 229 (854), dK / dV 319 (818)
 //   1 x 16384 x 8 of 2 x 128, causal, window 1024:     87 us (769),               112 (888),          187 (712)
 //   8 x 2305 x 12 x 64, window 145, 1 first token:     53 us (299),                75 (315),          114 (279)
-// In the last, whose band is little longer than its rows, 113 MB forward and 370 MB backward are half of the time at the rate of
+// In the last, whose band is little longer than its rows, 113 MB forward and 353 MB backward are half of the time at the rate of
 // a copy.
 #include <initializer_list>
 
@@ -39,7 +39,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TQ = 128;                       // rows of a workgroup: four waves of 32
 
 struct Slide {
-    const void* q; const void* k; const void* v; void* o; float* o32; float* lse; const int* lengths;
+    const void* q; const void* k; const void* v; void* o; int8_t* rest; float* lse; const int* lengths;
     const void* d_o; float* delta; void* dq; void* dk; void* dv;
     int B, N, Hq, Hkv, G;
     long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, do_b, do_n, do_h, dq_b, dq_n, dq_h, dk_b, dk_n, dk_h, dv_b, dv_n, dv_h;
@@ -368,6 +368,23 @@ template <typename T, int DH> __device__ __forceinline__ void put(T* row, const 
             Vec4<T>::store(row + 32 * d + 8 * b + 4 * (lane >> 5), x);
         }
 }
+// What rounding x to bf16 left, in units of 1/256 of the last place: with it an output has 15 bits behind the leading one, in
+// 8 bits more of memory (o in 32 bits beside it: 16384-token training pass 383 us, so 379, and 3 bytes an element more kept).
+__device__ __forceinline__ int rest_of(float x) {
+    const int r = (int)(__float_as_uint(x) - ((unsigned)__builtin_bit_cast(unsigned short, (bf16_t)x) << 16));
+    return least((r + 128) >> 8, 127);
+}
+template <int DH> __device__ __forceinline__ void put_rest(int8_t* row, const f32x16* acc, float mul, int lane) {
+#pragma unroll
+    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            unsigned x = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x |= (unsigned)(rest_of(acc[d][4 * b + e] * mul) & 255) << (8 * e);
+            *reinterpret_cast<unsigned*>(row + 32 * d + 8 * b + 4 * (lane >> 5)) = x;
+        }
+}
 // What the sums of dQ and dK are multiplied with.  A query that sees one key only has the probability 1 whatever its score:
 // where all do, the gradients of the scores are exactly 0, and not what dP - delta leaves after rounding.
 __device__ __forceinline__ float score_scale(const Slide& p, int n) { return p.single || n == 1 ? 0.f : p.scale; }
@@ -533,7 +550,7 @@ __device__ __forceinline__ void write_row(const Slide& p, int b, int h, int i, i
     const float x = total > 0.f ? sum / total : 0.f;
     const long row = ((long)b * p.N + i) * p.Hq + h;
     ((T*)p.o)[row * DH + d] = (T)x;
-    if (p.o32) p.o32[row * DH + d] = x;
+    if (sizeof(T) == 2 && p.rest) p.rest[row * DH + d] = (int8_t)rest_of(x);
     if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.N + i] = total > 0.f ? top + __log2f(total) : INFINITY;
 }
 // Band: 128 queries of one (sequence, head), each wave 32 of them; key tiles stream through LDS.
@@ -584,7 +601,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         const float inv = l > 0.f ? 1.f / l : 0.f;
         const long row = ((long)b * p.N + qi) * p.Hq + h;
         put<T, DH>((T*)p.o + row * DH, acc, inv, lane);
-        if (p.o32) put<float, DH>(p.o32 + row * DH, acc, inv, lane);
+        if (sizeof(T) == 2 && p.rest) put_rest<DH>(p.rest + row * DH, acc, inv, lane);
         // base-2 logarithm of the row's sum; +inf for a row that sees nothing, so that backward's probabilities are 0
         if (p.lse && lane < 32) p.lse[((long)b * p.Hq + h) * p.N + qi] = l > 0.f ? m + __log2f(l) : INFINITY;
     }
@@ -700,23 +717,29 @@ __device__ __forceinline__ f32x16 rows_of(const float* x, int r0) {
     }
     return y;
 }
-// delta = -dO . o of a kept row; o in 32 bits, so that what the rounded output lost is not multiplied by the cancellation in
-// dP - delta.
-template <int DH> __device__ __forceinline__ float delta_of(const Kept<bf16_t, DH>& d_o, const float* o, int h, bool ok) {
+// delta = -dO . o of a kept row, whose elements begin at `at` of o; o with what its rounding left, so that this is not multiplied
+// by the cancellation in dP - delta.
+template <int DH> __device__ __forceinline__ float delta_of(const Kept<bf16_t, DH>& d_o, const Slide& p, long at, int h, bool ok) {
     float s = 0.f;
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+        u32x4 x = {0, 0, 0, 0};
+        u32x2 y = {0, 0};
         if (ok) {
-            x = *reinterpret_cast<const f32x4*>(o + 16 * c + 8 * h);
-            y = *reinterpret_cast<const f32x4*>(o + 16 * c + 8 * h + 4);
+            x = *reinterpret_cast<const u32x4*>((const bf16_t*)p.o + at + 16 * c + 8 * h);
+            y = *reinterpret_cast<const u32x2*>(p.rest + at + 16 * c + 8 * h);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s += (float)d_o.f[c][e] * x[e] + (float)d_o.f[c][4 + e] * y[e];
+        for (int e = 0; e < 8; ++e) {
+            const unsigned high = e & 1 ? x[e >> 1] & 0xFFFF0000u : x[e >> 1] << 16;
+            const int low = ((int)(y[e >> 2] << (24 - 8 * (e & 3))) >> 24) * 256;
+            s += (float)d_o.f[c][e] * __uint_as_float(high + (unsigned)low);
+        }
     }
     return -(s + __shfl_xor(s, 32, 64));
 }
-template <int DH> __device__ __forceinline__ float delta_of(const Kept<float, DH>& d_o, const float* o, int h, bool ok) {
+template <int DH> __device__ __forceinline__ float delta_of(const Kept<float, DH>& d_o, const Slide& p, long at, int h, bool ok) {
+    const float* o = (const float*)p.o + at;
     float s = 0.f;
 #pragma unroll
     for (int t = 0; t < DH / 8; ++t) {
@@ -733,7 +756,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta
     const bool ok = i < length_of(p, b);
     Kept<T, DH> d_o;
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)i * p.do_n, lane >> 5, ok);
-    const float d = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + i) * p.Hq + h) * DH, lane >> 5, ok);
+    const float d = delta_of<DH>(d_o, p, (((long)b * p.N + i) * p.Hq + h) * DH, lane >> 5, ok);
     if (i < p.N && lane < 32) p.delta[((long)b * p.Hq + h) * p.N + i] = d;
 }
 
@@ -751,7 +774,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, qi < n);
     const long st = ((long)b * p.Hq + h) * p.N + qi;
     float lse = qi < n ? p.lse[st] : INFINITY;
-    float delta = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, qi < n);
+    float delta = delta_of<DH>(d_o, p, (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, qi < n);
     if (qi < p.N && lane < 32) p.delta[st] = delta;
     q.settle();
     d_o.settle();
@@ -799,7 +822,7 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
     d_o.load((const T*)p.d_o + b * p.do_b + h * p.do_h + (long)qi * p.do_n, lane >> 5, mine);
     const long st = ((long)b * p.Hq + h) * p.N + qi;
     const float lse = mine ? p.lse[st] : INFINITY;                       // not mine: probabilities of 0
-    const float delta = delta_of<DH>(d_o, p.o32 + (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, mine);
+    const float delta = delta_of<DH>(d_o, p, (((long)b * p.N + qi) * p.Hq + h) * DH, lane >> 5, mine);
     const float sc = p.scale * LOG2E;
     const Cover cover = keys_by<false>(qa, n, p.window, p.sinks);
     const Span sp = all ? keys_of<false>(qi, n, p.window, p.sinks) : Span{0, n, 0};
@@ -1324,7 +1347,7 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     if (!aligned(a->q, e, {a->q_b, a->q_n, a->q_h}) || !aligned(a->k, e, {a->k_b, a->k_n, a->k_h}) ||
         !aligned(a->v, e, {a->v_b, a->v_n, a->v_h})) return VITK_ERR_SHAPE;
     p = Slide{};
-    p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.o32 = a->o_f32; p.lse = a->lse; p.lengths = a->lengths;
+    p.q = a->q; p.k = a->k; p.v = a->v; p.o = a->o; p.rest = (int8_t*)a->o_rest; p.lse = a->lse; p.lengths = a->lengths;
     p.B = a->B; p.N = a->N; p.Hq = a->Hq; p.Hkv = a->Hkv; p.G = a->Hq / a->Hkv;
     p.q_b = a->q_b; p.q_n = a->q_n; p.q_h = a->q_h;
     p.k_b = a->k_b; p.k_n = a->k_n; p.k_h = a->k_h;
@@ -1340,11 +1363,11 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     p.scale = a->scale;
     if (!backward) {
         if (!a->o) return VITK_ERR_NULL;
-        return aligned(a->o, e, {}) && aligned(a->o_f32, 4, {}) ? 0 : VITK_ERR_SHAPE;
+        return aligned(a->o, e, {}) && aligned(a->o_rest, 1, {}) ? 0 : VITK_ERR_SHAPE;
     }
     if (!a->d_o || !a->lse || !a->delta || !a->dk != !a->dv || !(a->dq || a->dk)) return VITK_ERR_NULL;
-    if (dtype == VITK_BF16 ? !a->o_f32 : !a->o) return VITK_ERR_NULL;
-    if (!aligned(dtype == VITK_BF16 ? a->o_f32 : a->o, 4, {})) return VITK_ERR_SHAPE;
+    if (!a->o || (dtype == VITK_BF16 && !a->o_rest)) return VITK_ERR_NULL;
+    if (!aligned(a->o, e, {}) || !aligned(a->o_rest, 1, {})) return VITK_ERR_SHAPE;
     if (!aligned(a->d_o, e, {a->do_b, a->do_n, a->do_h}) || !aligned(a->dq, e, {a->dq_b, a->dq_n, a->dq_h}) ||
         !aligned(a->dk, e, {a->dk_b, a->dk_n, a->dk_h}) || !aligned(a->dv, e, {a->dv_b, a->dv_n, a->dv_h})) return VITK_ERR_SHAPE;
     p.d_o = a->d_o; p.delta = a->delta; p.dq = a->dq; p.dk = a->dk; p.dv = a->dv;
@@ -1394,7 +1417,6 @@ extern "C" int vitk_slide_attn_bwd(const vitk_slide_attn* a, int dtype, void* st
     Slide p;
     if (int e = fill(a, dtype, true, p)) return e;
     hipStream_t st = (hipStream_t)stream;
-    p.o32 = dtype == VITK_BF16 ? a->o_f32 : (float*)a->o;
 #define BWD(T, DH, C) run_bwd<T, DH, C>(p, a->workspace, st)
     SLIDE_FORMS(BWD);
 }

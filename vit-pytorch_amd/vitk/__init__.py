@@ -35,7 +35,7 @@ def _fields(text):
 
 
 class SlideAttn(ctypes.Structure):
-    _fields_ = _fields("vp: q k v o o_f32 lse lengths d_o delta dq dk dv workspace; l: q_b q_n q_h k_b k_n k_h v_b v_n v_h "
+    _fields_ = _fields("vp: q k v o o_rest lse lengths d_o delta dq dk dv workspace; l: q_b q_n q_h k_b k_n k_h v_b v_n v_h "
                        "do_b do_n do_h dq_b dq_n dq_h dk_b dk_n dk_h dv_b dv_n dv_h; i: B N Hq Hkv dh window sinks causal; f: scale")
 
 

@@ -182,12 +182,12 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _slide_args(q, k, v, o, o32, lse, lengths, meta, d_o=None, delta=None, dq=None, dk=None, dv=None):
+def _slide_args(q, k, v, o, rest, lse, lengths, meta, d_o=None, delta=None, dq=None, dk=None, dv=None):
     window, sinks, causal, scale = meta
     st = []
     for t in (q, k, v, d_o, dq, dk, dv):
         st += t.stride()[:3] if t is not None else (0, 0, 0)
-    return SlideAttn(_p(q), _p(k), _p(v), _p(o), _p(o32), _p(lse), _p(lengths), _p(d_o), _p(delta), _p(dq), _p(dk), _p(dv),
+    return SlideAttn(_p(q), _p(k), _p(v), _p(o), _p(rest), _p(lse), _p(lengths), _p(d_o), _p(delta), _p(dq), _p(dk), _p(dv),
                      None, *st, q.shape[0], q.shape[1], q.shape[2], k.shape[2], q.shape[3], window, sinks, int(causal), scale)
 
 
@@ -202,27 +202,27 @@ def _slide_workspace(a, code, backward, device):
 
 
 def _slide_forward(q, k, v, lengths, meta, keep):
-    """(o, o in 32 bits or None, lse or None): the last two are what a backward pass needs (`keep`)."""
+    """(o, what its rounding left or None, lse or None): the last two are what a backward pass needs besides o (`keep`)."""
     B, N, Hq, dh = q.shape
     o = torch.empty((B, N, Hq, dh), dtype=q.dtype, device=q.device)
-    o32 = torch.empty((B, N, Hq, dh), dtype=torch.float32, device=q.device) if keep and q.dtype != torch.float32 else None
+    rest = torch.empty((B, N, Hq, dh), dtype=torch.int8, device=q.device) if keep and q.dtype != torch.float32 else None
     lse = torch.empty((B, Hq, N), dtype=torch.float32, device=q.device) if keep else None
     if o.numel():
         with _On(q.device) as on:
-            a = _slide_args(q, k, v, o, o32, lse, lengths, meta)
+            a = _slide_args(q, k, v, o, rest, lse, lengths, meta)
             code = dtype_code(q.dtype)
             ws = _slide_workspace(a, code, False, q.device)  # noqa: F841  (lives until the launch is enqueued)
             check(lib.vitk_slide_attn_fwd(ctypes.byref(a), code, on.stream), "vitk_slide_attn_fwd")
-    return o, o32, lse
+    return o, rest, lse
 
 
-def _slide_backward(q, k, v, o, o32, lse, lengths, meta, d_o, dq, dk, dv):
+def _slide_backward(q, k, v, o, rest, lse, lengths, meta, d_o, dq, dk, dv):
     if d_o.dtype != q.dtype:
         d_o = convert(d_o, q.dtype)
     d_o = _rows(d_o)
     delta = torch.empty_like(lse)
     with _On(q.device) as on:
-        a = _slide_args(q, k, v, o, o32, lse, lengths, meta, d_o, delta, dq, dk, dv)
+        a = _slide_args(q, k, v, o, rest, lse, lengths, meta, d_o, delta, dq, dk, dv)
         code = dtype_code(q.dtype)
         ws = _slide_workspace(a, code, True, q.device)  # noqa: F841
         check(lib.vitk_slide_attn_bwd(ctypes.byref(a), code, on.stream), "vitk_slide_attn_bwd")
@@ -233,22 +233,22 @@ class SlidingAttentionFn(torch.autograd.Function):
     def forward(ctx, q, k, v, lengths, meta):
         keep = any(ctx.needs_input_grad[:3])
         q, k, v = _rows(q), _rows(k), _rows(v)
-        o, o32, lse = _slide_forward(q, k, v, lengths, meta, keep)
+        o, rest, lse = _slide_forward(q, k, v, lengths, meta, keep)
         if keep:
-            ctx.save_for_backward(q, k, v, o if o32 is None else None, o32, lse, lengths)
+            ctx.save_for_backward(q, k, v, o, rest, lse, lengths)
             ctx.meta = meta
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_o):
-        q, k, v, o, o32, lse, lengths = ctx.saved_tensors
+        q, k, v, o, rest, lse, lengths = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
         dk, dv = ((torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2)) if need_k or need_v
                   else (None, None))
         if q.numel():
-            _slide_backward(q, k, v, o, o32, lse, lengths, ctx.meta, d_o, dq, dk, dv)
+            _slide_backward(q, k, v, o, rest, lse, lengths, ctx.meta, d_o, dq, dk, dv)
         return dq, (dk if need_k else None), (dv if need_v else None), None, None
 
 
@@ -292,22 +292,22 @@ class SlidingAttentionQkvFn(torch.autograd.Function):
             with _On(x.device) as on:
                 _rope_call(x[:, :, :2 * H], qk, pos, pairs, base, interleaved, False, on)
         q, k, v = qk[:, :, :H], qk[:, :, H:2 * H], x[:, :, 2 * H:]
-        o, o32, lse = _slide_forward(q, k, v, None, meta, ctx.needs_input_grad[0])
+        o, rest, lse = _slide_forward(q, k, v, None, meta, ctx.needs_input_grad[0])
         if ctx.needs_input_grad[0]:
-            ctx.save_for_backward(qkv, qk if rope is not None else None, o if o32 is None else None, o32, lse, pos)
+            ctx.save_for_backward(qkv, qk if rope is not None else None, o, rest, lse, pos)
             ctx.meta = (shape, meta, rope[1:] if rope is not None else None)
         return o.view(B * N, -1)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_o):
-        qkv, qk, o, o32, lse, pos = ctx.saved_tensors
+        qkv, qk, o, rest, lse, pos = ctx.saved_tensors
         (B, N, H), meta, rope = ctx.meta
         x = qkv.view(B, N, 3 * H, -1)
         qk = x if qk is None else qk
         dqkv = torch.empty_like(qkv)
         g = dqkv.view(B, N, 3 * H, -1)
-        _slide_backward(qk[:, :, :H], qk[:, :, H:2 * H], x[:, :, 2 * H:], o, o32, lse, None, meta,
+        _slide_backward(qk[:, :, :H], qk[:, :, H:2 * H], x[:, :, 2 * H:], o, rest, lse, None, meta,
                         d_o.reshape(B, N, H, -1), g[:, :, :H], g[:, :, H:2 * H], g[:, :, 2 * H:])
         if rope is not None:
             pairs, base, interleaved = rope
