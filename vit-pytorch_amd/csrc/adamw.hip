@@ -38,13 +38,16 @@ static_assert(sizeof(Entry) == sizeof(vitk_adamw_entry), "table layout");
 
 struct Consts { float b1, c1, b2, c2, decay, step, root, eps; uint32_t key; };
 
-__device__ __forceinline__ double block_sum(double s) {
-    __shared__ double part[4];
+template <int WAVES> __device__ __forceinline__ double block_sum(double s) {
+    __shared__ double part[WAVES];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
     __syncthreads();
-    return (part[0] + part[1]) + (part[2] + part[3]);
+    s = part[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) s += part[w];
+    return s;
 }
 
 // A workgroup of any launch finds its tensor in `entry_of`: a search of the table is a chain of loads that a chunk of a
@@ -72,21 +75,19 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(const Entry* tab, const
         }
         for (int i = whole + threadIdx.x; i < cnt; i += 256) s += (double)g[i] * g[i];
     }
-    s = block_sum(s);
+    s = block_sum<4>(s);
     if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
-// slots[0]: the factor of every gradient.
-__global__ __launch_bounds__(256) void adamw_norm_final_kernel(const double* partial, int nb, double max_norm, double* slots, float* norm) {
-    double s = 0.0;
-    double t[8] = {};
-    for (int i = threadIdx.x; i < nb; i += 2048) {
+// slots[0]: the factor of every gradient.  One workgroup, every partial sum in flight at once.
+__global__ __launch_bounds__(1024) void adamw_norm_final_kernel(const double* partial, int nb, double max_norm, double* slots, float* norm) {
+    constexpr int EACH = PARTIALS / 1024;
+    double t[EACH] = {}, s = 0.0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (i + k * 256 < nb) t[k] += partial[i + k * 256];
-    }
+    for (int k = 0; k < EACH; ++k)
+        if ((int)threadIdx.x + k * 1024 < nb) t[k] = partial[threadIdx.x + k * 1024];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s += t[k];
-    s = block_sum(s);
+    for (int k = 0; k < EACH; ++k) s += t[k];
+    s = block_sum<16>(s);
     if (threadIdx.x == 0) {
         s = sqrt(s);
         const double r = max_norm / (s + 1e-6);
@@ -289,7 +290,7 @@ extern "C" int vitk_adamw_norm(const void* table, const int* entry_of, int n_blo
     const int nb = n_blocks < PARTIALS ? n_blocks : PARTIALS;
     hipLaunchKernelGGL(adamw_norm_kernel, dim3(nb), dim3(256), 0, st, (const Entry*)table, entry_of, n_blocks, slots + 1);
     VITK_CHECK_LAUNCH();
-    hipLaunchKernelGGL(adamw_norm_final_kernel, dim3(1), dim3(256), 0, st, slots + 1, nb, max_norm, slots, norm);
+    hipLaunchKernelGGL(adamw_norm_final_kernel, dim3(1), dim3(1024), 0, st, slots + 1, nb, max_norm, slots, norm);
     VITK_CHECK_LAUNCH();
     return 0;
 }
