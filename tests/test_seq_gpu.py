@@ -284,10 +284,11 @@ def test_gradients_against_differences():
             assert abs(diff - want) <= 1e-3 * scale, (causal, at, diff, want)
 
 
+@pytest.mark.parametrize("Hkv,dh", [(2, 64), (1, 128)])
 @pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
-def test_captured_training_pass_replays(dt):
+def test_captured_training_pass_replays(dt, Hkv, dh):
     from vitk import ops
-    q, k, v, d_o = _case(dt, B=1, N=190)
+    q, k, v, d_o = _case(dt, B=1, N=190, Hkv=Hkv, dh=dh)
     static = [t.clone().requires_grad_(True) for t in (q, k, v)]
     sd = d_o.clone()
     kw = dict(window=25, sinks=2, causal=False)
