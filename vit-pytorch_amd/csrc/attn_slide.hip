@@ -17,7 +17,8 @@
 // causal mask they look at every key.  The workgroup of a tile therefore handles the tile's BAND only (its window and, for
 // ordinary rows, the few first tokens on the other side), and what the first tokens see beyond their band is cut into
 // chunks of FAR items: 32 first tokens against a share of the far rows, dealt out to four waves that meet in LDS.
-// Bands and chunks of a first token leave 32-bit records in a workspace, which a last small launch adds in a fixed order.
+// Bands and chunks of a first token leave 32-bit records in a workspace, which a last small launch adds in a fixed order; so do the
+// workgroups that share a band of keys in the backward pass of few key heads.
 // Where the whole sequence is not much longer than a band, one item does all of 32 first tokens and nothing is left to add.
 // (Without the split the backward pass of 16384 causal tokens of the sizes below takes 663 us instead of 281.)
 //
