@@ -98,7 +98,7 @@ ATTN = [  # (B, N, Hq, Hkv, dh, causal, window, sinks, lengths)
     (1, 700, 5, 1, 64, True, 128, 4, None), (1, 1025, 1, 1, 64, False, 65, 33, (999,)),
     # few key heads, many queries a key: several workgroups to a band of keys
     (2, 700, 8, 1, 64, False, 150, 3, (700, 90)), (1, 150, 8, 1, 32, False, 100, 4, None), (2, 390, 12, 2, 128, True, None, 0, (390, 0)),
-    (1, 520, 16, 1, 128, True, 100, 40, (333,)), (1, 1500, 2, 1, 64, True, None, 0, None), (1, 260, 20, 1, 128, False, 70, 2, None)]
+    (1, 520, 16, 1, 128, True, 100, 40, (333,)), (1, 4100, 4, 1, 32, True, 1, 2, None), (1, 1500, 2, 1, 64, True, None, 0, None), (1, 260, 20, 1, 128, False, 70, 2, None)]
 
 
 @pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
