@@ -369,13 +369,46 @@ template <typename T, int DH> __device__ __forceinline__ void put(T* row, const 
             Vec4<T>::store(row + 32 * d + 8 * b + 4 * (lane >> 5), x);
         }
 }
+// LDS written by other lanes of this wave may be read behind it (a wave's LDS accesses take effect in order).
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 // What rounding x to bf16 left, in units of 1/256 of the last place: with it an output has 15 bits behind the leading one, in
 // 8 bits more of memory (o in 32 bits beside it: 16384-token training pass 383 us, so 379, and 3 bytes an element more kept).
 __device__ __forceinline__ int rest_of(float x) {
     const int r = (int)(__float_as_uint(x) - ((unsigned)__builtin_bit_cast(unsigned short, (bf16_t)x) << 16));
     return least((r + 128) >> 8, 127);
 }
-template <int DH> __device__ __forceinline__ void put_rest(int8_t* row, const f32x16* acc, float mul, int lane) {
+// The wave's 32 rows, `ld` elements apart, the first `count` of them, through its LDS tile `via`: a lane's elements of a row are 4 here
+// and 4 there, and rows written from registers cost the address units a line for each of them (8 images of 2305 tokens, what a forward pass
+// for training writes: 60.8 -> 55.2 us; backward 164 -> 160).
+template <int DH> __device__ __forceinline__ void put_rows(char* via, bf16_t* rows, long ld, int count, const f32x16* acc, float mul, int lane) {
+    using S = Shape<bf16_t, DH>;
+#pragma unroll
+    for (int d = 0; d < DH / 32; ++d)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            bf16x4 x;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = (bf16_t)(acc[d][4 * b + e] * mul);
+            *reinterpret_cast<bf16x4*>(via + S::at(lane & 31, 4 * d + b) + 8 * (lane >> 5)) = x;
+        }
+    wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < 32 * S::CHUNKS / 64; ++i) {
+        const int idx = lane + i * 64, r = idx / S::CHUNKS, c = idx % S::CHUNKS;
+        if (r < count) *reinterpret_cast<u32x4*>(rows + r * ld + 8 * c) = *reinterpret_cast<const u32x4*>(via + S::at(r, c));
+    }
+    wave_lds_fence();
+}
+template <int DH> __device__ __forceinline__ void put_rows(char*, float* rows, long ld, int count, const f32x16* acc, float mul, int lane) {
+    if ((lane & 31) < count) put<float, DH>(rows + (lane & 31) * ld, acc, mul, lane);
+}
+// The same of what their rounding left.
+template <int DH> __device__ __forceinline__ void put_rest(char* via, int8_t* rows, long ld, int count, const f32x16* acc, float mul, int lane) {
+    constexpr int CHUNKS = DH / 16;
+    const auto at = [](int r, int c) { return r * DH + ((c ^ ((r >> 2) & (CHUNKS - 1))) << 4); };
 #pragma unroll
     for (int d = 0; d < DH / 32; ++d)
 #pragma unroll
@@ -383,17 +416,18 @@ template <int DH> __device__ __forceinline__ void put_rest(int8_t* row, const f3
             unsigned x = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x |= (unsigned)(rest_of(acc[d][4 * b + e] * mul) & 255) << (8 * e);
-            *reinterpret_cast<unsigned*>(row + 32 * d + 8 * b + 4 * (lane >> 5)) = x;
+            *reinterpret_cast<unsigned*>(via + at(lane & 31, 2 * d + (b >> 1)) + 8 * (b & 1) + 4 * (lane >> 5)) = x;
         }
+    wave_lds_fence();
+#pragma unroll
+    for (int i = 0; i < 32 * CHUNKS / 64; ++i) {
+        const int idx = lane + i * 64, r = idx / CHUNKS, c = idx % CHUNKS;
+        if (r < count) *reinterpret_cast<u32x4*>(rows + r * ld + 16 * c) = *reinterpret_cast<const u32x4*>(via + at(r, c));
+    }
 }
 // What the sums of dQ and dK are multiplied with.  A query that sees one key only has the probability 1 whatever its score:
 // where all do, the gradients of the scores are exactly 0, and not what dP - delta leaves after rounding.
 __device__ __forceinline__ float score_scale(const Slide& p, int n) { return p.single || n == 1 ? 0.f : p.scale; }
-// LDS written by other lanes of this wave may be read behind it (a wave's LDS accesses take effect in order).
-__device__ __forceinline__ void wave_lds_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
 __device__ __forceinline__ int length_of(const Slide& p, int b) {
     if (!p.lengths) return p.N;
     const int n = p.lengths[b];
@@ -508,9 +542,9 @@ template <int DH, int NW, typename F> __device__ __forceinline__ void add_waves(
 
 // Tiles of two matrices through LDS, two buffers deep: while one tile is used, the next one is on its way, and one
 // barrier a tile orders the two.  use(first tile, second tile, first row); ready() waits for what the loop keeps with the first
-// tiles on their way (forward, 1024 tokens of 8 heads: 15.9 -> 15.1 us; in the backward kernels it gained nothing).
+// tiles on their way.  Returns the buffer that no wave reads any more (forward, 1024 tokens of 8 heads: 15.9 -> 15.1 us; in the backward kernels it gained nothing).
 template <typename T, int DH, typename R, typename F>
-__device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T* B, long ldb, const Tiles& tl, int n, int tid, R ready, F use) {
+__device__ __forceinline__ char* stream(char* lds, const T* A, long lda, const T* B, long ldb, const Tiles& tl, int n, int tid, R ready, F use) {
     using S = Shape<T, DH>;
     constexpr int BYTES = S::KT * S::ROW;
     const Stage<T, DH> fa(lda, tid), fb(ldb, tid);
@@ -531,6 +565,7 @@ __device__ __forceinline__ void stream(char* lds, const T* A, long lda, const T*
         }
         use(now, now + BYTES, tl.at(t) * S::KT);
     }
+    return lds + (cnt & 1) * 2 * BYTES;
 }
 // 32 rows from r0 of a matrix into an LDS tile of this wave alone.
 template <typename T, int DH> __device__ __forceinline__ void start_wave(char* tile, const T* base, long ld, int r0, int n, int lane) {
@@ -579,7 +614,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
     };
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&] { q.settle(); }, [&](const char* Ks, const char* Vs, int k0) {
+    char* via = stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [&] { q.settle(); }, [&](const char* Ks, const char* Vs, int k0) {
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
@@ -592,20 +627,21 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         }
     });
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
-    if (qi < p.N && !elsewhere) {
-        if (!CAUSAL && qi < p.rows) {
-            float* rec = p.ws + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * (DH + 4);
-            put<float, DH>(rec, acc, 1.f, lane);
-            if (lane < 32) { rec[DH] = m; rec[DH + 1] = l; }
-            return;
-        }
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const long row = ((long)b * p.N + qi) * p.Hq + h;
-        put<T, DH>((T*)p.o + row * DH, acc, inv, lane);
-        if (sizeof(T) == 2 && p.rest) put_rest<DH>(p.rest + row * DH, acc, inv, lane);
-        // base-2 logarithm of the row's sum; +inf for a row that sees nothing, so that backward's probabilities are 0
-        if (p.lse && lane < 32) p.lse[((long)b * p.Hq + h) * p.N + qi] = l > 0.f ? m + __log2f(l) : INFINITY;
+    if (elsewhere) return;
+    if (!CAUSAL && qa < p.rows) {
+        float* rec = p.ws + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * (DH + 4);
+        if (qi >= p.N) return;
+        put<float, DH>(rec, acc, 1.f, lane);
+        if (lane < 32) { rec[DH] = m; rec[DH + 1] = l; }
+        return;
     }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const long row = ((long)b * p.N + qa) * p.Hq + h, ld = (long)p.Hq * DH;
+    via += wave * 32 * S::ROW;
+    put_rows<DH>(via, (T*)p.o + row * DH, ld, p.N - qa, acc, inv, lane);
+    if (sizeof(T) == 2 && p.rest) put_rest<DH>(via, p.rest + row * DH, ld, p.N - qa, acc, inv, lane);
+    // base-2 logarithm of the row's sum; +inf for a row that sees nothing, so that backward's probabilities are 0
+    if (p.lse && lane < 32 && qi < p.N) p.lse[((long)b * p.Hq + h) * p.N + qi] = l > 0.f ? m + __log2f(l) : INFINITY;
 }
 // Far: 32 first queries against every (4 chunks)-th 32 keys behind their band; or, without chunks, against all they see.
 template <typename T, int DH>
@@ -787,7 +823,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     const Cover cover = keys_by<CAUSAL>(qa, n, p.window, p.sinks);
     f32x16 acc[DH / 32] = {};
     const Tiles tl = key_tiles<CAUSAL>(q0, q0 + TQ - 1, n, p.window, p.sinks, S::KT);
-    stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [] {}, [&](const char* Ks, const char* Vs, int k0) {
+    char* via = stream<T, DH>(lds, K, p.k_n, V, p.v_n, tl, n, tid, [] {}, [&](const char* Ks, const char* Vs, int k0) {
 #pragma unroll
         for (int sub = 0; sub < S::KT; sub += 32) {
             const int ka = k0 + sub;
@@ -801,11 +837,12 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
             gather<DH>(acc, Ks, sub, s, lane, T{});
         }
     });
-    if (qi >= p.N || elsewhere) return;
-    if (!CAUSAL && qi < p.rows)
+    if (elsewhere) return;
+    if (CAUSAL || qa >= p.rows)
+        put_rows<DH>(via + wave * 32 * S::ROW, (T*)p.dq + b * p.dq_b + (long)qa * p.dq_n + h * p.dq_h, p.dq_n, p.N - qa, acc,
+                     qi < n ? score_scale(p, n) : 0.f, lane);
+    else if (qi < p.N)
         put<float, DH>(p.ws_q + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * DH, acc, 1.f, lane);
-    else
-        put<T, DH>((T*)p.dq + b * p.dq_b + (long)qi * p.dq_n + h * p.dq_h, acc, qi < n ? score_scale(p, n) : 0.f, lane);
 }
 template <typename T, int DH>
 __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, int b, int n) {
@@ -997,15 +1034,25 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
         meet(dv);
         if (part) return;
     }
-    if (kj >= p.N || elsewhere) return;
-    if (kj < p.rows || p.shares > 1) {
+    if (elsewhere) return;
+    if (ka < p.rows || p.shares > 1) {
+        if (kj >= p.N) return;
         float* rec = p.shares > 1 ? p.ws_b + ((((long)b * p.Hkv + hk) * p.N + kj) * p.shares + share) * (2 * DH)
                                   : p.ws + ((((long)b * p.Hkv + hk) * p.rows + kj) * (p.chunks + 1) + p.chunks) * (2 * DH);
         put<float, DH>(rec, dk, 1.f, lane);
         put<float, DH>(rec + DH, dv, 1.f, lane);
     } else {
-        put<T, DH>((T*)p.dk + b * p.dk_b + (long)kj * p.dk_n + hk * p.dk_h, dk, kj < n ? score_scale(p, n) : 0.f, lane);
-        put<T, DH>((T*)p.dv + b * p.dv_b + (long)kj * p.dv_n + hk * p.dv_h, dv, kj < n ? 1.f : 0.f, lane);
+        T* K_to = (T*)p.dk + b * p.dk_b + hk * p.dk_h;
+        T* V_to = (T*)p.dv + b * p.dv_b + hk * p.dv_h;
+        const float by_k = kj < n ? score_scale(p, n) : 0.f, by_v = kj < n ? 1.f : 0.f;
+        if constexpr (L::PARTS == 1) {
+            char* via = lds + (cnt & 1) * L::BUF + wave * 32 * S::ROW;                  // no wave reads this buffer any more
+            put_rows<DH>(via, K_to + (long)ka * p.dk_n, p.dk_n, p.N - ka, dk, by_k, lane);
+            put_rows<DH>(via, V_to + (long)ka * p.dv_n, p.dv_n, p.N - ka, dv, by_v, lane);
+        } else if (kj < p.N) {          // half of the waves: the other way gained nothing here
+            put<T, DH>(K_to + (long)kj * p.dk_n, dk, by_k, lane);
+            put<T, DH>(V_to + (long)kj * p.dv_n, dv, by_v, lane);
+        }
     }
 }
 // Far: 32 first keys against every (NW chunks)-th 32 queries behind their band, of every head that shares them.
