@@ -22,12 +22,12 @@
 // Where the whole sequence is not much longer than a band, one item does all of 32 first tokens and nothing is left to add.
 // (Without the split the backward pass of 16384 causal tokens of the sizes below takes 663 us instead of 281.)
 //
-// Measured in bf16, rates of the pairs that are visible (4 dh operations each forward, 6 for dQ, 8 for dK / dV):
-//   8 x 2305 x 12 x 64, all visible:            forward 186 us (702 TFLOP/s), dQ 229 (854), dK / dV 319 (818)
-//   1 x 16384 x 8 of 2 x 128, causal, window 1024:     87 us (769),               112 (888),          187 (712)
-//   8 x 2305 x 12 x 64, window 145, 1 first token:     53 us (299),                75 (315),          114 (279)
-// In the last, whose band is little longer than its rows, 113 MB forward and 353 MB backward are half of the time at the rate of
-// a copy.
+// Measured in bf16, training, rates of the pairs that are visible (4 dh operations each forward, 6 for dQ, 8 for dK / dV):
+//   8 x 2305 x 12 x 64, all visible:            forward 191 us (683 TFLOP/s), dQ 230 (850), dK / dV 320 (815)
+//   1 x 16384 x 8 of 2 x 128, causal, window 1024:     89 us (747),               113 (880),          185 (720)
+//   8 x 2305 x 12 x 64, window 145, 1 first token:     55 us (288),                77 (308),          113 (280)
+// In the last, whose band is little longer than its rows, 127 MB forward and 353 MB backward are 0.4 of the time at the rate of a
+// copy.
 #include <initializer_list>
 
 #include "common.h"
