@@ -358,7 +358,8 @@ DECODE = [  # (B, cap, Hq, Hkv, dh, window, sinks, lengths)
     (1, 1, 1, 1, 64, 1, 0, (1,)), (3, 40, 4, 2, 64, 8, 3, (0, 1, 40)), (2, 33, 2, 2, 32, 100, 0, (33, 32)),
     (2, 300, 6, 1, 128, 65, 40, (299, 50)), (1, 1000, 40, 1, 64, 512, 4, (1000,)), (2, 1000, 8, 8, 64, None, 0, (1000, 31)),
     (2, 129, 3, 3, 64, 0, 5, (129, 2)), (2, 64, 2, 2, 64, 0, 0, (64, 64)), (1, 2050, 2, 2, 128, 1500, 700, (2050,)),
-    (5, 97, 35, 5, 32, 31, 31, (97, 96, 62, 61, 33)), (1, 9000, 2, 1, 64, 8000, 33, (8999,))]
+    (5, 97, 35, 5, 32, 31, 31, (97, 96, 62, 61, 33)), (1, 9000, 2, 1, 64, 8000, 33, (8999,)),
+    (1, 5000, 3, 1, 32, None, 2, (4990,)), (3, 3000, 40, 1, 64, 2500, 4, (3000, 17, 0))]
 
 
 @pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])

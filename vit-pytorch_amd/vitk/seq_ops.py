@@ -339,16 +339,22 @@ def sliding_attention_qkv(qkv, B, N, H, window, sinks=0, causal=False, scale=Non
 _CUS = {}         # compute units of each device
 
 
-def _splits(B, Hkv, G, window, sinks, esz, device):
-    """Workgroups that share the keys of one (sequence, key head): one workgroup a CU in all, none with fewer than 32 keys a
-    wave.  One stream of 65536 tokens, 8 key heads of 128: 488 us unsplit, 51 us with 32 each; 256 (sequence, head) pairs of
-    8192 keys: 190 us unsplit or halved, 206 us in eighths."""
+def _splits(B, Hkv, G, window, sinks, dh, esz, device):
+    """Workgroups that share the keys of one (sequence, key head): as many as give each CU one in all, none with fewer than 32
+    keys a wave.  One stream of 65536 tokens, 8 key heads of 128: 488 us unsplit, 51 us with 32 each; 12 heads of 64, 16384
+    tokens: 97 us unsplit, 16.7 us with 21 each, 19.4 with 22, which is more than there are CUs.
+    One workgroup alone while its waves have no more than 20 KB of keys each: a second launch and its workspace cost a call more
+    than the shares save (1024 keys of 64 elements, 12 heads: 12.9 us a call, 7.7 us replayed from a graph; shared by 5, 17.5
+    and 6.5)."""
     cus = _CUS.get(device.index)
     if cus is None:
         cus = _CUS[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
     groups = B * Hkv * ((G + 31) // 32)
     tiles = -(-window // 32) + -(-sinks // 32)
-    return max(1, min(-(-tiles // (8 if esz == 2 else 4)), -(-cus // groups), 64))
+    turns = -(-tiles // (8 if esz == 2 else 4))
+    if turns * 32 * dh * esz <= 20 * 1024:
+        return 1
+    return max(1, min(turns, cus // groups, 64))
 
 
 def sliding_attention_decode(q, k_cache, v_cache, lengths, window, sinks=0, scale=None):
@@ -373,7 +379,7 @@ def sliding_attention_decode(q, k_cache, v_cache, lengths, window, sinks=0, scal
     q, k, v = _rows(q), _rows(k_cache), _rows(v_cache)
     with _On(q.device) as on:
         o = torch.empty((B, Hq, dh), dtype=q.dtype, device=q.device)
-        splits = _splits(B, Hkv, Hq // Hkv, window, sinks, q.element_size(), q.device)
+        splits = _splits(B, Hkv, Hq // Hkv, window, sinks, dh, q.element_size(), q.device)
         ws = torch.empty(B * Hq * splits * (dh + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
         a = SlideCache(_p(q), _p(k), _p(v), _p(o), _p(lengths), _p(ws), *q.stride()[:2], *k.stride()[:3], *v.stride()[:3],
                        B, cap, Hq, Hkv, dh, window, sinks, splits, scale)
