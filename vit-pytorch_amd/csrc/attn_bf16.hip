@@ -126,8 +126,10 @@ __device__ __forceinline__ void fwd_update(FwdState& st, const Scores& sc_in, co
         }
     }
     // (v_max3 from assembly: fmaxf() makes the compiler quiet every input first, one more instruction per value;
-    // the values are MFMA results or -inf, never signalling NaNs)
-    float tmax = max3_raw(max3_raw(sv[0], sv[1], sv[2]), max3_raw(sv[3], sv[4], sv[5]), max3_raw(sv[6], sv[7], sv[7]));
+    // the values are MFMA results or -inf, never signalling NaNs.  The compiler does not wait for a matrix instruction's
+    // result in front of assembly: instructions of its own read both results first.)
+    const float t0 = max3_raw(sv[0] + 0.f, sv[4] + 0.f, sv[1]);
+    float tmax = max3_raw(max3_raw(t0, sv[2], sv[3]), max3_raw(t0, sv[5], sv[6]), sv[7]);
     tmax = max3_raw(tmax, __shfl_xor(tmax, 16, 64), tmax);
     tmax = max3_raw(tmax, __shfl_xor(tmax, 32, 64), tmax);
     const float mn = max3_raw(st.m, tmax, tmax);  // finite: the first tile of a row holds >= 1 valid key
