@@ -255,15 +255,19 @@ template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, in
     return acc;
 }
 // acc[d][column] += sum over 32 tile rows from r0 of tile[row][d] * w[row][column]; w as a product left it.  In bf16
-// the weights are rounded to the operand type here: 2^-9 of each, independent, and the sums stay in 32 bits.
-template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, bf16_t) {
+// the weights are rounded to the operand type here: 2^-9 of each, independent, and the sums stay in 32 bits; FINE: what
+// that leaves of them is a second operand.
+template <int DH, bool FINE = false> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, bf16_t) {
     using S = Shape<bf16_t, DH>;
     const int l15 = lane & 15, g = lane >> 4;
-    bf16x8 b[2];
+    bf16x8 b[2], rest[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[c][e] = (bf16_t)w[8 * c + e];
+        for (int e = 0; e < 8; ++e) {
+            b[c][e] = (bf16_t)w[8 * c + e];
+            if constexpr (FINE) rest[c][e] = (bf16_t)(w[8 * c + e] - (float)b[c][e]);
+        }
     // the transposing read takes 8 bytes of rows r ... r + 3 from each 16 lanes
     const int r = 4 * (g >> 1) + (l15 >> 2), ch = 2 * (g & 1) + ((l15 & 3) >> 1), half = (l15 & 1) * 8;
     const int a0 = S::at(r, ch) + half, a1 = S::at(r + 8, ch) + half;
@@ -275,13 +279,14 @@ template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char
             const char* t = tile + 16 * c * S::ROW;
             const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((VITK_LDS bf16x4*)(t + (a0 ^ (d << 6))));
             const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((VITK_LDS bf16x4*)(t + (a1 ^ (d << 6))));
-            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]},
-                                                             b[c], acc[d], 0, 0, 0);
+            const bf16x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b[c], acc[d], 0, 0, 0);
+            if constexpr (FINE) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, rest[c], acc[d], 0, 0, 0);
         }
     }
-    reads_ahead<DH / 16, 2>();
+    if constexpr (!FINE) reads_ahead<DH / 16, 2>();
 }
-template <int DH> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, float) {
+template <int DH, bool FINE = false> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, float) {
     using S = Shape<float, DH>;
     const int ch = (lane & 31) >> 2, low = (lane & 3) * 4;
     tile += r0 * S::ROW;
@@ -799,7 +804,7 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta
 
 // dQ of a band: as the forward pass, with a second product of the same shape for dP and the deltas on the way (a kernel of its
 // own for them cost 20 us of the 250 of a training pass).  Matrix cores busy 51 % of the cycles, vector pipes 61 %.
-template <typename T, int DH, bool CAUSAL>
+template <typename T, int DH, bool CAUSAL, bool FINE>
 __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
@@ -834,7 +839,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
             if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, 0.f);      // of hidden pairs it may be infinite
-            gather<DH>(acc, Ks, sub, s, lane, T{});
+            gather<DH, FINE>(acc, Ks, sub, s, lane, T{});
         }
     });
     if (elsewhere) return;
@@ -844,7 +849,7 @@ __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h
     else if (qi < p.N)
         put<float, DH>(p.ws_q + ((((long)b * p.Hq + h) * p.rows + qi) * (p.chunks + 1) + p.chunks) * DH, acc, 1.f, lane);
 }
-template <typename T, int DH>
+template <typename T, int DH, bool FINE>
 __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, int b, int n) {
     using S = Shape<T, DH>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
@@ -879,7 +884,7 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
         hide(s, sp, k0 + 4 * (lane >> 5), k0 < p.sinks, 0.f);
-        gather<DH>(acc, Ks, 0, s, lane, T{});
+        gather<DH, FINE>(acc, Ks, 0, s, lane, T{});
         wave_lds_fence();
     }
     add_waves<DH, 4>(lds, acc, tid, [&](int c, int d, float sum) {
@@ -888,21 +893,21 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
         else if (i < p.N) ((T*)p.dq)[b * p.dq_b + (long)i * p.dq_n + h * p.dq_h + d] = (T)(i < n ? sum * score_scale(p, n) : 0.f);
     });
 }
-template <typename T, int DH, bool CAUSAL>
+template <typename T, int DH, bool CAUSAL, bool FINE>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void slide_dq_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
     const Item it = item_of(p, p.Hq, (p.N + TQ - 1) / TQ);
     if (it.none) return;
     const int n = length_of(p, it.b);
     if constexpr (!CAUSAL)
-        if (it.far) return dq_far<T, DH>(p, lds, it.x, it.h, it.b, n);
-    dq_band<T, DH, CAUSAL>(p, lds, it.x * TQ, it.h, it.b, n);
+        if (it.far) return dq_far<T, DH, FINE>(p, lds, it.x, it.h, it.b, n);
+    dq_band<T, DH, CAUSAL, FINE>(p, lds, it.x * TQ, it.h, it.b, n);
 }
 
 // 32 x 32 scores, their probabilities and score gradients, and what they add to dV and dK: rows of the tile are queries,
 // columns keys; lse, delta: the rows' (the second product starts from the negative delta).  x0: the query of the tile's
 // first row for this lane's half, for `masked` tiles.
-template <typename T, int DH, typename K>
+template <typename T, int DH, bool FINE, typename K>
 __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const float* lse, const float* delta, int sub,
                                          const K& k, const K& v, f32x16* dk, f32x16* dv, float sc, int lane,
                                          bool masked, const Span& sp, int x0, bool first) {
@@ -916,7 +921,7 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const f
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] *= s[r];
     gather<DH>(dv, Os, sub, s, lane, T{});
-    gather<DH>(dk, Qs, sub, dp, lane, T{});
+    gather<DH, FINE>(dk, Qs, sub, dp, lane, T{});
 }
 // How a workgroup of the dK / dV kernel is laid out: NW waves, 32 KG keys; wave w keeps keys 32 (w % KG) and takes every
 // (NW / KG)-th 32 queries, and the parts are added at the end.  Four waves of 32 keys each where there are enough of them;
@@ -951,7 +956,7 @@ template <typename T, int DH, int NT> __device__ __forceinline__ void keep_rows(
 // Band: the queries of every head that shares the keys stream through LDS, so that dK and dV are sums of one workgroup and need no
 // atomics.  Matrix cores busy 47 % of the cycles, vector pipes 41 %, LDS 36 %: four products read a tile in two
 // orders, and the registers of two sums leave two waves a SIMD to hide one in the other.
-template <typename T, int DH, bool CAUSAL, int NW, int KG>
+template <typename T, int DH, bool CAUSAL, int NW, int KG, bool FINE>
 __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int share, int hk, int b, int n) {
     using S = Shape<T, DH>;
     using L = Layout<T, DH, NW, KG>;
@@ -1015,7 +1020,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
             if (cov == 0 || elsewhere) continue;
             const int x0 = qa + 4 * (lane >> 5);
             const bool first = !CAUSAL && qa < p.sinks;
-            dkv_tile<T, DH>(now, now + L::TILE, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1, sp, x0, first);
+            dkv_tile<T, DH, FINE>(now, now + L::TILE, Ls, Ls + S::KT, sub, k, v, dk, dv, sc, lane, cov == 1, sp, x0, first);
         }
     }
     if constexpr (L::PARTS == 2) {
@@ -1056,7 +1061,7 @@ __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int 
     }
 }
 // Far: 32 first keys against every (NW chunks)-th 32 queries behind their band, of every head that shares them.
-template <typename T, int DH, bool CAUSAL, int NW, int KG>
+template <typename T, int DH, bool CAUSAL, int NW, int KG, bool FINE>
 __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk, int b, int n) {
     using S = Shape<T, DH>;
     using L = Layout<T, DH, NW, KG>;
@@ -1100,7 +1105,7 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
         Ls[lane] = (lane < 32 ? p.lse : p.delta)[st + (q0 + r < n ? r : n - 1 - q0)];
         dma_wait();
         wave_lds_fence();
-        dkv_tile<T, DH>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, sp, q0 + 4 * (lane >> 5), !CAUSAL && q0 < p.sinks);
+        dkv_tile<T, DH, FINE>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, sp, q0 + 4 * (lane >> 5), !CAUSAL && q0 < p.sinks);
         wave_lds_fence();
     }
     const auto leave = [&](f32x16* acc, bool values) {
@@ -1117,16 +1122,16 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
     leave(dk, false);
     leave(dv, true);
 }
-template <typename T, int DH, bool CAUSAL, int NW, int KG>
+template <typename T, int DH, bool CAUSAL, int NW, int KG, bool FINE>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && (DH < 128 || NW == 8) ? 2 : 1) void slide_dkv_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
     const Item it = item_of(p, p.Hkv, (p.N + 32 * KG - 1) / (32 * KG) * p.shares);
     if (it.none) return;
     const int n = length_of(p, it.b);
-    if (it.far) dkv_far<T, DH, CAUSAL, NW, KG>(p, lds, it.x, it.h, it.b, n);
+    if (it.far) dkv_far<T, DH, CAUSAL, NW, KG, FINE>(p, lds, it.x, it.h, it.b, n);
     else {
         const int band = p.shares > 1 ? it.x / p.shares : it.x;
-        dkv_band<T, DH, CAUSAL, NW, KG>(p, lds, band * (32 * KG), it.x - band * p.shares, it.h, it.b, n);
+        dkv_band<T, DH, CAUSAL, NW, KG, FINE>(p, lds, band * (32 * KG), it.x - band * p.shares, it.h, it.b, n);
     }
 }
 // Records become gradients.  Of the keys that are first tokens: their far items' and the band's; of all keys, where shares of
@@ -1304,11 +1309,11 @@ template <typename T, int DH> constexpr int lds_bytes(bool far) {      // of the
     const int joined = join_bytes<DH>(), wide = staged > joined ? staged : joined;
     return far && wide > band ? wide : band;
 }
-template <typename T, int DH, bool CAUSAL, int NW, int KG> int launch_dkv(Slide& p, hipStream_t st) {
+template <typename T, int DH, bool CAUSAL, int NW, int KG, bool FINE> int launch_dkv(Slide& p, hipStream_t st) {
     const int bytes = Layout<T, DH, NW, KG>::bytes(p.rows > 0);
-    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, NW, KG>, bytes)) return e;
+    if (int e = allow_lds(slide_dkv_kernel<T, DH, CAUSAL, NW, KG, FINE>, bytes)) return e;
     const unsigned grid = grid_of(p, p.Hkv, p.rows > 0, 32 * KG, p.shares);
-    hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, NW, KG>), dim3(grid), dim3(NW * 64), bytes, st, p);
+    hipLaunchKernelGGL((slide_dkv_kernel<T, DH, CAUSAL, NW, KG, FINE>), dim3(grid), dim3(NW * 64), bytes, st, p);
     VITK_CHECK_LAUNCH();
     return 0;
 }
@@ -1329,13 +1334,13 @@ template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipSt
     }
     return 0;
 }
-template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipStream_t st) {
+template <typename T, int DH, bool CAUSAL, bool FINE> int run_bwd(Slide p, float* ws, hipStream_t st) {
     const Records rk = records_of(p.B, p.N, p.Hkv, p.G, 2 * DH, p.window, p.sinks, dkv_waves(sizeof(T) == 2, DH));
     const Bands bands = bands_of(p.B, p.N, p.Hkv, p.G, CAUSAL, p.window, sizeof(T) == 2, DH);
     const Records rq = CAUSAL ? Records{0, 0, 0} : records_of(p.B, p.N, p.Hq, 1, DH, p.window, p.sinks, 4);
     if (rk.floats + bands.floats + rq.floats && !ws) return VITK_ERR_NULL;
     const int bytes = lds_bytes<T, DH>(rq.rows > 0);
-    if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL>, bytes)) return e;
+    if (int e = allow_lds(slide_dq_kernel<T, DH, CAUSAL, FINE>, bytes)) return e;
     p.ws = ws;
     p.ws_b = ws + rk.floats;
     p.ws_q = p.ws_b + bands.floats;
@@ -1343,7 +1348,7 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipSt
     if (p.dq) {
         p.rows = rq.rows; p.chunks = rq.chunks;
         const unsigned grid = grid_of(p, p.Hq, rq.rows > 0);
-        hipLaunchKernelGGL((slide_dq_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
+        hipLaunchKernelGGL((slide_dq_kernel<T, DH, CAUSAL, FINE>), dim3(grid), dim3(256), bytes, st, p);
     } else {
         hipLaunchKernelGGL((slide_delta_kernel<T, DH>), dim3(vitk_ceil_div(p.N, TQ), p.Hq, p.B), dim3(256), 0, st, p);
     }
@@ -1351,9 +1356,9 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipSt
     if (p.dk) {
         p.rows = rk.rows; p.chunks = rk.chunks;
         int e;
-        if constexpr (dkv_waves(sizeof(T) == 2, DH) == 8) e = launch_dkv<T, DH, CAUSAL, 8, 4>(p, st);
-        else if (bands.groups == 2) e = launch_dkv<T, DH, CAUSAL, 4, 2>(p, st);
-        else e = launch_dkv<T, DH, CAUSAL, 4, 4>(p, st);
+        if constexpr (dkv_waves(sizeof(T) == 2, DH) == 8) e = launch_dkv<T, DH, CAUSAL, 8, 4, FINE>(p, st);
+        else if (bands.groups == 2) e = launch_dkv<T, DH, CAUSAL, 4, 2, FINE>(p, st);
+        else e = launch_dkv<T, DH, CAUSAL, 4, 4, FINE>(p, st);
         if (e) return e;
     }
     const int first = rk.rows < p.N ? rk.rows : p.N;
@@ -1367,6 +1372,16 @@ template <typename T, int DH, bool CAUSAL> int run_bwd(Slide p, float* ws, hipSt
         VITK_CHECK_LAUNCH();
     }
     return 0;
+}
+// bf16 score gradients go into their products as two numbers each where a window holds few keys: with one, dQ and dK are off by
+// 0.0024 of their norm (of a result rounded once 0.0017), and by 0.0025 and more in rows of a few keys, where the deltas' own error has
+// nothing to average over; with two by 0.0017 to 0.0019.  8 x 2305 x 12 x 64, backward: window 1 64.5 us and 65.4, window 17 85 us and
+// 91; at a window of 145 it would be 125 us and 146.
+constexpr int FINE_WINDOW = 16;
+template <typename T, int DH, bool CAUSAL> int run_bwd(const Slide& p, float* ws, hipStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (p.window <= FINE_WINDOW) return run_bwd<T, DH, CAUSAL, true>(p, ws, st);
+    return run_bwd<T, DH, CAUSAL, false>(p, ws, st);
 }
 template <typename T, int DH> int run_decode(const Decode& p, hipStream_t st) {
     constexpr int NW = sizeof(T) == 2 ? 8 : 4;                         // what LDS holds of a head of 128
