@@ -374,11 +374,14 @@ template <typename T, int DH> __device__ __forceinline__ void put(T* row, const 
             Vec4<T>::store(row + 32 * d + 8 * b + 4 * (lane >> 5), x);
         }
 }
-// LDS written by other lanes of this wave may be read behind it (a wave's LDS accesses take effect in order).
+// LDS written by other lanes of this wave may be read behind it (a wave's LDS instructions take effect in order).
 __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
+// The same towards copies that go straight into LDS: those write when memory answers, in no order with LDS instructions, so what
+// this wave has read of the tile has to have arrived before the next one is asked for.
+__device__ __forceinline__ void wave_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // What rounding x to bf16 left, in units of 1/256 of the last place: with it an output has 15 bits behind the leading one, in
 // 8 bits more of memory (o in 32 bits beside it: 16384-token training pass 383 us, so 379, and 3 bytes an element more kept).
 __device__ __forceinline__ int rest_of(float x) {
@@ -572,7 +575,7 @@ __device__ __forceinline__ char* stream(char* lds, const T* A, long lda, const T
     }
     return lds + (cnt & 1) * 2 * BYTES;
 }
-// 32 rows from r0 of a matrix into an LDS tile of this wave alone.
+// 32 rows from r0 of a matrix into an LDS tile of this wave alone, which nothing of it reads any more (wave_reads_done()).
 template <typename T, int DH> __device__ __forceinline__ void start_wave(char* tile, const T* base, long ld, int r0, int n, int lane) {
     using S = Shape<T, DH>;
     const unsigned to = __builtin_amdgcn_readfirstlane(lds_addr(tile));
@@ -683,7 +686,7 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
             for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
         });
         gather<DH>(acc, Vs, 0, s, lane, T{});
-        wave_lds_fence();
+        wave_reads_done();
     }
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
     float* base = p.ws + ((((long)b * p.Hq + h) * p.rows + qa) * (chunks + 1) + chunk) * (DH + 4);
@@ -885,7 +888,7 @@ __device__ __forceinline__ void dq_far(const Slide& p, char* lds, int x, int h, 
         for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sc, -lse)) * (dp[r] + delta);
         hide(s, sp, k0 + 4 * (lane >> 5), k0 < p.sinks, 0.f);
         gather<DH, FINE>(acc, Ks, 0, s, lane, T{});
-        wave_lds_fence();
+        wave_reads_done();
     }
     add_waves<DH, 4>(lds, acc, tid, [&](int c, int d, float sum) {
         const int i = qa + c;
@@ -1106,7 +1109,7 @@ __device__ __forceinline__ void dkv_far(const Slide& p, char* lds, int x, int hk
         dma_wait();
         wave_lds_fence();
         dkv_tile<T, DH, FINE>(Qs, Os, Ls, Ls + 32, 0, k, v, dk, dv, sc, lane, true, sp, q0 + 4 * (lane >> 5), !CAUSAL && q0 < p.sinks);
-        wave_lds_fence();
+        wave_reads_done();
     }
     const auto leave = [&](f32x16* acc, bool values) {
         add_waves<DH, NW>(lds, acc, tid, [&](int c, int d, float sum) {
