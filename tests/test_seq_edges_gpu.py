@@ -68,3 +68,96 @@ CHUNKED = [  # (B, N, Hq, Hkv, dh, window, sinks, lengths)
 @pytest.mark.parametrize("B,N,Hq,Hkv,dh,window,sinks,lengths", CHUNKED)
 def test_first_tokens_of_long_sequences_in_chunks(B, N, Hq, Hkv, dh, window, sinks, lengths, dt):
     _check_attention(B, N, Hq, Hkv, dh, False, window, sinks, lengths, dt)
+
+
+# ----------------------------------------------------------------------------- values that are not finite
+def _pairs(N, window, sinks, causal):
+    return SO.visible(N, N, N if window is None else window, sinks, causal, N)
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,window,sinks,causal", [(150, 20, 3, False), (150, 20, 3, True), (1700, 40, 3, False), (90, None, 0, False)])
+@pytest.mark.parametrize("place", ["q", "k", "v"])
+def test_a_nan_reaches_every_query_that_sees_it(N, window, sinks, causal, dt, place):
+    """No query that looks at a NaN may come out as a number, least of all as the 0 of one that sees nothing; a NaN in a query
+    or a key leaves the others alone."""
+    from vitk import ops
+    B, H, dh, bad = 1, 2, 64, N - 40
+    t = {n: _rand(B, N, H, dh, dtype=dt, seed=s) for s, n in enumerate(("q", "k", "v"))}
+    d_o = _rand(B, N, H, dh, dtype=dt, seed=5)
+    want = SO.sliding_attention(t["q"], t["k"], t["v"], N if window is None else window, sinks, causal, None, dh ** -0.5, R[dt])["o"]
+    t[place][0, bad, 0, 7] = math.nan
+    seen = _pairs(N, window, sinks, causal)
+    hit = (torch.arange(N) == bad) if place == "q" else seen[:, bad]
+    leaves = [t[n].to(DEV).requires_grad_(True) for n in ("q", "k", "v")]
+    o = ops.sliding_attention(*leaves, window, sinks=sinks, causal=causal)
+    dq, dk, dv = torch.autograd.grad(o, leaves, d_o.to(DEV))
+    got = o.detach().cpu()[0, :, 0]
+    if place == "v":
+        assert got[hit, 7].isnan().all()
+    else:
+        assert got[hit].isnan().all()
+        _hold("others", o[:, ~hit, 0], want[0][:, ~hit, 0], want[1][:, ~hit, 0])
+        assert dq.cpu()[0, hit, 0].isnan().all()
+        of = seen[hit].any(0)                       # the keys that such a query sees
+        assert dk.cpu()[0, of, 0].isnan().all() and dv.cpu()[0, of, 0].isnan().all()
+    _hold("the other head", o[:, :, 1], want[0][:, :, 1], want[1][:, :, 1])
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,bad", [(1700, slice(1000, 1700)), (1700, slice(200, 1700)), (400, slice(128, 256))])
+def test_a_run_of_nan_keys_is_not_dropped(N, bad, dt):
+    """First tokens see everything: also where all that one chunk, or one wave, of them looks at is NaN."""
+    from vitk import ops
+    q, k, v = (_rand(1, N, 1, 64, dtype=dt, seed=s) for s in range(3))
+    k[:, bad] = math.nan
+    o = ops.sliding_attention(q.to(DEV), k.to(DEV), v.to(DEV), 20, sinks=3).cpu()
+    hit = _pairs(N, 20, 3, False)[:, bad].any(1)
+    assert o[0, hit].isnan().all() and torch.isfinite(o[0, ~hit]).all()
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_infinite_keys(dt, causal):
+    """A score of minus infinity is a weight of 0, one of plus infinity leaves no number."""
+    from vitk import ops
+    N, bad = 150, 60
+    q, k, v = (_rand(1, N, 1, 64, dtype=dt, seed=s) for s in range(3))
+    q[0, :2, 0, 0] = torch.tensor([1.0, -1.0])      # of the first tokens, which see it without a causal mask, one of each
+    want = SO.sliding_attention(q, k, v, 20, 3, causal, None, 0.125, R[dt])["o"]
+    without = SO.attention(q[0, :, 0].double(), k[0, :, 0].double(), v[0, :, 0].double(),
+                           _pairs(N, 20, 3, causal) & (torch.arange(N) != bad), 0.125, R[dt])["o"]
+    k[0, bad, 0, 0] = math.inf
+    o = ops.sliding_attention(q.to(DEV), k.to(DEV), v.to(DEV), 20, sinks=3, causal=causal).cpu()[0, :, 0]
+    seen, up = _pairs(N, 20, 3, causal)[:, bad], q[0, :, 0, 0].float() > 0
+    assert o[seen & up].isnan().all() and (seen & up).any()
+    for rows, (val, e) in ((~seen, (want[0][0, :, 0], want[1][0, :, 0])), (seen & ~up, without)):
+        _hold("rows", o[rows], val[rows], e[rows])
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("cap,window", [(90, 50), (6000, 5000)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_decode_of_values_that_are_not_finite(cap, window, value, dt):
+    from vitk import ops
+    B, Hq, Hkv, dh = 2, 4, 2, 64
+    q, k, v = _rand(B, Hq, dh, dtype=dt).abs(), _rand(B, cap, Hkv, dh, dtype=dt, seed=1), _rand(B, cap, Hkv, dh, dtype=dt, seed=2)
+    n = torch.tensor([cap, cap - 7], dtype=torch.int32, device=DEV)
+
+    def call(q, k):
+        return ops.sliding_attention_decode(q.to(DEV), k.to(DEV), v.to(DEV), n, window, sinks=2).cpu()
+
+    clean = call(q, k)
+    bad = q.clone()
+    bad[0, 1, 3] = value
+    o = call(bad, k)
+    assert o[0, 1].isnan().all() and torch.equal(o[0, 0], clean[0, 0]) and torch.equal(o[:, 2:], clean[:, 2:])
+    for at, hit in ((cap - 9, True), (1, True), (cap - window - 10, False)):
+        bad = k.clone()
+        bad[1, at, 0, 3] = value
+        o = call(q, bad)
+        assert o[1, :2].isnan().all() if hit else torch.equal(o, clean), at
+        assert torch.equal(o[0], clean[0]) and torch.equal(o[:, 2:], clean[:, 2:])
+    bad = k.clone()
+    bad[1, cap - window - 7:cap - 8] = value                  # all that some workgroups look at
+    assert call(q, bad)[1].isnan().all()

@@ -502,6 +502,11 @@ __device__ __forceinline__ Item item_of(const Slide& p, int heads, int tiles) {
     it.b = k / tiles / heads;
     return it;
 }
+// The factor of a record whose maximum is m, towards the common maximum.  Where both are -inf its sums are 0, or NaN if all
+// that it looked at was: either way they stay what they are.
+__device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.f : __builtin_amdgcn_exp2f(m - top); }
+// A row's result from its sums; a total of exactly 0 is a row that sees nothing (a NaN is not).
+__device__ __forceinline__ float share_of(float sum, float total) { return total == 0.f ? 0.f : sum / total; }
 // Sums of the waves, [32 columns][DH + 4] each, in LDS.
 template <int DH> constexpr int join_bytes(int waves = 4) { return waves * 32 * (DH + 4) * (int)sizeof(float); }
 
@@ -524,7 +529,7 @@ template <int DH, int NW, typename F> __device__ __forceinline__ void join_waves
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const float* rec = out + (w * 32 + c) * W;
-            const float e = rec[DH] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(rec[DH] - top);
+            const float e = weight_of(rec[DH], top);
             x += rec[d] * e;
             sum += rec[DH + 1] * e;
         }
@@ -591,11 +596,11 @@ template <typename T, int DH> __device__ __forceinline__ void start_wave(char* t
 // Element d of an output row from its sums, the maximum behind them (base 2) and their total.
 template <typename T, int DH>
 __device__ __forceinline__ void write_row(const Slide& p, int b, int h, int i, int d, float sum, float top, float total) {
-    const float x = total > 0.f ? sum / total : 0.f;
+    const float x = share_of(sum, total);
     const long row = ((long)b * p.N + i) * p.Hq + h;
     ((T*)p.o)[row * DH + d] = (T)x;
     if (sizeof(T) == 2 && p.rest) p.rest[row * DH + d] = (int8_t)rest_of(x);
-    if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.N + i] = total > 0.f ? top + __log2f(total) : INFINITY;
+    if (p.lse && d == 0) p.lse[((long)b * p.Hq + h) * p.N + i] = total == 0.f ? INFINITY : top + __log2f(total);
 }
 // Band: 128 queries of one (sequence, head), each wave 32 of them; key tiles stream through LDS.
 // A head of 64 is bound by vector instructions: 96 beside 8 matrix ones to a 32 x 32 tile, 16 of them exponentials at a
@@ -643,13 +648,13 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
         if (lane < 32) { rec[DH] = m; rec[DH + 1] = l; }
         return;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     const long row = ((long)b * p.N + qa) * p.Hq + h, ld = (long)p.Hq * DH;
     via += wave * 32 * S::ROW;
     put_rows<DH>(via, (T*)p.o + row * DH, ld, p.N - qa, acc, inv, lane);
     if (sizeof(T) == 2 && p.rest) put_rest<DH>(via, p.rest + row * DH, ld, p.N - qa, acc, inv, lane);
     // base-2 logarithm of the row's sum; +inf for a row that sees nothing, so that backward's probabilities are 0
-    if (p.lse && lane < 32 && qi < p.N) p.lse[((long)b * p.Hq + h) * p.N + qi] = l > 0.f ? m + __log2f(l) : INFINITY;
+    if (p.lse && lane < 32 && qi < p.N) p.lse[((long)b * p.Hq + h) * p.N + qi] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 // Far: 32 first queries against every (4 chunks)-th 32 keys behind their band; or, without chunks, against all they see.
 template <typename T, int DH>
@@ -720,22 +725,22 @@ template <int DH> __device__ __forceinline__ Joined<DH> join_records(const float
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float* r = rec + (long)least(s0 + u, count - 1) * width;
-            m[u] = s0 + u < count ? r[DH] : -INFINITY;
-            l[u] = r[DH + 1];
-            v[u] = r[d];
+            const bool is = s0 + u < count;
+            m[u] = is ? r[DH] : -INFINITY;
+            l[u] = is ? r[DH + 1] : 0.f;
+            v[u] = is ? r[d] : 0.f;
         }
         float t = j.top;
 #pragma unroll
         for (int u = 0; u < U; ++u) t = fmaxf(t, m[u]);
-        if (t == -INFINITY) continue;
-        const float a = __builtin_amdgcn_exp2f(j.top - t);
+        const float a = weight_of(j.top, t);
         j.x *= a;
         j.sum *= a;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const float e = __builtin_amdgcn_exp2f(m[u] - t);
-            j.x += e > 0.f ? v[u] * e : 0.f;
-            j.sum += e > 0.f ? l[u] * e : 0.f;
+            const float e = weight_of(m[u], t);
+            j.x += v[u] * e;
+            j.sum += l[u] * e;
         }
         j.top = t;
     }
@@ -1232,7 +1237,7 @@ __global__ __launch_bounds__(NW * 64, 1) void slide_decode_kernel(Decode p) {
         if (g0 + c >= p.G) return;
         const long row = (long)b * p.Hq + hk * p.G + g0 + c;
         if (p.splits == 1) {
-            ((T*)p.o)[row * DH + d] = (T)(sum > 0.f ? x / sum : 0.f);
+            ((T*)p.o)[row * DH + d] = (T)share_of(x, sum);
         } else {
             float* rec = p.ws + (row * p.splits + split) * (DH + 2);
             rec[d] = x;
@@ -1245,7 +1250,7 @@ template <typename T, int DH> __global__ __launch_bounds__(DH < 64 ? 64 : DH) vo
     const int d = threadIdx.x;
     if (d >= DH) return;
     const Joined<DH> j = join_records<DH>(p.ws + row * p.splits * (DH + 2), p.splits, DH + 2, d);
-    ((T*)p.o)[row * DH + d] = (T)(j.sum > 0.f ? j.x / j.sum : 0.f);
+    ((T*)p.o)[row * DH + d] = (T)share_of(j.x, j.sum);
 }
 
 // ----------------------------------------------------------------------------- host side

@@ -259,7 +259,8 @@ def sliding_attention(q, k, v, window, sinks=0, causal=False, lengths=None, scal
     j <= i when i - j < window or j < sinks; otherwise when |i - j| < window or j < sinks or i < sinks (first tokens
     such as a class token see everything).  ``window`` None: no limit.  ``lengths`` int32 [B] on the same device: how many tokens
     of each sequence there are; tokens behind it may hold anything, their outputs and gradients are 0, as are those of
-    a query that sees nothing.  Values of the tokens that are there have to be finite.  Returns [B, N, Hq, dh]."""
+    a query that sees nothing.  A query that looks at a NaN, or at an infinity whose score is no number or plus infinity, gives NaN, and
+    so does its gradient (one in v, or in a gradient, may reach queries and keys up to 63 tokens beyond as well).  Returns [B, N, Hq, dh]."""
     what = "sliding_attention"
     if q.dim() != 4:
         raise VitkError(f"{what}: q is [batch, tokens, heads, head size], got {tuple(q.shape)}")
@@ -362,7 +363,8 @@ def sliding_attention_decode(q, k_cache, v_cache, lengths, window, sinks=0, scal
     last ``window`` of the lengths[b] cached tokens (its own key and value among them).
 
     q [B, Hq, dh]; k_cache, v_cache [B, capacity, Hkv, dh] (any strides); lengths int32 [B] on the same device, at most the
-    capacity; 0 gives a row of zeros.  ``window`` None: no limit.  Not differentiable.  Returns [B, Hq, dh]."""
+    capacity; 0 gives a row of zeros, a NaN among what is seen a row of NaN.  ``window`` None: no limit.  Not differentiable.
+    Returns [B, Hq, dh]."""
     what = "sliding_attention_decode"
     if q.dim() != 3:
         raise VitkError(f"{what}: q is [batch, heads, head size], got {tuple(q.shape)}")
