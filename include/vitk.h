@@ -437,7 +437,8 @@ int vitk_adamw_norm(const void* table, const int* entry_of, int n_blocks, double
  * m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  * param = param (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * `step` counts from 1.  Eight-bit states are rounded at random from the word of (seed, step, element): the expectation
- * of what is held is the moment itself. */
+ * of what is held is the moment itself, but for roots of second moments below 2^-9 of their scale, which are held as 2^-9 of it.
+ * A moment that is no finite number is held as the code's NaN and does not count for the scale. */
 int vitk_adamw_step(const void* table, const int* entry_of, int first_block, int n_blocks, const double* slots, double lr,
                     double beta1, double beta2, double eps, double weight_decay, long step, int state_bits, uint32_t seed,
                     void* stream);

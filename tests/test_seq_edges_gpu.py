@@ -161,3 +161,59 @@ def test_decode_of_values_that_are_not_finite(cap, window, value, dt):
     bad = k.clone()
     bad[1, cap - window - 7:cap - 8] = value                  # all that some workgroups look at
     assert call(q, bad)[1].isnan().all()
+
+
+# ----------------------------------------------------------------------------- AdamW
+def _pair_of_optimizers(n, **kw):
+    from utils.optim import FusedAdamW
+    out = []
+    for _ in range(2):
+        p = torch.nn.Parameter(_rand(n).to(DEV))
+        out.append((p, FusedAdamW([p], lr=1e-2, state_bits=8, **kw)))
+    return out
+
+
+def _moments(p, opt):
+    st = opt.state[p]
+    return [st[x].view(torch.uint8).cpu() for x in ("exp_avg", "exp_avg_sq")] + [st[x + "_scale"].cpu() for x in ("exp_avg", "exp_avg_sq")]
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_adamw_8_bit_holds_what_is_not_finite_where_it_is(value):
+    """One gradient that is no number: its own element shows it from here on, as in 32 bits; its 255 neighbours keep their moments."""
+    (p, a), (q, b) = _pair_of_optimizers(700)
+    at, others = 300, torch.arange(700) != 300
+    for t in range(5):
+        g = _rand(700, seed=10 + t)
+        g[at] = 0.01
+        q.grad = g.to(DEV)
+        if t == 2:
+            g = g.clone()
+            g[at] = value
+        p.grad = g.to(DEV)
+        a.step()
+        b.step()
+        assert torch.equal(p.cpu()[others], q.cpu()[others]), t
+        (m, v, ms, vs), (m2, v2, ms2, vs2) = _moments(p, a), _moments(q, b)
+        assert torch.equal(m[others], m2[others]) and torch.equal(v[others], v2[others]) and torch.equal(ms, ms2) and torch.equal(vs, vs2), t
+        assert bool(p.cpu()[at].isnan()) == (t >= 2)
+        assert bool((m[at] & 127) == 127) == (t >= 2) and bool((v[at] & 127) == 127) == (t >= 2)
+
+
+def test_adamw_8_bit_second_moment_that_overflows_is_not_forgotten():
+    (p, a), _ = _pair_of_optimizers(700)
+    for t in range(3):
+        g = _rand(700, seed=10 + t)
+        if t == 1:
+            g[300] = 1e20                           # its square is beyond 32 bits
+        was = p.detach().clone()
+        p.grad = g.to(DEV)
+        a.step()
+        if t:
+            _, v, _, vs = _moments(p, a)
+            assert (v[300] & 127) == 127            # from now on no number, where 32 bits hold an infinity
+            others = torch.arange(700) != 300
+            assert (v[others] > 0).all() and (vs > 0).all() and torch.isfinite(vs).all()
+            # a step of ordinary size: |m| / sqrt(v) of up to three steps is sqrt(3) at most, codes off by 1/8 twice each; and the decay
+            assert ((p - was).abs().cpu()[others] <= 1e-2 * (4 + 0.01 * 5)).all()
+    assert p[300].isnan()

@@ -14,6 +14,8 @@
 // codes are rounded at random, m in proportion to its distance from the two neighbours and v in proportion to the
 // distance of their SQUARES (in proportion to the roots, E[v] would grow by the variance of the root at each step, more
 // than the 1 - b2 that pulls it back).  A root that is not zero is never held as zero: the next step would divide by eps.
+// What is no finite number (a gradient's NaN or infinity, a square beyond 32 bits) is held as the code's NaN, since there is none for
+// infinity: it shows in its own parameter at the next step, and the other 255 elements keep their moments.
 // The update itself uses the moments before they are rounded.  Nothing below is contracted, and
 // sums have a fixed order, so codes, scales and parameters are the same bits wherever the same inputs are.
 #include "common.h"
@@ -232,7 +234,21 @@ __device__ __forceinline__ void step8(const Entry& en, long base, int cnt, float
             um = um > a ? um : a;
             uv = uv > b ? uv : b;
         }
-        const float tm = wave_max(um), tv = wave_max(uv);
+        float tm = wave_max(um), tv = wave_max(uv);
+        uint32_t mn = 0, vn = 0;                         // codes of NaN where a moment is no finite number
+        if (!(tm < INFINITY && tv < INFINITY)) {         // the scales come from the others, which keep what they hold
+            um = uv = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t a = __float_as_uint(m[k]) & 0x7FFFFFFFu, b = __float_as_uint(root[k]) & 0x7FFFFFFFu;
+                if (a >= 0x7F800000u) { mn |= 0x7Fu << (8 * k); m[k] = 0.f; }
+                else um = um > a ? um : a;
+                if (b >= 0x7F800000u) { vn |= 0x7Fu << (8 * k); root[k] = 0.f; }
+                else uv = uv > b ? uv : b;
+            }
+            tm = wave_max(um);
+            tv = wave_max(uv);
+        }
         const float im = tm >= 1.925929944387236e-34f ? TOP / tm : 0.f;          // 2^-112: nothing to hold
         const float iv = tv >= 1.925929944387236e-34f ? TOP / tv : 0.f;
 #pragma unroll
@@ -245,6 +261,8 @@ __device__ __forceinline__ void step8(const Entry& en, long base, int cnt, float
         mc = __builtin_amdgcn_cvt_pk_fp8_f32(m[2], m[3], mc, true);
         vc = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
         vc = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], vc, true);
+        mc |= mn;
+        vc |= vn;
         if (whole) {
             Vec4<float>::store(en.p + at, p);
             *reinterpret_cast<uint32_t*>((uint8_t*)en.m + at) = mc;

@@ -145,7 +145,8 @@ class FusedAdamW(torch.optim.Optimizer):
     whose state dicts it loads.  8: e4m3 codes of the parameter's shape with one fp32 scale for each 256 consecutive
     elements (`exp_avg_scale`, `exp_avg_sq_scale`); an element of `exp_avg` is code * scale, of `exp_avg_sq`
     (code * scale)^2.  Codes are rounded at random from (``seed``, step, element), so that their expectation is the
-    moment; replicas with equal gradients stay bit-identical.  Parameters and gradients are contiguous fp32 tensors on
+    moment (but for roots below 2^-9 of a scale, which are held as 2^-9); a moment that is no finite number is held as NaN, alone.
+    Replicas with equal gradients stay bit-identical.  Parameters and gradients are contiguous fp32 tensors on
     one GPU.  A step counts on the host, so it is not captured into a graph."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
