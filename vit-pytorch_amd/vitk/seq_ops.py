@@ -2,13 +2,15 @@
 attention with a sliding window and first tokens that stay visible, and its single-token form over a cache.
 
 All of them take ``[batch, tokens, heads, head size]`` tensors in bf16 or fp32 with any strides, run on the current
-stream of the tensors' device (whichever device is current) and raise ``VitkError`` for what they do not take.
+stream of the tensors' device (whichever device is current) and raise ``VitkError`` for what they do not take, forward-mode
+derivatives among it.
 They are offered through ``vitk.ops``.
 """
 import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import Rope, SlideAttn, SlideCache, VitkError, check, dtype_code, lib
@@ -41,6 +43,12 @@ def _one_device(what, first, *ts):
     for t in ts:
         if t is not None and t.device != device:
             raise VitkError(f"{what}: tensors on {device} and {t.device}")
+
+
+def _no_tangents(what, *ts):
+    """Forward-mode derivatives are refused: a call that records nothing for backward would drop them without a word."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise VitkError(f"{what}: no forward-mode derivatives")
 
 
 def _rows(t):
@@ -91,6 +99,7 @@ def _rope_args(x, positions, pairs, base):
         raise VitkError(f"axial_rope: positions are [{N}, {len(pairs)}] or [{B}, {N}, {len(pairs)}], got {tuple(positions.shape)}")
     if not (base > 0 and math.isfinite(base)):
         raise VitkError(f"axial_rope: base must be positive, got {base}")
+    _no_tangents("axial_rope", x, positions)
     _one_device("axial_rope", x, positions)
     return positions.contiguous(), pairs, float(base)
 
@@ -127,6 +136,8 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     (2 i, 2 i + 1) when ``interleaved``.  Angles are reduced to one turn in 64 bits, so positions may be far.
     Returns a new contiguous tensor, or writes ``out`` (same shape and type, consecutive elements inside a head; it may be
     x itself, in a part of a cache, ...; not differentiable)."""
+    if out is not None:
+        _no_tangents("axial_rope", out)
     pos, pairs, base = _rope_args(x, positions, pairs, base)
     interleaved = bool(interleaved)
     if out is None:
@@ -270,6 +281,7 @@ def sliding_attention(q, k, v, window, sinks=0, causal=False, lengths=None, scal
     window, sinks, scale = _reach(what, window, sinks, scale, q.shape[1], q.shape[3])
     if lengths is not None:
         lengths = _lengths(what, lengths, q.shape[0])
+    _no_tangents(what, q, k, v)
     _one_device(what, q, k, v, lengths)
     meta = (window, sinks, bool(causal), scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -326,6 +338,7 @@ def sliding_attention_qkv(qkv, B, N, H, window, sinks=0, causal=False, scale=Non
         raise VitkError(f"{what}: qkv {tuple(qkv.shape)} is not [{B} * {N}, 3 * {H} heads]")
     if (positions is None) != (pairs is None):
         raise VitkError(f"{what}: positions and pairs go together")
+    _no_tangents(what, qkv)
     _one_device(what, qkv)
     qkv = qkv if qkv.is_contiguous() and qkv.data_ptr() % 16 == 0 else qkv.clone(memory_format=torch.contiguous_format)
     x = qkv.detach().view(B, N, 3 * H, -1)
@@ -370,6 +383,7 @@ def sliding_attention_decode(q, k_cache, v_cache, lengths, window, sinks=0, scal
         raise VitkError(f"{what}: q is [batch, heads, head size], got {tuple(q.shape)}")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise VitkError(f"{what}: not differentiable; call it under torch.no_grad()")
+    _no_tangents(what, q, k_cache, v_cache)
     _heads(what, q, k_cache, v_cache)
     B, Hq, dh = q.shape
     cap, Hkv = k_cache.shape[1:3]
