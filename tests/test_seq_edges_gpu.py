@@ -217,3 +217,19 @@ def test_adamw_8_bit_second_moment_that_overflows_is_not_forgotten():
             # a step of ordinary size: |m| / sqrt(v) of up to three steps is sqrt(3) at most, codes off by 1/8 twice each; and the decay
             assert ((p - was).abs().cpu()[others] <= 1e-2 * (4 + 0.01 * 5)).all()
     assert p[300].isnan()
+
+
+# ----------------------------------------------------------------------------- rotary positions
+def test_axial_rope_in_place_is_seen_by_autograd():
+    from vitk import ops
+    x = _rand(1, 5, 2, 64).to(DEV)
+    w = _rand(1, 5, 2, 64, seed=1).to(DEV).requires_grad_(True)
+    y = (w * x).sum()                                # its backward pass needs x
+    before = x._version
+    ops.axial_rope(x, torch.arange(5, device=DEV)[:, None], (32,), out=x)
+    assert x._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():                     # such tensors have no versions
+        z = torch.ones(1, 5, 2, 64, device=DEV)
+        assert ops.axial_rope(z, torch.arange(5, device=DEV)[:, None], (32,), out=z) is z

@@ -135,7 +135,7 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     axis a turns by ``positions[..., a] * base ** (-i / pairs[a])``.  With P = sum(pairs), pairs are elements (i, i + P), or
     (2 i, 2 i + 1) when ``interleaved``.  Angles are reduced to one turn in 64 bits, so positions may be far.
     Returns a new contiguous tensor, or writes ``out`` (same shape and type, consecutive elements inside a head; it may be
-    x itself, in a part of a cache, ...; not differentiable)."""
+    x itself, in a part of a cache, ...; not differentiable; for autograd it counts as modified in place)."""
     if out is not None:
         _no_tangents("axial_rope", out)
     pos, pairs, base = _rope_args(x, positions, pairs, base)
@@ -155,6 +155,8 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     if out.numel():
         with _On(x.device) as on:
             _rope_call(x, out, pos, pairs, base, interleaved, False, on)
+        if not out.is_inference():             # written through a raw pointer: a graph that keeps `out` has to know
+            torch.autograd.graph.increment_version(out)
     return out
 
 
