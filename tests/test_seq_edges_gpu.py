@@ -233,3 +233,44 @@ def test_axial_rope_in_place_is_seen_by_autograd():
     with torch.inference_mode():                     # such tensors have no versions
         z = torch.ones(1, 5, 2, 64, device=DEV)
         assert ops.axial_rope(z, torch.arange(5, device=DEV)[:, None], (32,), out=z) is z
+
+
+ODD = ["pointer", "tokens", "heads", "sequence of one", "gradient"]
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("odd", ODD)
+def test_axial_rope_takes_rows_at_odd_places(odd, inter, dt):
+    from vitk import ops
+    B, N, H, dh, pairs = 2, 5, 3, 64, (7, 20)
+    pos = torch.randint(0, 50, (N, 2), generator=torch.Generator().manual_seed(1))
+    x, dy = _rand(B, N, H, dh, dtype=dt), _rand(B, N, H, dh, dtype=dt, seed=1)
+    if odd == "sequence of one":
+        x, dy = x[:1], dy[:1]
+
+    def place(t):
+        t = t.to(DEV)
+        if odd == "pointer":
+            return torch.zeros(t.numel() + 1, dtype=dt, device=DEV)[1:].view(t.shape).copy_(t)
+        if odd == "tokens":
+            return torch.zeros(B, N, H * dh + 1, dtype=dt, device=DEV)[:, :, :H * dh].unflatten(2, (H, dh)).copy_(t)
+        if odd == "heads":
+            return torch.zeros(B, N, H, dh + 3, dtype=dt, device=DEV)[..., :dh].copy_(t)
+        if odd == "sequence of one":
+            return t.as_strided(t.shape, (7, *t.stride()[1:]))
+        return t
+
+    xd = place(x).detach().requires_grad_(True)
+    y = ops.axial_rope(xd, pos.to(DEV), pairs, interleaved=inter)
+    if odd == "gradient":                            # the slice of a wider one
+        wide = torch.cat([y, torch.ones(B, N, H, 1, dtype=dt, device=DEV)], -1)
+        wide.backward(torch.cat([dy, torch.ones(B, N, H, 1, dtype=dt)], -1).to(DEV))
+    else:
+        y.backward(place(dy))
+    for name, got, src, inv in (("y", y, x, False), ("dx", xd.grad, dy, True)):
+        val, e = SO.rope(src, pos, pairs, 10000.0, inter, inv)
+        _hold(name, got, val, e + (R[dt] + SO.U) * val.abs())
+    to = place(torch.zeros_like(x))
+    assert ops.axial_rope(x.to(DEV), pos.to(DEV), pairs, interleaved=inter, out=to) is to
+    assert torch.equal(to, y)

@@ -104,8 +104,18 @@ def _rope_args(x, positions, pairs, base):
     return positions.contiguous(), pairs, float(base)
 
 
+def _odd(t):
+    """Whether a head of `t` may begin at an odd element: the kernel moves interleaved pairs as wholes."""
+    st = t.stride()
+    return (t.data_ptr() // t.element_size() | st[0] | st[1] | st[2]) & 1
+
+
+def _rope_rows(x, interleaved):
+    return x if x.stride(-1) == 1 and not (interleaved and _odd(x)) else x.clone(memory_format=torch.contiguous_format)
+
+
 def _rope_new(x, pos, pairs, base, interleaved, inverse):
-    x = x if x.stride(-1) == 1 else x.contiguous()
+    x = _rope_rows(x, interleaved)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if y.numel():
         with _On(x.device) as on:
@@ -151,7 +161,9 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise VitkError("axial_rope: out holds an element in more than one place")
     _one_device("axial_rope", x, out)
-    x = x if x.stride(-1) == 1 else x.contiguous()
+    if interleaved and _odd(out):
+        return out.copy_(_rope_new(x, pos, pairs, base, interleaved, False))
+    x = _rope_rows(x, interleaved)
     if out.numel():
         with _On(x.device) as on:
             _rope_call(x, out, pos, pairs, base, interleaved, False, on)
