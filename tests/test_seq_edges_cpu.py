@@ -33,3 +33,28 @@ def test_forward_mode_derivatives_are_refused(which, grad):
                 call()
     with pytest.raises(VitkError, match="GPU only"):
         ops.sliding_attention(_t(2, 5, 4, 64), _t(2, 5, 2, 64), _t(2, 5, 2, 64), 3)
+
+
+def _views():
+    """(x, out, whether they share an element at different indices) of one buffer, told element by element."""
+    for shape in ((1, 4, 2, 2), (2, 3, 1, 4), (1, 1, 3, 2), (2, 2, 2, 2)):
+        for st in ((16, 4, 2, 1), (2, 8, 4, 1), (24, 8, 4, 1), (3, 5, 2, 1), (0, 4, 2, 1)):
+            for to in (st, (16, 4, 2, 1)):
+                for at in range(-9, 10):
+                    base = torch.arange(200)
+                    x, out = base.as_strided(shape, st, 20), base.as_strided(shape, to, 20 + at)
+                    if out.unique().numel() == out.numel():
+                        yield x, out, bool(((x.reshape(-1, 1) == out.reshape(1, -1)) & ~torch.eye(x.numel(), dtype=torch.bool)).any())
+
+
+def test_axial_rope_knows_where_out_meets_x():
+    from vitk.seq_ops import _meets
+    said = known = 0
+    for x, out, shares in _views():
+        if shares:
+            assert _meets(x, out), (x.shape, x.stride(), out.stride(), out.storage_offset())
+        said, known = said + (not _meets(x, out)), known + (not shares)
+    assert said > known // 3                           # and does not always copy
+    packed = torch.zeros(2, 5, 6, 8)
+    assert not _meets(packed[:, :, :3], packed[:, :, 3:]) and not _meets(packed, packed) and not _meets(packed, packed.clone())
+    assert _meets(packed[:, :-1], packed[:, 1:]) and _meets(packed[:, :, :4], packed[:, :, 2:])

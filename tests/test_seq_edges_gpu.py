@@ -274,3 +274,18 @@ def test_axial_rope_takes_rows_at_odd_places(odd, inter, dt):
     to = place(torch.zeros_like(x))
     assert ops.axial_rope(x.to(DEV), pos.to(DEV), pairs, interleaved=inter, out=to) is to
     assert torch.equal(to, y)
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_axial_rope_into_a_place_that_overlaps_its_input(inter):
+    from vitk import ops
+    cache = _rand(2, 4000, 6, 64, dtype=BF).to(DEV)
+    pos = torch.arange(3999, device=DEV)[:, None]
+    want = ops.axial_rope(cache[:, :-1, :4], pos, (32,), interleaved=inter)
+    for to in (lambda c: c[:, 1:, :4], lambda c: c[:, :-1, 1:5], lambda c: c[:, :-1, 2:], lambda c: c[:, :-1, :4]):
+        work = cache.clone()
+        out = to(work)
+        rest = torch.ones_like(work, dtype=torch.bool)
+        to(rest).fill_(False)
+        ops.axial_rope(work[:, :-1, :4], pos, (32,), interleaved=inter, out=out)
+        assert torch.equal(out, want) and torch.equal(work[rest], cache[rest])

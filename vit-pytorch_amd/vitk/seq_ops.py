@@ -114,6 +114,31 @@ def _rope_rows(x, interleaved):
     return x if x.stride(-1) == 1 and not (interleaved and _odd(x)) else x.clone(memory_format=torch.contiguous_format)
 
 
+def _meets(x, out):
+    """Whether a write to `out` may land on elements of `x` other than the one it comes from, which another workgroup may not have
+    read yet.  Both have the same shape; a layout too tangled to tell counts as one that meets."""
+    if any(n == 0 for n in x.shape):
+        return False
+    st = [0 if n == 1 else s for s, n in zip(x.stride(), x.shape)]
+    to = [0 if n == 1 else s for s, n in zip(out.stride(), x.shape)]
+    at = (out.data_ptr() - x.data_ptr()) // x.element_size()
+    if at >= 1 + sum((n - 1) * s for n, s in zip(x.shape, st)) or -at >= 1 + sum((n - 1) * s for n, s in zip(x.shape, to)):
+        return False
+    if st != to:
+        return True
+    dims = sorted(((s, n) for s, n in zip(st, x.shape) if n > 1), reverse=True)
+    if any(s <= sum((m - 1) * t for t, m in dims[i + 1:]) for i, (s, _) in enumerate(dims)):
+        return True
+
+    def hits(at, dims):                # whether a difference of two elements' indices is `at` apart
+        if not dims:
+            return at == 0
+        (s, n), c = dims[0], at // dims[0][0]
+        return any(abs(k) < n and hits(at - k * s, dims[1:]) for k in (c, c + 1))
+
+    return at != 0 and hits(at, dims)
+
+
 def _rope_new(x, pos, pairs, base, interleaved, inverse):
     x = _rope_rows(x, interleaved)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -145,7 +170,7 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     axis a turns by ``positions[..., a] * base ** (-i / pairs[a])``.  With P = sum(pairs), pairs are elements (i, i + P), or
     (2 i, 2 i + 1) when ``interleaved``.  Angles are reduced to one turn in 64 bits, so positions may be far.
     Returns a new contiguous tensor, or writes ``out`` (same shape and type, consecutive elements inside a head; it may be
-    x itself, in a part of a cache, ...; not differentiable; for autograd it counts as modified in place)."""
+    x itself, in a part of a cache, overlap x, ...; not differentiable; for autograd it counts as modified in place)."""
     if out is not None:
         _no_tangents("axial_rope", out)
     pos, pairs, base = _rope_args(x, positions, pairs, base)
@@ -161,7 +186,7 @@ def axial_rope(x, positions, pairs, base=10000.0, interleaved=False, out=None):
     if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
         raise VitkError("axial_rope: out holds an element in more than one place")
     _one_device("axial_rope", x, out)
-    if interleaved and _odd(out):
+    if (interleaved and _odd(out)) or _meets(x, out):
         return out.copy_(_rope_new(x, pos, pairs, base, interleaved, False))
     x = _rope_rows(x, interleaved)
     if out.numel():
