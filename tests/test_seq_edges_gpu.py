@@ -289,3 +289,17 @@ def test_axial_rope_into_a_place_that_overlaps_its_input(inter):
         to(rest).fill_(False)
         ops.axial_rope(work[:, :-1, :4], pos, (32,), interleaved=inter, out=out)
         assert torch.equal(out, want) and torch.equal(work[rest], cache[rest])
+
+
+@pytest.mark.parametrize("N", [2 ** 25 + 5, 2 ** 26 + 3])
+def test_axial_rope_of_more_tokens_than_a_launch_counts_threads_for(N):
+    from vitk import ops
+    x = torch.randn(1, N, 1, 2, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    pos = torch.arange(N, device=DEV, dtype=torch.int32)[:, None]
+    y = ops.axial_rope(x, pos, (1,))[0, :, 0]
+    for lo in range(0, N, 1 << 23):
+        a, b = x[0, lo:lo + (1 << 23), 0].double().unbind(1)
+        turn = pos[lo:lo + (1 << 23), 0].double()
+        for got, val in ((y[lo:lo + (1 << 23), 0], a * turn.cos() - b * turn.sin()), (y[lo:lo + (1 << 23), 1], b * turn.cos() + a * turn.sin())):
+            # the bound of the oracle; 2^26 radians are 2^-26 of one off in 64 bits
+            assert ((got.double() - val).abs() <= 11 * SO.U * (a.abs() + b.abs())).all(), lo

@@ -17,6 +17,7 @@ struct Rope {
     long x_b, x_n, x_h, y_b, y_n, y_h, pos_b;
     int N, H, dh, P, axes, pos_kind;
     long tokens;                     // B * N
+    long from;                       // the first of this launch
     float sign;
     int first[MAX_AXES + 1];         // pairs [first[a], first[a + 1]) belong to axis a
     double turns[MAX_PAIRS];         // turns per unit of position
@@ -35,7 +36,7 @@ __device__ __forceinline__ double position(const Rope& p, long at) {
 template <typename T, int V, bool INTERLEAVED, int TOK>
 __global__ __launch_bounds__(256) void rope_kernel(Rope p) {
     __shared__ float cs[TOK][MAX_PAIRS], sn[TOK][MAX_PAIRS];
-    const long t0 = (long)blockIdx.x * TOK;
+    const long t0 = p.from + (long)blockIdx.x * TOK;
     const int toks = p.tokens - t0 < TOK ? (int)(p.tokens - t0) : TOK;
     for (int i = threadIdx.x; i < toks * p.P; i += 256) {
         const int t = i / p.P, pr = i - t * p.P;
@@ -87,10 +88,14 @@ __global__ __launch_bounds__(256) void rope_kernel(Rope p) {
     }
 }
 
-template <typename T, int V, bool I> int launch(const Rope& p, hipStream_t st) {
+template <typename T, int V, bool I> int launch(Rope p, hipStream_t st) {
     constexpr int TOK = 4;
-    hipLaunchKernelGGL((rope_kernel<T, V, I, TOK>), dim3((unsigned)((p.tokens + TOK - 1) / TOK)), dim3(256), 0, st, p);
-    VITK_CHECK_LAUNCH();
+    constexpr long MOST = 1L << 23;          // workgroups of a launch, whose threads are counted in 32 bits
+    for (; p.from < p.tokens; p.from += MOST * TOK) {
+        const long blocks = (p.tokens - p.from + TOK - 1) / TOK;
+        hipLaunchKernelGGL((rope_kernel<T, V, I, TOK>), dim3((unsigned)(blocks < MOST ? blocks : MOST)), dim3(256), 0, st, p);
+        VITK_CHECK_LAUNCH();
+    }
     return 0;
 }
 template <typename T, bool I> int by_width(const Rope& p, int v, hipStream_t st) {
