@@ -58,3 +58,10 @@ def test_axial_rope_knows_where_out_meets_x():
     packed = torch.zeros(2, 5, 6, 8)
     assert not _meets(packed[:, :, :3], packed[:, :, 3:]) and not _meets(packed, packed) and not _meets(packed, packed.clone())
     assert _meets(packed[:, :-1], packed[:, 1:]) and _meets(packed[:, :, :4], packed[:, :, 2:])
+
+
+def test_axial_rope_refuses_what_its_counters_do_not_hold():
+    one, at = _t(1, 1, 1, 2), torch.zeros(1, 1, dtype=torch.int64)
+    for shape in ((1, 1 << 31, 1, 2), (1 << 16, 1 << 16, 1, 2), (1, (1 << 32) + 5, 1, 2), (1, 1, 1 << 27, 2)):
+        with pytest.raises(VitkError, match="tokens"):
+            ops.axial_rope(one.expand(shape), at.expand(shape[1], 1), (1,))

@@ -89,6 +89,8 @@ def _rope_args(x, positions, pairs, base):
     B, N, H, dh = x.shape
     if dh % 2 or dh > 256 or dh == 0:
         raise VitkError(f"axial_rope: even head sizes up to 256, got {dh}")
+    if B * N >= 1 << 31 or H * dh >= 1 << 28:
+        raise VitkError(f"axial_rope: fewer than 2^31 tokens of fewer than 2^28 elements, got {tuple(x.shape)}")
     if not 1 <= len(pairs) <= 8 or min(pairs) < 1 or sum(pairs) > dh // 2:
         raise VitkError(f"axial_rope: 1 to 8 axes of at least one pair, {dh // 2} pairs in all: got {pairs}")
     if positions.dtype not in _POS_KIND:
