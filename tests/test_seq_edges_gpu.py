@@ -303,3 +303,16 @@ def test_axial_rope_of_more_tokens_than_a_launch_counts_threads_for(N):
         for got, val in ((y[lo:lo + (1 << 23), 0], a * turn.cos() - b * turn.sin()), (y[lo:lo + (1 << 23), 1], b * turn.cos() + a * turn.sin())):
             # the bound of the oracle; 2^26 radians are 2^-26 of one off in 64 bits
             assert ((got.double() - val).abs() <= 11 * SO.U * (a.abs() + b.abs())).all(), lo
+
+
+# ----------------------------------------------------------------------------- no query heads
+def test_key_heads_without_queries_have_gradients_of_zero():
+    from vitk import ops
+    junk = [torch.full((2, 50, 2, 64), math.nan, device=DEV) for _ in range(4)]
+    del junk
+    q, k, v = (torch.ones(2, 50, h, 64, device=DEV, requires_grad=True) for h in (0, 2, 2))
+    junk = [torch.full((2, 50, 2, 64), math.nan, device=DEV) for _ in range(4)]
+    del junk
+    o = ops.sliding_attention(q, k, v, 5)
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), torch.ones_like(o))
+    assert o.shape == dq.shape == q.shape and not dk.any() and not dv.any()

@@ -296,9 +296,9 @@ class SlidingAttentionFn(torch.autograd.Function):
     def backward(ctx, d_o):
         q, k, v, o, rest, lse, lengths = ctx.saved_tensors
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if need_q else None
-        dk, dv = ((torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2)) if need_k or need_v
-                  else (None, None))
+        new = torch.empty if q.numel() else torch.zeros              # keys without queries: gradients of 0
+        dq = new(q.shape, dtype=q.dtype, device=q.device) if need_q else None
+        dk, dv = (new(k.shape, dtype=k.dtype, device=k.device) for _ in range(2)) if need_k or need_v else (None, None)
         if q.numel():
             _slide_backward(q, k, v, o, rest, lse, lengths, ctx.meta, d_o, dq, dk, dv)
         return dq, (dk if need_k else None), (dv if need_v else None), None, None
