@@ -214,7 +214,7 @@ int vitk_window_attn_bwd(const void* qkv, const float* bias_table, const void* o
  * vitk_slide_attn_bwd reads q, k, v, d_o, lse, o, o_rest (bf16) and writes dq, dk, dv (strided; dq, or dk and dv together,
  * may be NULL: not wanted); delta:[B, Hq, N] is workspace.  Sums have a fixed order: equal inputs give equal bits.
  * dh 32, 64 or 128; every pointer 16-byte aligned, every stride a multiple of 16 bytes, *_n below 2^23; Hq % Hkv == 0; window, sinks >= 0;
- * scale > 0. */
+ * scale > 0, finite times log2(e) too. */
 typedef struct vitk_slide_attn {
     const void* q; const void* k; const void* v;
     void* o; signed char* o_rest; float* lse;

@@ -1,8 +1,11 @@
 """What the long-sequence operators refuse or keep, without a GPU, beyond tests/test_seq_cpu.py."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+import vitk
 from vitk import VitkError, ops
 
 
@@ -65,3 +68,19 @@ def test_axial_rope_refuses_what_its_counters_do_not_hold():
     for shape in ((1, 1 << 31, 1, 2), (1 << 16, 1 << 16, 1, 2), (1, (1 << 32) + 5, 1, 2), (1, 1, 1 << 27, 2)):
         with pytest.raises(VitkError, match="tokens"):
             ops.axial_rope(one.expand(shape), at.expand(shape[1], 1), (1,))
+
+
+@pytest.mark.parametrize("scale", [3.4e38, 1e39, 1e300, 1e-40, 1e-300, float("inf"), float("nan"), 0.0, -1.0])
+def test_scales_that_32_bits_do_not_hold_are_refused(scale):
+    n = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: ops.sliding_attention(_t(2, 5, 4, 64), _t(2, 5, 2, 64), _t(2, 5, 2, 64), 3, scale=scale),
+                 lambda: ops.sliding_attention_decode(_t(2, 4, 64), _t(2, 9, 2, 64), _t(2, 9, 2, 64), n, 3, scale=scale)):
+        with pytest.raises(VitkError, match="scale"):
+            call()
+
+
+@pytest.mark.parametrize("scale", [3.4e38, float("inf")])
+def test_c_entries_refuse_scales_that_overflow(scale):
+    a = dict(q=4096, k=4096, v=4096, o=4096, B=1, Hq=2, Hkv=2, dh=64, window=3, scale=scale)
+    assert vitk.lib.vitk_slide_attn_fwd(ctypes.byref(vitk.SlideAttn(**a, N=5)), 0, None) == -1
+    assert vitk.lib.vitk_slide_decode(ctypes.byref(vitk.SlideCache(**a, cap=5, splits=1, lengths=4096)), 0, None) == -1

@@ -1417,7 +1417,7 @@ int fill(const vitk_slide_attn* a, int dtype, bool backward, Slide& p) {
     if (dtype != VITK_BF16 && dtype != VITK_F32) return VITK_ERR_DTYPE;
     if (a->dh != 32 && a->dh != 64 && a->dh != 128) return VITK_ERR_UNSUPPORTED;
     if (a->B <= 0 || a->N <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->B > 65535 || a->Hq > 32767) return VITK_ERR_SHAPE;
-    if (a->N > (1 << 30) || a->window < 0 || a->sinks < 0 || !(a->scale > 0.f)) return VITK_ERR_SHAPE;
+    if (a->N > (1 << 30) || a->window < 0 || a->sinks < 0 || !(a->scale > 0.f && a->scale * LOG2E < INFINITY)) return VITK_ERR_SHAPE;
     const int e = dtype == VITK_BF16 ? 2 : 4;
     if (!aligned(a->q, e, {a->q_b, a->q_n, a->q_h}) || !aligned(a->k, e, {a->k_b, a->k_n, a->k_h}) ||
         !aligned(a->v, e, {a->v_b, a->v_n, a->v_h})) return VITK_ERR_SHAPE;
@@ -1501,7 +1501,7 @@ extern "C" int vitk_slide_decode(const vitk_slide_cache* a, int dtype, void* str
     if (dtype != VITK_BF16 && dtype != VITK_F32) return VITK_ERR_DTYPE;
     if (a->dh != 32 && a->dh != 64 && a->dh != 128) return VITK_ERR_UNSUPPORTED;
     if (a->B <= 0 || a->cap <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv || a->B > 65535) return VITK_ERR_SHAPE;
-    if (a->cap > (1 << 30) || a->window < 0 || a->sinks < 0 || !(a->scale > 0.f) || a->splits < 1 || a->splits > 1024) return VITK_ERR_SHAPE;
+    if (a->cap > (1 << 30) || a->window < 0 || a->sinks < 0 || !(a->scale > 0.f && a->scale * LOG2E < INFINITY) || a->splits < 1 || a->splits > 1024) return VITK_ERR_SHAPE;
     if (a->splits > 1 && !a->workspace) return VITK_ERR_NULL;
     const int e = dtype == VITK_BF16 ? 2 : 4;
     if (!aligned(a->q, e, {a->q_b, a->q_h}) || !aligned(a->k, e, {a->k_b, a->k_n, a->k_h}) || !aligned(a->v, e, {a->v_b, a->v_n, a->v_h}))

@@ -219,8 +219,8 @@ def _reach(what, window, sinks, scale, tokens, dh):
     if window < 0 or sinks < 0:
         raise VitkError(f"{what}: window and sinks count tokens, got {window} and {sinks}")
     scale = 1.0 / math.sqrt(dh) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise VitkError(f"{what}: scale must be positive, got {scale}")
+    if not 2.0 ** -126 <= scale < 2.0 ** 127:           # in 32 bits, times the 1.44 of the base-2 exponential too
+        raise VitkError(f"{what}: scale must be positive and a number in 32 bits, got {scale}")
     return min(window, tokens), min(sinks, tokens), scale
 
 
