@@ -316,3 +316,38 @@ def test_key_heads_without_queries_have_gradients_of_zero():
     o = ops.sliding_attention(q, k, v, 5)
     dq, dk, dv = torch.autograd.grad(o, (q, k, v), torch.ones_like(o))
     assert o.shape == dq.shape == q.shape and not dk.any() and not dv.any()
+
+
+# ----------------------------------------------------------------------------- AdamW: parameters written through raw pointers
+def test_adamw_update_is_seen_by_autograd():
+    """A parameter that a graph has kept is not silently another one in its backward pass."""
+    from utils.optim import FusedAdamW
+    for bits in (8, 32):
+        p = torch.nn.Parameter(_rand(300).to(DEV))
+        x = _rand(300, seed=1).to(DEV).requires_grad_(True)
+        opt = FusedAdamW([p], state_bits=bits)
+        y = (p * x).sum()
+        p.grad = torch.ones_like(p)
+        before = p._version
+        opt.step()
+        assert p._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+def test_adamw_update_of_a_weight_whose_operands_another_one_holds():
+    """Query, key and value share one pair of GEMM operands, kept with the query's weight: also when only the key's is trained."""
+    from utils.optim import FusedAdamW
+    from vitk import ops
+    ws = [torch.nn.Parameter(_rand(64, 64, seed=i).to(DEV)) for i in range(3)]
+    bs = [torch.nn.Parameter(torch.zeros(64, device=DEV)) for _ in range(3)]
+    x = _rand(64, 64, dtype=BF).to(DEV)
+    opt = FusedAdamW([ws[1]], lr=0.1)
+    with torch.no_grad():
+        before = ops.linear(x, tuple(ws), tuple(bs)).clone()
+        ws[1].grad = torch.ones_like(ws[1])
+        opt.step()
+        after = ops.linear(x, tuple(ws), tuple(bs)).clone()
+        ops.invalidate_operands(ws)
+        assert torch.equal(after, ops.linear(x, tuple(ws), tuple(bs)))
+    assert not torch.equal(after[:, 64:128], before[:, 64:128]) and torch.equal(after[:, :64], before[:, :64])

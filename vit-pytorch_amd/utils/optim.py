@@ -313,6 +313,8 @@ class FusedAdamW(torch.optim.Optimizer):
                            "adamw_step")
             for st in all_sts:
                 st["step"] += 1
-            # the parameters were written through raw pointers: renew the GEMM operands kept with them (one launch)
+            # the parameters were written through raw pointers: graphs and operands that have kept them see a new version, and
+            # the GEMM operands kept with them are renewed (one launch)
+            torch.autograd.graph.increment_version(all_ps)
             vitk.ops.refresh_operands(all_ps)
         return norm
