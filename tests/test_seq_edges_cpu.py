@@ -84,3 +84,16 @@ def test_c_entries_refuse_scales_that_overflow(scale):
     a = dict(q=4096, k=4096, v=4096, o=4096, B=1, Hq=2, Hkv=2, dh=64, window=3, scale=scale)
     assert vitk.lib.vitk_slide_attn_fwd(ctypes.byref(vitk.SlideAttn(**a, N=5)), 0, None) == -1
     assert vitk.lib.vitk_slide_decode(ctypes.byref(vitk.SlideCache(**a, cap=5, splits=1, lengths=4096)), 0, None) == -1
+
+
+def test_adamw_copies_keep_their_settings():
+    import copy
+    import pickle
+    from utils.optim import FusedAdamW
+    opt = FusedAdamW([torch.nn.Parameter(torch.zeros(3))], lr=1e-2, state_bits=8, seed=5)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (other.state_bits, other.seed, other.param_groups[0]["lr"]) == (8, 5, 1e-2)
+        assert other.step() is None                   # no gradients
+        other.param_groups[0]["params"][0].grad = torch.zeros(3)
+        with pytest.raises(ValueError, match="GPU"):
+            other.step()

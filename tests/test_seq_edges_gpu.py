@@ -351,3 +351,26 @@ def test_adamw_update_of_a_weight_whose_operands_another_one_holds():
         ops.invalidate_operands(ws)
         assert torch.equal(after, ops.linear(x, tuple(ws), tuple(bs)))
     assert not torch.equal(after[:, 64:128], before[:, 64:128]) and torch.equal(after[:, :64], before[:, :64])
+
+
+def test_adamw_copies_step_on():
+    import copy
+    import io
+    from utils.optim import FusedAdamW
+    for bits in (8, 32):
+        p = torch.nn.Parameter(_rand(300).to(DEV))
+        opt = FusedAdamW([p], state_bits=bits, seed=7)
+        p.grad = _rand(300, seed=2).to(DEV)
+        opt.step()
+        opt.step()                                   # the gradients' addresses are known to the table by now
+        file = io.BytesIO()                          # (torch's tensors of 8-bit floats are not taken by `pickle` itself)
+        torch.save((p, opt), file)
+        file.seek(0)
+        others = [copy.deepcopy((p, opt)), torch.load(file, weights_only=False)]
+        for q, _ in others:
+            q.grad = p.grad.clone()
+        opt.step(max_grad_norm=1.0)
+        for q, o in others:
+            o.step(max_grad_norm=1.0)
+            assert torch.equal(p, q)
+            assert all(torch.equal(opt.state[p][n].float(), o.state[q][n].float()) for n in ("exp_avg", "exp_avg_sq"))

@@ -158,10 +158,21 @@ class FusedAdamW(torch.optim.Optimizer):
             raise ValueError("state_bits is 8 or 32")
         self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFF
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self._empty()
+
+    def _empty(self):
         self._slots = None
         self._dev = None          # the table on the device
         self._last = None         # its contents (numpy), to skip uploads of an unchanged table
         self._ring, self._turn = [], 0
+
+    def __getstate__(self):       # copies and pickles: the settings, and buffers of their own
+        return dict(super().__getstate__(), state_bits=self.state_bits, seed=self.seed)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "_ring" not in self.__dict__:                 # (not when load_state_dict() comes this way)
+            self._empty()
 
     def load_state_dict(self, state_dict):
         held = [s for s in state_dict["state"].values() if s]
