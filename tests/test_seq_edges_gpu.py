@@ -374,3 +374,32 @@ def test_adamw_copies_step_on():
             o.step(max_grad_norm=1.0)
             assert torch.equal(p, q)
             assert all(torch.equal(opt.state[p][n].float(), o.state[q][n].float()) for n in ("exp_avg", "exp_avg_sq"))
+
+
+# ----------------------------------------------------------------------------- decode: alone, shared, replayed
+@pytest.mark.parametrize("dt,dh,window", [(BF, 64, 1500), (BF, 64, 1700), (BF, 64, 1024), (FP, 32, 700), (BF, 128, 700), (BF, 128, 900), (FP, 64, 4000)])
+def test_decode_replays_what_it_gives_eagerly(dt, dh, window):
+    """On both sides of the size from which workgroups share a stream's keys."""
+    from vitk import ops
+    B, Hq, Hkv, cap = 2, 4, 2, window + 40
+    q, k, v = _rand(B, Hq, dh, dtype=dt).to(DEV), _rand(B, cap, Hkv, dh, dtype=dt, seed=1).to(DEV), _rand(B, cap, Hkv, dh, dtype=dt, seed=2).to(DEV)
+    n = torch.tensor([cap, cap - 30], dtype=torch.int32, device=DEV)
+    ops.sliding_attention_decode(q, k, v, n, window, sinks=3)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = ops.sliding_attention_decode(q, k, v, n, window, sinks=3)
+    for turn in range(3):
+        q.copy_(_rand(B, Hq, dh, dtype=dt, seed=10 + turn))
+        n.fill_(cap - turn)
+        want = ops.sliding_attention_decode(q, k, v, n, window, sinks=3)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want), turn
+        for b in range(B):
+            L = cap - turn
+            seen = torch.zeros(1, L, dtype=torch.bool)
+            seen[:, L - window:] = seen[:, :3] = True
+            for h in range(Hq):
+                val, e = SO.attention(q[b, h:h + 1].double().cpu(), k[b, :L, h // 2].double().cpu(), v[b, :L, h // 2].double().cpu(), seen, dh ** -0.5, R[dt])["o"]
+                _hold(f"{turn} {b} {h}", want[b, h:h + 1], val, e)

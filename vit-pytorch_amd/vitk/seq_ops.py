@@ -398,16 +398,22 @@ def _splits(B, Hkv, G, window, sinks, dh, esz, device):
     """Workgroups that share the keys of one (sequence, key head): as many as give each CU one in all, none with fewer than 32
     keys a wave.  One stream of 65536 tokens, 8 key heads of 128: 488 us unsplit, 51 us with 32 each; 12 heads of 64, 16384
     tokens: 97 us unsplit, 16.7 us with 21 each, 19.4 with 22, which is more than there are CUs.
-    One workgroup alone while its waves have no more than 20 KB of keys each: a second launch and its workspace cost a call more
-    than the shares save (1024 keys of 64 elements, 12 heads: 12.9 us a call, 7.7 us replayed from a graph; shared by 5, 17.5
-    and 6.5)."""
+    One workgroup alone while its waves have no more than 24 KB of keys each: shared, the kernels are faster, but a second launch
+    costs an eager call 4 us of host time.  Microseconds alone and shared, eager | replayed from a graph, by KB a wave:
+      12 heads of 64, bf16    8: 12.6 16.5 | 4.8 6.1    20: 12.8 16.8 | 7.6 6.2    24: 12.6 16.8 | 9.7 6.2    32: 12.6 16.8 | 11.7 6.4
+      8 of 4 x 128, bf16     16: 12.7 16.9 | 6.2 7.5    24: 12.6 16.8 | 9.4 7.7    40: 12.7 16.9 | 11.2 7.7   48: 14.8 17.1 | 14.5 7.8
+      4 of 2 x 32, bf16      12: 12.2 16.1 | 6.6 5.5    16: 12.3 16.0 | 7.9 5.5    24: 12.1 15.9 | 10.4 6.0   32: 13.2 16.0 | 12.8 6.3
+      12 heads of 64, fp32   16: 12.5 16.6 | 9.5 8.4    24: 12.6 16.7 | 12.1 8.4   40: 18.4 16.7 | 18.1 8.4   48: 21.3 16.8 | 20.9 8.5
+      4 of 4 x 128, fp32     32: 16.2 16.7 | 16.1 12.4  48: 21.0 16.8 | 20.8 12.3
+    Up to 24 KB what an eager call gains is about what a replay loses, and beyond it is not.  The rule does not ask whether a
+    graph is being captured, so that a replay gives the bits of the eager call."""
     cus = _CUS.get(device.index)
     if cus is None:
         cus = _CUS[device.index] = torch.cuda.get_device_properties(device).multi_processor_count
     groups = B * Hkv * ((G + 31) // 32)
     tiles = -(-window // 32) + -(-sinks // 32)
     turns = -(-tiles // (8 if esz == 2 else 4))
-    if turns * 32 * dh * esz <= 20 * 1024:
+    if turns * 32 * dh * esz <= 24 * 1024:
         return 1
     return max(1, min(turns, cus // groups, 64))
 
