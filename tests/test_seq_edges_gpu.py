@@ -403,3 +403,17 @@ def test_decode_replays_what_it_gives_eagerly(dt, dh, window):
             for h in range(Hq):
                 val, e = SO.attention(q[b, h:h + 1].double().cpu(), k[b, :L, h // 2].double().cpu(), v[b, :L, h // 2].double().cpu(), seen, dh ** -0.5, R[dt])["o"]
                 _hold(f"{turn} {b} {h}", want[b, h:h + 1], val, e)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,dh,cap,window,sinks", [(4, 12, 12, 64, 1100, 1024, 4), (8, 8, 2, 128, 3000, 2900, 0), (16, 8, 4, 32, 300, 200, 3), (32, 12, 12, 64, 40, 9, 2)])
+def test_decode_is_off_by_the_rounding_of_its_result(B, Hq, Hkv, dh, cap, window, sinks):
+    """bf16: probabilities are held in 16 bits behind the leading one, so the error's norm is that of the exact result rounded once,
+    but for 2^-8 of it and the 32-bit sums: a tenth more at most, where probabilities of 8 bits would make it sqrt(2) of that."""
+    from vitk import ops
+    q, k, v = _rand(B, Hq, dh, dtype=BF), _rand(B, cap, Hkv, dh, dtype=BF, seed=1), _rand(B, cap, Hkv, dh, dtype=BF, seed=2)
+    n = torch.full((B,), cap, dtype=torch.int32, device=DEV)
+    o = ops.sliding_attention_decode(q.to(DEV), k.to(DEV), v.to(DEV), n, window, sinks=sinks)
+    at = torch.cat([torch.arange(sinks), torch.arange(cap - window, cap)])
+    qd, kd, vd = q.double().view(B, Hkv, -1, dh), k[:, at].double().transpose(1, 2).contiguous(), v[:, at].double().transpose(1, 2).contiguous()
+    want = (torch.softmax(qd @ kd.transpose(2, 3).contiguous() * dh ** -0.5, -1) @ vd).view(B, Hq, dh)
+    _near("o", o, want, 1.1 * float((want.to(BF).double() - want).norm() / want.norm()))

@@ -400,12 +400,12 @@ def _splits(B, Hkv, G, window, sinks, dh, esz, device):
     tokens: 97 us unsplit, 16.7 us with 21 each, 19.4 with 22, which is more than there are CUs.
     One workgroup alone while its waves have no more than 24 KB of keys each: shared, the kernels are faster, but a second launch
     costs an eager call 4 us of host time.  Microseconds alone and shared, eager | replayed from a graph, by KB a wave:
-      12 heads of 64, bf16    8: 12.6 16.5 | 4.8 6.1    20: 12.8 16.8 | 7.6 6.2    24: 12.6 16.8 | 9.7 6.2    32: 12.6 16.8 | 11.7 6.4
-      8 of 4 x 128, bf16     16: 12.7 16.9 | 6.2 7.5    24: 12.6 16.8 | 9.4 7.7    40: 12.7 16.9 | 11.2 7.7   48: 14.8 17.1 | 14.5 7.8
-      4 of 2 x 32, bf16      12: 12.2 16.1 | 6.6 5.5    16: 12.3 16.0 | 7.9 5.5    24: 12.1 15.9 | 10.4 6.0   32: 13.2 16.0 | 12.8 6.3
-      12 heads of 64, fp32   16: 12.5 16.6 | 9.5 8.4    24: 12.6 16.7 | 12.1 8.4   40: 18.4 16.7 | 18.1 8.4   48: 21.3 16.8 | 20.9 8.5
-      4 of 4 x 128, fp32     32: 16.2 16.7 | 16.1 12.4  48: 21.0 16.8 | 20.8 12.3
-    Up to 24 KB what an eager call gains is about what a replay loses, and beyond it is not.  The rule does not ask whether a
+      12 heads of 64, bf16    8: 12.7 16.8 | 5.1 6.6    20: 12.7 17.0 | 8.9 6.8    24: 12.6 16.9 | 11.4 6.8   32: 14.5 17.0 | 14.3 7.1
+      8 of 4 x 128, bf16     16: 12.7 16.9 | 6.7 8.0    24: 12.7 16.9 | 10.4 8.2   40: 13.3 17.0 | 12.9 8.3   48: 17.7 16.9 | 17.3 8.4
+      4 of 2 x 32, bf16      12: 12.7 16.7 | 7.9 6.0    16: 12.7 16.8 | 9.8 6.1    24: 13.6 16.8 | 13.2 7.0   32: 17.0 16.8 | 16.7 7.2
+      12 heads of 64, fp32   16: 12.8 16.9 | 9.4 8.6    24: 12.8 16.9 | 11.9 8.7   40: 18.2 17.0 | 17.8 8.7   48: 21.0 16.9 | 20.6 8.8
+      4 of 4 x 128, fp32     32: 16.2 17.1 | 16.0 12.5  48: 20.9 17.0 | 20.5 12.4
+    Up to about 24 KB an eager call gains what a replay loses, and beyond it does not.  The rule does not ask whether a
     graph is being captured, so that a replay gives the bits of the eager call."""
     cus = _CUS.get(device.index)
     if cus is None:
