@@ -417,3 +417,19 @@ def test_decode_is_off_by_the_rounding_of_its_result(B, Hq, Hkv, dh, cap, window
     qd, kd, vd = q.double().view(B, Hkv, -1, dh), k[:, at].double().transpose(1, 2).contiguous(), v[:, at].double().transpose(1, 2).contiguous()
     want = (torch.softmax(qd @ kd.transpose(2, 3).contiguous() * dh ** -0.5, -1) @ vd).view(B, Hq, dh)
     _near("o", o, want, 1.1 * float((want.to(BF).double() - want).norm() / want.norm()))
+
+
+# ----------------------------------------------------------------------------- short windows
+@pytest.mark.parametrize("N,Hq,Hkv,dh,causal,window,sinks", [(700, 4, 2, 64, False, 9, 0), (700, 2, 2, 128, True, 16, 0), (1700, 2, 2, 64, False, 16, 3),
+                                                             (500, 4, 4, 32, True, 3, 2)])
+def test_short_windows_are_off_by_the_rounding_of_their_results(N, Hq, Hkv, dh, causal, window, sinks):
+    """bf16, windows of up to 16 keys: what goes into the products is held in 16 bits, so an error's norm is nearer to that of the exact result
+    rounded once than to that and another rounding of probabilities or score gradients, sqrt(2) of it; the limit lies half way."""
+    from vitk import ops
+    q, k, v, d_o = (_rand(1, N, h, dh, dtype=BF, seed=s) for s, h in enumerate((Hq, Hkv, Hkv, Hq)))
+    want = SO.sliding_attention(q, k, v, window, sinks, causal, None, dh ** -0.5, R[BF], d_o)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (q, k, v)]
+    o = ops.sliding_attention(*leaves, window, sinks=sinks, causal=causal)
+    for name, got in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, d_o.to(DEV)))):
+        val = want[name][0]
+        _near(name, got, val, (1 + math.sqrt(2.0)) / 2 * float((val.to(BF).double() - val).norm() / val.norm()))

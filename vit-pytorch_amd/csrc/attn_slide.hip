@@ -255,7 +255,7 @@ template <int DH> __device__ __forceinline__ f32x16 product(const char* tile, in
     return acc;
 }
 // acc[d][column] += sum over 32 tile rows from r0 of tile[row][d] * w[row][column]; w as a product left it.  In bf16
-// the weights are rounded to the operand type here: 2^-9 of each, independent, and the sums stay in 32 bits; FINE: what
+// the weights are rounded to the operand type here: by up to 2^-8 of each, independent, and the sums stay in 32 bits; FINE: what
 // that leaves of them is a second operand.
 template <int DH, bool FINE = false> __device__ __forceinline__ void gather(f32x16* acc, const char* tile, int r0, const f32x16& w, int lane, bf16_t) {
     using S = Shape<bf16_t, DH>;
@@ -607,7 +607,7 @@ __device__ __forceinline__ void write_row(const Slide& p, int b, int h, int i, i
 // quarter of the rate (vector pipes busy 67 % of the cycles, matrix cores 38 %).  Four waves of 32 queries share each staged
 // tile; with two tiles in LDS at once and the copies behind the barrier the loop does not wait for memory (single
 // buffers: 104 us where two took 70).
-template <typename T, int DH, bool CAUSAL>
+template <typename T, int DH, bool CAUSAL, bool FINE>
 __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
@@ -636,7 +636,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
             f32x16 s = product<DH>(Ks, sub, q, lane);
             if (cov == 1) hide(s, sp, ka + 4 * (lane >> 5), ka < p.sinks, -INFINITY);
             sm.step(s, sc, rescale);
-            gather<DH>(acc, Vs, sub, s, lane, T{});
+            gather<DH, FINE>(acc, Vs, sub, s, lane, T{});
         }
     });
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
@@ -657,7 +657,7 @@ __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int 
     if (p.lse && lane < 32 && qi < p.N) p.lse[((long)b * p.Hq + h) * p.N + qi] = l == 0.f ? INFINITY : m + __log2f(l);
 }
 // Far: 32 first queries against every (4 chunks)-th 32 keys behind their band; or, without chunks, against all they see.
-template <typename T, int DH>
+template <typename T, int DH, bool FINE>
 __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h, int b, int n) {
     using S = Shape<T, DH>;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = h / p.G;
@@ -690,7 +690,7 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
 #pragma unroll
             for (int d = 0; d < DH / 32; ++d) acc[d] *= alpha;
         });
-        gather<DH>(acc, Vs, 0, s, lane, T{});
+        gather<DH, FINE>(acc, Vs, 0, s, lane, T{});
         wave_reads_done();
     }
     const float l = sm.total(), m = sm.m == -INFINITY ? -INFINITY : sm.m * sc;
@@ -705,15 +705,15 @@ __device__ __forceinline__ void fwd_far(const Slide& p, char* lds, int x, int h,
         if (d == 0) { rec[DH] = top; rec[DH + 1] = total; }
     });
 }
-template <typename T, int DH, bool CAUSAL>
+template <typename T, int DH, bool CAUSAL, bool FINE>
 __global__ __launch_bounds__(256, 2) void slide_fwd_kernel(Slide p) {
     extern __shared__ __align__(16) char lds[];
     const Item it = item_of(p, p.Hq, (p.N + TQ - 1) / TQ);
     if (it.none) return;
     const int n = length_of(p, it.b);
     if constexpr (!CAUSAL)
-        if (it.far) return fwd_far<T, DH>(p, lds, it.x, it.h, it.b, n);
-    fwd_band<T, DH, CAUSAL>(p, lds, it.x * TQ, it.h, it.b, n);
+        if (it.far) return fwd_far<T, DH, FINE>(p, lds, it.x, it.h, it.b, n);
+    fwd_band<T, DH, CAUSAL, FINE>(p, lds, it.x * TQ, it.h, it.b, n);
 }
 // One softmax from `count` records of `width` numbers, as element d sees it: several records are in flight at a time.
 template <int DH> struct Joined { float x, top, sum; };
@@ -928,7 +928,7 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const f
     if (masked) hide(s, sp, x0, first, 0.f);
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] *= s[r];
-    gather<DH>(dv, Os, sub, s, lane, T{});
+    gather<DH, FINE>(dv, Os, sub, s, lane, T{});
     gather<DH, FINE>(dk, Qs, sub, dp, lane, T{});
 }
 // How a workgroup of the dK / dV kernel is laid out: NW waves, 32 KG keys; wave w keeps keys 32 (w % KG) and takes every
@@ -1328,16 +1328,16 @@ template <typename T, int DH, bool CAUSAL, int NW, int KG, bool FINE> int launch
     VITK_CHECK_LAUNCH();
     return 0;
 }
-template <typename T, int DH, bool CAUSAL> int run_fwd(Slide p, float* ws, hipStream_t st) {
+template <typename T, int DH, bool CAUSAL, bool FINE> int run_fwd(Slide p, float* ws, hipStream_t st) {
     if (!CAUSAL) {
         const Records r = records_of(p.B, p.N, p.Hq, 1, DH + 4, p.window, p.sinks, 4);
         p.rows = r.rows; p.chunks = r.chunks; p.ws = ws;
         if (r.floats && !ws) return VITK_ERR_NULL;
     }
     const int bytes = lds_bytes<T, DH>(p.rows > 0);
-    if (int e = allow_lds(slide_fwd_kernel<T, DH, CAUSAL>, bytes)) return e;
+    if (int e = allow_lds(slide_fwd_kernel<T, DH, CAUSAL, FINE>, bytes)) return e;
     const unsigned grid = grid_of(p, p.Hq, p.rows > 0);
-    hipLaunchKernelGGL((slide_fwd_kernel<T, DH, CAUSAL>), dim3(grid), dim3(256), bytes, st, p);
+    hipLaunchKernelGGL((slide_fwd_kernel<T, DH, CAUSAL, FINE>), dim3(grid), dim3(256), bytes, st, p);
     VITK_CHECK_LAUNCH();
     if (p.chunks) {
         hipLaunchKernelGGL((slide_fwd_join_kernel<T, DH>), dim3(p.rows < p.N ? p.rows : p.N, p.Hq, p.B), dim3(DH < 64 ? 64 : DH), 0, st, p);
@@ -1384,11 +1384,19 @@ template <typename T, int DH, bool CAUSAL, bool FINE> int run_bwd(Slide p, float
     }
     return 0;
 }
-// bf16 score gradients go into their products as two numbers each where a window holds few keys: with one, dQ and dK are off by
-// 0.0024 of their norm (of a result rounded once 0.0017), and by 0.0025 and more in rows of a few keys, where the deltas' own error has
-// nothing to average over; with two by 0.0017 to 0.0019.  8 x 2305 x 12 x 64, backward: window 1 64.5 us and 65.4, window 17 85 us and
-// 91; at a window of 145 it would be 125 us and 146.
+// In bf16, probabilities and score gradients go into their products as two numbers each where a window holds few keys: o, dQ, dK and
+// dV are then off by their own rounding alone (0.0016 to 0.0017 of their norm), and by 0.0024 with one number each, dQ and dK of rows
+// of a few keys by 0.0025 and more: the deltas take over the error of o, which has nothing to average over there.  8 x 2305 x 12 x 64, one
+// number and two, whole calls: window 16 forward 33 us and 36, backward 106 and 118; window 33 33 and 35, 102 and 115; window 145 46 and
+// 57, 143 and 172.  16384 causal tokens, 8 heads of 2 x 128: window 16 30 and 32, 99 and 109; window 1024 84 and 110, 275 and 354.
+// The rule goes by the window: the first rows of a causal sequence and sequences of up to 16 tokens in a longer batch, which see few keys under
+// any window, stay at one number.
 constexpr int FINE_WINDOW = 16;
+template <typename T, int DH, bool CAUSAL> int run_fwd(const Slide& p, float* ws, hipStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (p.window <= FINE_WINDOW) return run_fwd<T, DH, CAUSAL, true>(p, ws, st);
+    return run_fwd<T, DH, CAUSAL, false>(p, ws, st);
+}
 template <typename T, int DH, bool CAUSAL> int run_bwd(const Slide& p, float* ws, hipStream_t st) {
     if constexpr (sizeof(T) == 2)
         if (p.window <= FINE_WINDOW) return run_bwd<T, DH, CAUSAL, true>(p, ws, st);
