@@ -419,6 +419,37 @@ def test_decode_is_off_by_the_rounding_of_its_result(B, Hq, Hkv, dh, cap, window
     _near("o", o, want, 1.1 * float((want.to(BF).double() - want).norm() / want.norm()))
 
 
+# ----------------------------------------------------------------------------- many bands
+# Bands of 128 keys want 512 of them; with 1024 bands one item does first tokens of up to 96 tiles.  (B, N, Hq, Hkv, dh, causal, window,
+# sinks): the last two rows reach 1024.
+MANY = [(16, 130, 16, 16, 64, False, 40, 1), (16, 130, 16, 16, 32, True, 20, 0), (8, 150, 64, 32, 64, False, 9, 3), (13, 257, 14, 14, 128, False, 70, 5),
+        (16, 200, 32, 16, 64, True, 200, 0), (8, 2305, 12, 12, 64, False, 145, 1), (16, 385, 64, 16, 32, False, 12, 40)]
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("B,N,Hq,Hkv,dh,causal,window,sinks", MANY)
+def test_attention_of_many_heads(B, N, Hq, Hkv, dh, causal, window, sinks, dt):
+    """Some heads of a launch with many: first, last and in between, each with its neighbours' memory around it."""
+    from vitk import ops
+    G = Hq // Hkv
+    g = torch.Generator(device=DEV).manual_seed(N)
+    q, k, v, d_o = (torch.randn(B, N, h, dh, device=DEV, generator=g).to(dt) for h in (Hq, Hkv, Hkv, Hq))
+    n = torch.full((B,), N, dtype=torch.int32, device=DEV)
+    n[B // 2] = N - 77
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    o = ops.sliding_attention(*leaves, window, sinks=sinks, causal=causal, lengths=n)
+    got = (o, *torch.autograd.grad(o, leaves, d_o))
+    for b, h in ((0, 0), (B // 2, Hkv // 2), (B - 1, Hkv - 1)):
+        qs, ks = slice(h * G, (h + 1) * G), slice(h, h + 1)
+        at = [t.detach()[b:b + 1, :, s].cpu() for t, s in ((q, qs), (k, ks), (v, ks), (d_o, qs))]
+        want = SO.sliding_attention(*at[:3], window, sinks, causal, (int(n[b]),), dh ** -0.5, R[dt], at[3])
+        for name, t, s in zip(("o", "dq", "dk", "dv"), got, (qs, qs, ks, ks)):
+            _hold(f"{name} {b} {h}", t[b:b + 1, :, s], *want[name])
+            if dt == BF:
+                _near(f"{name} {b} {h}", t[b:b + 1, :, s], want[name][0], TWICE)
+    assert all(not t[B // 2, N - 77:].any() for t in got)
+
+
 # ----------------------------------------------------------------------------- short windows
 @pytest.mark.parametrize("N,Hq,Hkv,dh,causal,window,sinks", [(700, 4, 2, 64, False, 9, 0), (700, 2, 2, 128, True, 16, 0), (1700, 2, 2, 64, False, 16, 3),
                                                              (500, 4, 4, 32, True, 3, 2)])
