@@ -464,3 +464,20 @@ def test_short_windows_are_off_by_the_rounding_of_their_results(N, Hq, Hkv, dh, 
     for name, got in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, leaves, d_o.to(DEV)))):
         val = want[name][0]
         _near(name, got, val, (1 + math.sqrt(2.0)) / 2 * float((val.to(BF).double() - val).norm() / val.norm()))
+
+
+def test_decode_reads_a_cache_of_far_apart_tokens_where_it_is():
+    """Tokens outermost, with room between them: no copy of the cache, whatever the stride."""
+    from vitk import ops
+    cap, dh, apart = 40, 64, (1 << 23) + 64
+    cache = torch.zeros(cap, apart, dtype=BF, device=DEV)
+    k, v = (cache[:, at:at + dh].unflatten(1, (1, dh))[None] for at in (0, dh))
+    k.copy_(_rand(1, cap, 1, dh, dtype=BF, seed=1))
+    v.copy_(_rand(1, cap, 1, dh, dtype=BF, seed=2))
+    q, n = _rand(1, 2, dh, dtype=BF).to(DEV), torch.tensor([cap], dtype=torch.int32, device=DEV)
+    want = ops.sliding_attention_decode(q, k.contiguous(), v.contiguous(), n, 30, sinks=2)
+    assert k.stride(1) == apart
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = ops.sliding_attention_decode(q, k, v, n, 30, sinks=2)
+    assert torch.equal(got, want) and torch.cuda.max_memory_allocated() - before < 2 * k.numel()

@@ -51,11 +51,11 @@ def _no_tangents(what, *ts):
         raise VitkError(f"{what}: no forward-mode derivatives")
 
 
-def _rows(t):
+def _rows(t, apart=1 << 23):
     """`t` as the kernels address it: consecutive elements inside a head, pointer and strides multiples of 16 bytes, tokens
-    less than 2^23 elements apart."""
+    less than `apart` elements from one to the next (attention's tiles count bytes in 32 bits, a decoded cache is addressed in 64)."""
     st, unit = t.stride(), 16 // t.element_size()
-    if t.data_ptr() % 16 == 0 and st[-1] == 1 and st[1] < 1 << 23 and not any(s % unit for s in st[:-1]):
+    if t.data_ptr() % 16 == 0 and st[-1] == 1 and st[1] < apart and not any(s % unit for s in st[:-1]):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -439,7 +439,7 @@ def sliding_attention_decode(q, k_cache, v_cache, lengths, window, sinks=0, scal
     _one_device(what, q, k_cache, v_cache, lengths)
     if B == 0 or Hq == 0 or cap == 0:
         return torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    q, k, v = _rows(q), _rows(k_cache), _rows(v_cache)
+    q, k, v = (_rows(t, 1 << 62) for t in (q, k_cache, v_cache))
     with _On(q.device) as on:
         o = torch.empty((B, Hq, dh), dtype=q.dtype, device=q.device)
         splits = _splits(B, Hkv, Hq // Hkv, window, sinks, dh, q.element_size(), q.device)
