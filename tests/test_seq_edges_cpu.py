@@ -97,3 +97,17 @@ def test_adamw_copies_keep_their_settings():
         other.param_groups[0]["params"][0].grad = torch.zeros(3)
         with pytest.raises(ValueError, match="GPU"):
             other.step()
+
+
+@pytest.mark.parametrize("asked", [dict(attention_window=4), dict(rope_pairs=(8, 8)), dict(attention_window=4, rope_pairs=(8, 8))])
+@pytest.mark.parametrize("name", ["RKR", "PB", "PBG", "RKRPB", "RKRPBG", "RKRTSN"])
+def test_models_without_a_window_refuse_one(name, asked):
+    """The task-conditioned models have full attention only: a configuration that asks for more is no silent full attention."""
+    import importlib
+    from models.config import get_tiny_config
+    Attention = importlib.import_module(f"models.ViT.modeling_{name}").Attention
+    cfg = get_tiny_config()
+    cfg.transformer.update(asked)
+    args = (cfg, False) + ((0,) if "PBG" in name else ())
+    with pytest.raises(ValueError, match="|".join(asked)):
+        Attention(*args)

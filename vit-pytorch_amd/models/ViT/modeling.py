@@ -65,6 +65,13 @@ def _pair(v):
     return tuple(v) if isinstance(v, (tuple, list)) else (v, v)
 
 
+def full_attention_only(config):
+    """For the task-conditioned models, whose attention has no window and no rotary positions."""
+    asked = [k for k in ("attention_window", "rope_pairs") if config.transformer.get(k) is not None]
+    if asked:
+        raise ValueError(f"{' / '.join(asked)}: models.ViT.modeling only")
+
+
 class Attention(nn.Module):
     """Multi-head self-attention: one fused QKV GEMM, fused online-softmax attention that reads
     and writes heads in place (no transpose_for_scores copies), output projection GEMM."""

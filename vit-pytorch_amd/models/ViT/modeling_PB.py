@@ -20,6 +20,7 @@ LN_EPS = rkr.LN_EPS
 class Attention(rkr.Attention):
     def __init__(self, config, vis):
         nn.Module.__init__(self)
+        rkr.base.full_attention_only(config)
         self.vis = vis
         self.num_attention_heads = config.transformer["num_heads"]
         self.attention_head_size = int(config.hidden_size / self.num_attention_heads)

@@ -92,6 +92,7 @@ class SFG_FC(nn.Module):
 class Attention(nn.Module):
     def __init__(self, config, vis):
         super().__init__()
+        base.full_attention_only(config)
         self.vis = vis
         self.num_attention_heads = config.transformer["num_heads"]
         self.attention_head_size = int(config.hidden_size / self.num_attention_heads)

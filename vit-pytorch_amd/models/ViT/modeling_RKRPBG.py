@@ -113,6 +113,7 @@ def _fc(config, h_in, h_out, task):
 class Attention(rkr.Attention):
     def __init__(self, config, vis, task):
         nn.Module.__init__(self)
+        base.full_attention_only(config)
         self.vis = vis
         self.num_attention_heads = config.transformer["num_heads"]
         self.attention_head_size = int(config.hidden_size / self.num_attention_heads)
