@@ -119,13 +119,14 @@ def _rope_rows(x, interleaved):
 def _meets(x, out):
     """Whether a write to `out` may land on elements of `x` other than the one it comes from, which another workgroup may not have
     read yet.  Both have the same shape; a layout too tangled to tell counts as one that meets."""
-    if any(n == 0 for n in x.shape):
+    B, N, H, dh = x.shape
+    (a, b, c, d), (e, f, g, h) = x.stride(), out.stride()
+    at = (out.data_ptr() - x.data_ptr()) // x.element_size()
+    if (at > (B - 1) * a + (N - 1) * b + (H - 1) * c + (dh - 1) * d or -at > (B - 1) * e + (N - 1) * f + (H - 1) * g + (dh - 1) * h
+            or x.numel() == 0):
         return False
     st = [0 if n == 1 else s for s, n in zip(x.stride(), x.shape)]
     to = [0 if n == 1 else s for s, n in zip(out.stride(), x.shape)]
-    at = (out.data_ptr() - x.data_ptr()) // x.element_size()
-    if at >= 1 + sum((n - 1) * s for n, s in zip(x.shape, st)) or -at >= 1 + sum((n - 1) * s for n, s in zip(x.shape, to)):
-        return False
     if st != to:
         return True
     dims = sorted(((s, n) for s, n in zip(st, x.shape) if n > 1), reverse=True)
