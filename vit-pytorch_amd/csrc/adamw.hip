@@ -4,9 +4,9 @@
 //   m = b1 m + (1 - b1) g';  v = b2 v + (1 - b2) g'^2;  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // HBM-bound: 4 bytes of every parameter for the norm, then 28 (states in 32 bits) or 16 + 16/256 (in 8), which leaves the
-// 8-bit update about 90 vector instructions an element before it is bound by those instead.  A large copy reaches 4.9 TB/s;
-// 87 million parameters in 32 bits: norm 98 us (3.5 TB/s), update 441 us (5.5 TB/s); 304 million in 8 bits: norm 236 us (5.2 TB/s),
-// update 991 us (4.9 TB/s).
+// 8-bit update about 90 vector instructions an element before it is bound by those instead.  A large copy reaches 5.0 TB/s;
+// 87 million parameters in 32 bits: norm 99 us (3.5 TB/s), update 440 us (5.5 TB/s); 304 million in 8 bits: norm 236 us (5.2 TB/s),
+// update 1005 us (4.8 TB/s), each launch by itself.
 //
 // States in 8 bits are e4m3 codes in units of a scale that 256 consecutive elements share (largest value / 448); the
 // second moment is held as its root, which halves the range that the code has to span.  A code's neighbours are 1/16 to

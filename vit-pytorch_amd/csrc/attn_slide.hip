@@ -20,14 +20,15 @@
 // Bands and chunks of a first token leave 32-bit records in a workspace, which a last small launch adds in a fixed order; so do the
 // workgroups that share a band of keys in the backward pass of few key heads.
 // Where the whole sequence is not much longer than a band, one item does all of 32 first tokens and nothing is left to add.
-// (Without the split the backward pass of 16384 causal tokens of the sizes below takes 663 us instead of 281.)
+// (Without the split the backward pass of 16384 causal tokens of the sizes below takes 659 us instead of 276.)
 //
-// Measured in bf16, training, rates of the pairs that are visible (4 dh operations each forward, 6 for dQ, 8 for dK / dV):
-//   8 x 2305 x 12 x 64, all visible:            forward 191 us (683 TFLOP/s), dQ 230 (850), dK / dV 320 (815)
-//   1 x 16384 x 8 of 2 x 128, causal, window 1024:     89 us (747),               113 (880),          185 (720)
-//   8 x 2305 x 12 x 64, window 145, 1 first token:     55 us (288),                77 (308),          113 (280)
-// In the last, whose band is little longer than its rows, 127 MB forward and 353 MB backward are 0.4 of the time at the rate of a
-// copy.
+// Measured in bf16, training, replayed from graphs, rates of the pairs that are visible (4 dh operations each forward, 6 for dQ, 8 for
+// dK / dV, whose time is what they add to a backward pass):
+//   8 x 2305 x 12 x 64, all visible:            forward 184 us (711 TFLOP/s), dQ 228 (860), dK / dV 298 (877)
+//   1 x 16384 x 8 of 2 x 128, causal, window 1024:     87 us (766),               112 (895),          164 (815)
+//   8 x 2305 x 12 x 64, window 145, 1 first token:     52 us (310),                64 (372),           78 (407)
+// In the last, whose band is little longer than its rows, 127 MB forward and 353 MB backward are half of the time at the rate of a
+// copy.  Every such time below is of the same run: of whole launches back to back, replayed.
 #include <initializer_list>
 
 #include "common.h"
@@ -162,9 +163,9 @@ template <bool CAUSAL> __device__ __forceinline__ Tiles query_tiles(int ka, int 
 template <typename T, int DH> struct Shape {
     static constexpr int ROW = DH * (int)sizeof(T);
     static constexpr int CHUNKS = ROW / 16;
-    // Rows of a staged tile.  In fp32, 64 rows of a head of 32 (4 sequences of 4099 causal tokens, backward: 381 us with 32 rows, 338 us),
-    // but 32 of a head of 64, whose tiles of 64 would leave two workgroups a CU (the same: 702 and 663 us; 8 images of 2305
-    // tokens: 974 and 1016 us).
+    // Rows of a staged tile.  In fp32, 64 rows of a head of 32 (4 x 4099 causal tokens, 16 heads of 8, window 512, backward: 605 us, with 32 rows
+    // 640), but 32 of a head of 64, whose tiles of 64 would leave two workgroups a CU (8 images of 2305 tokens: 977 us, with 64 rows 1017; the
+    // causal tokens 1280 and 1222).
     static constexpr int KT = ROW <= 128 || sizeof(T) == 2 ? 64 : 32;
     static constexpr int PER = ROW >= 256 ? 1 : 256 / ROW;        // rows in 64 banks
     static __device__ __forceinline__ int mix(int r) {
@@ -383,14 +384,14 @@ __device__ __forceinline__ void wave_lds_fence() {
 // this wave has read of the tile has to have arrived before the next one is asked for.
 __device__ __forceinline__ void wave_reads_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 // What rounding x to bf16 left, in units of 1/256 of the last place: with it an output has 15 bits behind the leading one, in
-// 8 bits more of memory (o in 32 bits beside it: 16384-token training pass 383 us, so 379, and 3 bytes an element more kept).
+// 8 bits more of memory (o in 32 bits beside it would be 3 bytes an element more to write, keep and read).
 __device__ __forceinline__ int rest_of(float x) {
     const int r = (int)(__float_as_uint(x) - ((unsigned)__builtin_bit_cast(unsigned short, (bf16_t)x) << 16));
     return least((r + 128) >> 8, 127);
 }
 // The wave's 32 rows, `ld` elements apart, the first `count` of them, through its LDS tile `via`: a lane's elements of a row are 4 here
-// and 4 there, and rows written from registers cost the address units a line for each of them (8 images of 2305 tokens, what a forward pass
-// for training writes: 60.8 -> 55.2 us; backward 164 -> 160).
+// and 4 there, and rows written from registers cost the address units a line for each of them (8 images of 2305 tokens, window 145, backward: 143 us,
+// from registers 150; 16384 tokens: no difference).
 template <int DH> __device__ __forceinline__ void put_rows(char* via, bf16_t* rows, long ld, int count, const f32x16* acc, float mul, int lane) {
     using S = Shape<bf16_t, DH>;
 #pragma unroll
@@ -555,7 +556,8 @@ template <int DH, int NW, typename F> __device__ __forceinline__ void add_waves(
 
 // Tiles of two matrices through LDS, two buffers deep: while one tile is used, the next one is on its way, and one
 // barrier a tile orders the two.  use(first tile, second tile, first row); ready() waits for what the loop keeps with the first
-// tiles on their way.  Returns the buffer that no wave reads any more (forward, 1024 tokens of 8 heads: 15.9 -> 15.1 us; in the backward kernels it gained nothing).
+// tiles on their way, which gains a little in the forward pass and nothing in the backward kernels.  Returns the buffer that no wave reads
+// any more.
 template <typename T, int DH, typename R, typename F>
 __device__ __forceinline__ char* stream(char* lds, const T* A, long lda, const T* B, long ldb, const Tiles& tl, int n, int tid, R ready, F use) {
     using S = Shape<T, DH>;
@@ -604,9 +606,8 @@ __device__ __forceinline__ void write_row(const Slide& p, int b, int h, int i, i
 }
 // Band: 128 queries of one (sequence, head), each wave 32 of them; key tiles stream through LDS.
 // A head of 64 is bound by vector instructions: 96 beside 8 matrix ones to a 32 x 32 tile, 16 of them exponentials at a
-// quarter of the rate (vector pipes busy 67 % of the cycles, matrix cores 38 %).  Four waves of 32 queries share each staged
-// tile; with two tiles in LDS at once and the copies behind the barrier the loop does not wait for memory (single
-// buffers: 104 us where two took 70).
+// quarter of the rate (all visible: vector pipes busy 75 % of the cycles, matrix cores 42 %; window 145: 67 and 23 %).  Four waves of 32
+// queries share each staged tile; with two tiles in LDS at once and the copies behind the barrier the loop does not wait for memory.
 template <typename T, int DH, bool CAUSAL, bool FINE>
 __device__ __forceinline__ void fwd_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
@@ -811,7 +812,8 @@ template <typename T, int DH> __global__ __launch_bounds__(256) void slide_delta
 }
 
 // dQ of a band: as the forward pass, with a second product of the same shape for dP and the deltas on the way (a kernel of its
-// own for them cost 20 us of the 250 of a training pass).  Matrix cores busy 51 % of the cycles, vector pipes 61 %.
+// own for them takes 18 us, beside 143 of the whole backward pass of 8 images of window 145).  All visible: matrix cores busy 51 % of the
+// cycles, vector pipes 62 %.
 template <typename T, int DH, bool CAUSAL, bool FINE>
 __device__ __forceinline__ void dq_band(const Slide& p, char* lds, int q0, int h, int b, int n) {
     using S = Shape<T, DH>;
@@ -934,8 +936,9 @@ __device__ __forceinline__ void dkv_tile(const char* Qs, const char* Os, const f
 // How a workgroup of the dK / dV kernel is laid out: NW waves, 32 KG keys; wave w keeps keys 32 (w % KG) and takes every
 // (NW / KG)-th 32 queries, and the parts are added at the end.  Four waves of 32 keys each where there are enough of them;
 // bands of 64 keys where heads are few; and for bf16 heads of 128, whose four operands and sums of a wave leave room for
-// one wave a SIMD only, eight waves with K and V in LDS, two to a SIMD (16384 causal tokens, 2 key heads, window 1024: 249 us with
-// four waves, 187 us, which is 711 TFLOP/s).
+// one wave a SIMD only, eight waves with K and V in LDS, two to a SIMD (16384 causal tokens, 2 key heads, window 1024: 164 us, with four
+// waves 208).  Without a causal mask the eight waves' kernel keeps 13 registers of a lane in scratch memory and four waves would do (4 x 2305 x
+// 8 heads, window 145: 85 us and 75).
 template <typename T, int DH, int NW, int KG> struct Layout {
     using S = Shape<T, DH>;
     static constexpr bool IN_LDS = NW == 8;
@@ -962,7 +965,7 @@ template <typename T, int DH, int NT> __device__ __forceinline__ void keep_rows(
     }
 }
 // Band: the queries of every head that shares the keys stream through LDS, so that dK and dV are sums of one workgroup and need no
-// atomics.  Matrix cores busy 47 % of the cycles, vector pipes 41 %, LDS 36 %: four products read a tile in two
+// atomics.  All visible, heads of 64: matrix cores busy 48 % of the cycles, vector pipes 42 %, LDS 37 %: four products read a tile in two
 // orders, and the registers of two sums leave two waves a SIMD to hide one in the other.
 template <typename T, int DH, bool CAUSAL, int NW, int KG, bool FINE>
 __device__ __forceinline__ void dkv_band(const Slide& p, char* lds, int k0, int share, int hk, int b, int n) {
@@ -1189,7 +1192,7 @@ struct Decode {
     float scale;
 };
 // The heads that share a key head are the 32 MFMA columns.  Memory-bound, 5.9 TB/s with 32 streams of 8192 keys (8 key heads of 128:
-// 183 us; a large copy reaches 4.9, which writes as much as it reads): each of NW waves stages its own 32 keys at a time (no
+// 184 us; a large copy reaches 5.0, which writes as much as it reads, a library's sum 4.0): each of NW waves stages its own 32 keys at a time (no
 // barrier in the loop) and keeps a softmax of its own; the waves are joined through LDS, the splits through the workspace:
 // [B, Hq, splits] records of DH sums, a maximum (scaled, base 2) and a sum.
 // Probabilities go into their product as two bf16 numbers each, since matrix cores wait for memory here: an output is off by its own
@@ -1265,10 +1268,10 @@ constexpr int dkv_waves(bool bf16, int dh) { return bf16 && dh == 128 ? 8 : 4; }
 // Items of the first tokens: rows (a multiple of 32; 0: none needed), chunks of far items for each 32 of them, floats of
 // workspace for their records.  One item for all (no records, no second launch) while it ends before the bands do, which
 // its turns, of a microsecond or so each, decide: up to 24 of its waves where there are four bands a CU and more (2305 tokens,
-// 8 sequences of 12 heads: forward 53 us, with chunks 63; backward 163, with chunks 172), up to 12 with fewer bands (577
-// tokens, 6 of 8 heads: backward 34 us, with chunks 37; 2305 tokens, one of 12 heads: 55 us, with chunks 38; 16384 causal
-// tokens, 2 key heads of 4 queries each: 663 us, with chunks 286).  Else a chunk gives each of its waves about 4 far tiles (that
-// backward: 2 tiles 299 us, 4 286, 8 291), and fewer chunks do where there are items enough without them.
+// 8 sequences of 12 heads: forward 52 us, with chunks 57; backward 143, with chunks 156), up to 12 with fewer bands (577
+// tokens, 6 of 8 heads: backward 36 us, with chunks 39; 2305 tokens, one of 12 heads: 57 us, with chunks 38, and four, just below the
+// border: 83 and 94; 16384 causal tokens, 2 key heads of 4 queries each: 659 us, with chunks 276).  Else a chunk gives each of its
+// waves about 4 far tiles (that backward: 2 tiles 281 us, 4 276, 8 282), and fewer chunks do where there are items enough without them.
 struct Records { int rows, chunks; long floats; };
 Records records_of(int B, int N, int heads, int G, int width, int window, int sinks, int waves) {
     Records r{0, 0, 0};
@@ -1285,10 +1288,10 @@ Records records_of(int B, int N, int heads, int G, int width, int window, int si
     return r;
 }
 // Bands of the dK / dV kernel: 32 `groups` keys, `shares` workgroups each, floats of workspace for their records.  Bands of 64
-// keys where there are fewer than two of 128 for each CU (577 tokens, 6 of 4 key heads: 22 us, bands of 128 26 us; at 750 bands
-// 50 us against 41), and then as many shares as it takes to fill the chip, of 8 turns and more, behind which the records
-// are added (4096 causal tokens, 2 key heads of 4 queries each, 128 elements: 139 us unsplit, 76 us; 1024 tokens of 64: 48 us and 23 us,
-// and with shares of 2 turns 29 us).
+// keys where there are fewer than two of 128 for each CU (577 tokens, 6 of 4 key heads: 23 us, bands of 128 28; 25 of 6, which is 750 bands:
+// 80 us, bands of 128 66), and then as many shares as it takes to fill the chip, of 8 turns and more, behind which the records
+// are added (4096 causal tokens, 2 key heads of 4 queries each, 128 elements, window 1024: 65 us, unsplit 135; 1024 tokens of 64: 21 us and 63,
+// with shares of 2 turns 24; the 577 tokens with shares of 2 turns 37).  Times with the deltas' kernel.
 struct Bands { int groups, shares; long floats; };
 Bands bands_of(int B, int N, int Hkv, int G, bool causal, int window, bool bf16, int dh) {
     Bands r{4, 1, 0};
@@ -1375,7 +1378,7 @@ template <typename T, int DH, bool CAUSAL, bool FINE> int run_bwd(Slide p, float
     const int first = rk.rows < p.N ? rk.rows : p.N;
     const int keys = !p.dk ? 0 : (bands.shares > 1 ? p.N : rk.chunks ? first : 0) * p.Hkv, queries = p.dq && rq.chunks ? first * p.Hq : 0;
     if (keys + queries) {
-        // many records of few rows are added by 1024 threads (64 chunks: 5.3 us, with 256 threads 11.7; 16 chunks: no gain)
+        // many records of few rows are added by 1024 threads (16384 tokens, 64 chunks: backward 276 us, with 256 threads 282)
         if (bands.shares == 1 && (rk.chunks >= 32 || rq.chunks >= 32))
             hipLaunchKernelGGL((slide_bwd_join_kernel<T, DH, 1024>), dim3(keys + queries, p.B), dim3(1024), 0, st, p, keys, rk.rows, rk.chunks, rq.chunks);
         else

@@ -397,8 +397,8 @@ _CUS = {}         # compute units of each device
 
 def _splits(B, Hkv, G, window, sinks, dh, esz, device):
     """Workgroups that share the keys of one (sequence, key head): as many as give each CU one in all, none with fewer than 32
-    keys a wave.  One stream of 65536 tokens, 8 key heads of 128: 488 us unsplit, 51 us with 32 each; 12 heads of 64, 16384
-    tokens: 97 us unsplit, 16.7 us with 21 each, 19.4 with 22, which is more than there are CUs.
+    keys a wave.  One stream of 65536 tokens, 8 key heads of 4 x 128: 575 us unsplit, 50 us with 32 each; 12 heads of 64, 16384
+    tokens: 111 us unsplit, 18.5 us with 21 each, 21.8 with 22, which is more than there are CUs.
     One workgroup alone while its waves have no more than 24 KB of keys each: shared, the kernels are faster, but a second launch
     costs an eager call 4 us of host time.  Microseconds alone and shared, eager | replayed from a graph, by KB a wave:
       12 heads of 64, bf16    8: 12.7 16.8 | 5.1 6.6    20: 12.7 17.0 | 8.9 6.8    24: 12.6 16.9 | 11.4 6.8   32: 14.5 17.0 | 14.3 7.1
