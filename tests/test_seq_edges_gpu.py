@@ -117,6 +117,21 @@ def test_a_run_of_nan_keys_is_not_dropped(N, bad, dt):
 
 
 @pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("N,bad,clean", [(1700, slice(1600, 1601), slice(3, 1499)), (1700, slice(300, 1700), slice(3, 199)), (1700, slice(1500, 1501), slice(1602, 1700)),
+                                         (500, slice(300, 301), slice(32, 199)), (500, slice(300, 301), slice(402, 500))])
+def test_a_nan_in_v_stays_near_those_that_look_at_it(N, bad, clean, dt):
+    """Queries further than 62 tokens (31 of a tile of keys and 31 of one of queries) from one that looks at it are clean; in long
+    sequences, where chunks are records of their own, those beside a first token too."""
+    from vitk import ops
+    q, k, v = (_rand(1, N, 1, 64, dtype=dt, seed=s) for s in range(3))
+    want = SO.sliding_attention(q, k, v, 40, 3, False, None, 0.125, R[dt])["o"]
+    v[:, bad] = math.nan
+    o = ops.sliding_attention(q.to(DEV), k.to(DEV), v.to(DEV), 40, sinks=3).cpu()
+    assert o[0, _pairs(N, 40, 3, False)[:, bad].any(1)].isnan().all()
+    _hold("o", o[:, clean], want[0][:, clean], want[1][:, clean])
+
+
+@pytest.mark.parametrize("dt", [FP, BF], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("causal", [True, False])
 def test_infinite_keys(dt, causal):
     """A score of minus infinity is a weight of 0, one of plus infinity leaves no number."""

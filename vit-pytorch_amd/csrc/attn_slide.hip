@@ -504,8 +504,10 @@ __device__ __forceinline__ Item item_of(const Slide& p, int heads, int tiles) {
     return it;
 }
 // The factor of a record whose maximum is m, towards the common maximum.  Where both are -inf its sums are 0, or NaN if all
-// that it looked at was: either way they stay what they are.
+// that it looked at was: either way they stay what they are.  A record with a total of exactly 0 saw nothing: whatever its sums are (0
+// times a NaN in v that another row of the item looked at), they do not count.
 __device__ __forceinline__ float weight_of(float m, float top) { return m == top ? 1.f : __builtin_amdgcn_exp2f(m - top); }
+__device__ __forceinline__ float counted(float x, float total, float weight) { return total == 0.f ? 0.f : x * weight; }
 // A row's result from its sums; a total of exactly 0 is a row that sees nothing (a NaN is not).
 __device__ __forceinline__ float share_of(float sum, float total) { return total == 0.f ? 0.f : sum / total; }
 // Sums of the waves, [32 columns][DH + 4] each, in LDS.
@@ -531,7 +533,7 @@ template <int DH, int NW, typename F> __device__ __forceinline__ void join_waves
         for (int w = 0; w < NW; ++w) {
             const float* rec = out + (w * 32 + c) * W;
             const float e = weight_of(rec[DH], top);
-            x += rec[d] * e;
+            x += counted(rec[d], rec[DH + 1], e);
             sum += rec[DH + 1] * e;
         }
         f(c, d, x, top, sum);
@@ -740,7 +742,7 @@ template <int DH> __device__ __forceinline__ Joined<DH> join_records(const float
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float e = weight_of(m[u], t);
-            j.x += v[u] * e;
+            j.x += counted(v[u], l[u], e);
             j.sum += l[u] * e;
         }
         j.top = t;

@@ -313,7 +313,8 @@ def sliding_attention(q, k, v, window, sinks=0, causal=False, lengths=None, scal
     such as a class token see everything).  ``window`` None: no limit.  ``lengths`` int32 [B] on the same device: how many tokens
     of each sequence there are; tokens behind it may hold anything, their outputs and gradients are 0, as are those of
     a query that sees nothing.  A query that looks at a NaN, or at an infinity whose score is no number or plus infinity, gives NaN, and
-    so does its gradient (one in v, or in a gradient, may reach queries and keys up to 63 tokens beyond as well).  Returns [B, N, Hq, dh]."""
+    so does its gradient (one in v, or in a gradient, may also reach those up to 62 tokens beyond, and of the same 32 as a first token).
+    Returns [B, N, Hq, dh]."""
     what = "sliding_attention"
     if q.dim() != 4:
         raise VitkError(f"{what}: q is [batch, tokens, heads, head size], got {tuple(q.shape)}")
